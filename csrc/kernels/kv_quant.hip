@@ -1,0 +1,344 @@
+// Writing the 8-bit paged KV cache (kv_quant.h) and reading it back.
+#include "kv_quant.h"
+
+namespace xgk {
+
+// ---- append ------------------------------------------------------------------------------------------------------------
+// A wave takes a window of four tokens of one head: 16 lanes a row, D / 16 numbers a lane, K and V in turn. A row's largest
+// magnitude joins over its 16 lanes by register rotations; nothing goes through memory but the row itself (2 D bytes in,
+// D + 4 out: bound by HBM for long steps, by one trip to memory and the launch for single tokens).
+//
+// Codes as the mathematics has them: with bf16 x and a, the distance of 127 x / a (448 x / a) from the border of two codes
+// is 0 or at least 2^-16 of it, so x (127 / a), off by less than 2^-22, rounded to 20 bits is on the border exactly when
+// the quotient is, and rounds to even there.
+//
+// V's order puts four tokens' codes of a dim into one word: a window whose slots fill such a quad (tokens of a prompt)
+// exchanges its codes within the wave and writes words; other tokens write bytes.
+struct KvAppend {
+  uint16_t* q;                 // ROPE: query heads, rotated in place (row stride as k)
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_stride, v_stride;  // elements between tokens
+  const int32_t* slots;        // slot of each token; outside [0, num_slots): not written
+  const int32_t* positions;    // ROPE
+  const float* cos_sin;        // ROPE: [max_pos, D]
+  uint8_t* kc;
+  uint8_t* vc;
+  float* scales;
+  int64_t num_slots;
+  int T, Hq, Hkv, bs;
+};
+
+template <int N>
+struct Codes { uint32_t w[N / 4]; };
+
+// codes of this lane's D / 16 numbers of a row that 16 lanes hold, and the row's scale
+template <int FMT, int N>
+__device__ __forceinline__ Codes<N> kv_quantise(const uint16_t (&x)[N], float& scale) {
+  constexpr float LARGEST = FMT == KV_FP8 ? 448.f : 127.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = max(top, static_cast<uint32_t>(x[i] & 0x7FFF));
+  // (magnitudes of bf16 order as whole numbers do, NaN above infinity; as floats of the same bits they do too)
+  float m = __uint_as_float(top);
+  auto join = [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); };
+  m = join(m, row_ror<8>(m));
+  m = join(m, row_ror<4>(m));
+  m = join(m, row_ror<2>(m));
+  m = join(m, row_ror<1>(m));
+  top = __float_as_uint(m);
+  const float a = __uint_as_float(top << 16);
+  const bool usable = top < 0x7F80u && top != 0;
+  scale = usable ? a / LARGEST : (top == 0 ? 0.f : __uint_as_float(0x7FC00000u));
+  const float lift = a < 0x1p-90f ? 0x1p60f : 1.f;  // 448 / a has to be a float
+  const float inv = usable ? LARGEST / (a * lift) : 0.f;
+  float y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = usable ? bf2f(x[i]) * lift * inv : 0.f;
+    y[i] = __uint_as_float((__float_as_uint(f) + 8u) & ~15u);
+  }
+  Codes<N> c;
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (FMT == KV_FP8) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j], y[4 * j + 1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j + 2], y[4 * j + 3], w, true);
+      c.w[j] = static_cast<uint32_t>(w);
+    } else {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w |= (static_cast<uint32_t>(static_cast<int>(rintf(y[4 * j + i]))) & 0xFFu) << (8 * i);
+      c.w[j] = w;
+    }
+#else
+    c.w[j] = 0;
+#endif
+  }
+  return c;
+}
+
+template <int N>
+__device__ __forceinline__ void kv_load_row(const uint16_t* p, uint16_t (&x)[N]) {
+  if constexpr (N == 8) {
+    const uint4 v = ld16(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = w[i] & 0xFFFF; x[2 * i + 1] = w[i] >> 16; }
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = v.x & 0xFFFF; x[1] = v.x >> 16; x[2] = v.y & 0xFFFF; x[3] = v.y >> 16;
+  }
+}
+
+// rotate_half of a row that 16 lanes hold: lane c's partner is c ^ 8 (D / 2 numbers on)
+template <int N>
+__device__ __forceinline__ void kv_rotate(uint16_t (&x)[N], const float* cs, int c) {
+  const float* cp = cs + (c & 7) * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = bf2f(x[i]), o = row_ror<8>(f);
+    const float co = cp[i], si = cp[8 * N + i];
+    x[i] = f2bf(c < 8 ? f * co - o * si : f * co + o * si);
+  }
+}
+
+template <int FMT, int D, bool ROPE>
+__global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
+  constexpr int N = D / 16;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = (blockIdx.x * 4 + wid) * 4, head = blockIdx.y;
+  const int i = lane >> 4, c = lane & 15;
+  if (t0 >= p.T) return;
+  if (ROPE && head >= p.Hkv) {   // a query head, rotated in place
+    const int t = t0 + i;
+    if (t < p.T) {
+      uint16_t* row = p.q + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head - p.Hkv) * D + c * N;
+      uint16_t x[N];
+      kv_load_row<N>(row, x);
+      kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j)
+        *reinterpret_cast<uint2*>(row + 4 * j) = make_uint2(x[4 * j] | (static_cast<uint32_t>(x[4 * j + 1]) << 16),
+                                                            x[4 * j + 2] | (static_cast<uint32_t>(x[4 * j + 3]) << 16));
+    }
+    return;
+  }
+  // slots of the tokens around the window, -1 where there is none
+  int s[10];
+#pragma unroll
+  for (int j = 0; j < 10; ++j) {
+    const int t = t0 - 3 + j;
+    const int v = p.slots[min(max(t, 0), p.T - 1)];
+    s[j] = t >= 0 && t < p.T && static_cast<int64_t>(v) < p.num_slots ? v : -1;
+  }
+  // the quad that begins in this window, and this window's tokens that no quad takes
+  int quad = -1;
+  uint32_t taken = 0;
+#pragma unroll
+  for (int b = 0; b < 7; ++b)
+    if (s[b] >= 0 && (s[b] & 3) == 0 && s[b + 1] == s[b] + 1 && s[b + 2] == s[b] + 2 && s[b + 3] == s[b] + 3) {
+      if (b >= 3) quad = t0 - 3 + b;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (b + j >= 3 && b + j < 7) taken |= 1u << (b + j - 3);
+    }
+  auto row_of = [&](int t, bool value, uint16_t (&x)[N]) {
+    const uint16_t* src = value ? p.v + static_cast<int64_t>(t) * p.v_stride : p.k + static_cast<int64_t>(t) * p.k_stride;
+    kv_load_row<N>(src + static_cast<int64_t>(head) * D + c * N, x);
+    if (ROPE && !value) kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
+  };
+  auto tile_of = [&](int slot, int64_t& scale_at) {
+    const int64_t page = slot / p.bs;
+    const int off = slot % p.bs;
+    scale_at = (page * p.Hkv + head) * 2 * p.bs + off;
+    return ((page * p.Hkv + head) * p.bs + (off & ~15)) * D;
+  };
+  auto put_k = [&](const Codes<N>& w, int slot, int64_t tile) {
+    uint8_t* dst = p.kc + tile + kv_k_byte(slot % p.bs & 15, c * N);
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w.w[0], w.w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w.w[0];
+  };
+  if (quad >= 0) {
+    const int slot = p.slots[quad] + i;
+    int64_t at;
+    const int64_t tile = tile_of(slot, at);
+    uint16_t xk[N], xv[N];
+    row_of(quad + i, false, xk);
+    row_of(quad + i, true, xv);
+    float sk, sv;
+    put_k(kv_quantise<FMT, N>(xk, sk), slot, tile);
+    const Codes<N> w = kv_quantise<FMT, N>(xv, sv);
+    if (c == 0) {
+      p.scales[at] = sk;
+      p.scales[at + p.bs] = sv;
+    }
+    // lane (i, c) collects its dims' codes of all four tokens: dims N c + (N / 4) i ..
+    uint32_t four[N / 4] = {};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t got[N / 4];
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) got[j] = __shfl(w.w[j], t * 16 + c, 64);
+#pragma unroll
+      for (int e = 0; e < N / 4; ++e) {
+        const int d = (N / 4) * i + e;   // of the lane's N
+        const uint32_t word = N == 8 && d >= 4 ? got[N / 4 - 1] : got[0];
+        four[e] |= ((word >> (8 * (d & 3))) & 0xFFu) << (8 * t);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N / 4; ++e)
+      *reinterpret_cast<uint32_t*>(p.vc + tile + kv_v_byte((slot % p.bs & 15) & ~3, c * N + (N / 4) * i + e)) = four[e];
+  }
+  const int slot = s[3 + 0] * (i == 0) + s[3 + 1] * (i == 1) + s[3 + 2] * (i == 2) + s[3 + 3] * (i == 3);
+  if (!(taken >> i & 1) && slot >= 0) {   // (16 lanes are of one mind: the rotations within them stay whole)
+    int64_t at;
+    const int64_t tile = tile_of(slot, at);
+    uint16_t xk[N], xv[N];
+    row_of(t0 + i, false, xk);
+    row_of(t0 + i, true, xv);
+    float sk, sv;
+    put_k(kv_quantise<FMT, N>(xk, sk), slot, tile);
+    const Codes<N> w = kv_quantise<FMT, N>(xv, sv);
+    if (c == 0) {
+      p.scales[at] = sk;
+      p.scales[at + p.bs] = sv;
+    }
+    uint8_t* dst = p.vc + tile + kv_v_byte(slot % p.bs & 15, c * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) dst[16 * e] = (w.w[e >> 2] >> (8 * (e & 3))) & 0xFF;
+  }
+}
+
+template <int FMT, int D>
+static void launch_append(const KvAppend& p, bool rope, hipStream_t st) {
+  const dim3 grid((p.T + 15) / 16, p.Hkv + (rope ? p.Hq : 0));
+  if (rope) hipLaunchKernelGGL((kv_append_kernel<FMT, D, true>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((kv_append_kernel<FMT, D, false>), grid, dim3(256), 0, st, p);
+}
+
+// positions / cos_sin null: k and v as they are; else q (Hq heads, in place) and k are rotated first.
+int kv_append(int fmt, uint16_t* q, const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
+              const int32_t* slots, const int32_t* positions, const float* cos_sin, uint8_t* kc, uint8_t* vc, float* scales,
+              int64_t num_blocks, int T, int Hq, int Hkv, int D, int bs, hipStream_t st) {
+  if (T <= 0) return 0;
+  if (bs <= 0 || bs % KV_TILE || Hkv < 1 || (D != 64 && D != 128) || k_stride % (D / 16) || v_stride % (D / 16)) return -1;
+  const bool rope = cos_sin != nullptr;
+  if (rope && (q == nullptr || positions == nullptr)) return -1;
+  const KvAppend p{q, k, v, k_stride, v_stride, slots, positions, cos_sin, kc, vc, scales, num_blocks * bs, T, Hq, Hkv, bs};
+  if (fmt == KV_FP8 && D == 128) launch_append<KV_FP8, 128>(p, rope, st);
+  else if (fmt == KV_FP8) launch_append<KV_FP8, 64>(p, rope, st);
+  else if (fmt == KV_INT8 && D == 128) launch_append<KV_INT8, 128>(p, rope, st);
+  else if (fmt == KV_INT8) launch_append<KV_INT8, 64>(p, rope, st);
+  else return -1;
+  return 0;
+}
+
+// ---- read back ---------------------------------------------------------------------------------------------------------
+// Tokens starts[s] + i, i < cu[s + 1] - cu[s], of every sequence as bf16 rows [n, Hkv, D]. A wave takes one 16-token tile of
+// one head: two (D = 128) whole 1 KiB reads of K and of V, widened, scaled and put in rows through LDS (V's codes come in
+// token quads a dim), written as 16 bytes a lane. (D + 4) bytes in and 2 D out a row: bound by HBM.
+// Tile j of the launch belongs to the last sequence s with cu[s] / 16 + 2 s <= j: n tokens that begin anywhere in a tile
+// touch at most n / 16 + 2 of them.
+template <int FMT, int D>
+__global__ void __launch_bounds__(256) kv_read_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                      const float* __restrict__ scales,
+                                                      const int32_t* __restrict__ tables, int64_t table_stride, int width,
+                                                      const int32_t* __restrict__ starts, const int32_t* __restrict__ cu,
+                                                      int S, int n, int num_blocks, int Hkv, int bs, uint16_t* __restrict__ k,
+                                                      uint16_t* __restrict__ v) {
+  constexpr int ROW = D + 8;      // LDS row, padded: 16 rows of a column fall on different banks
+  constexpr int LOADS = D / 64;
+  __shared__ __attribute__((aligned(16))) uint16_t rows[4][16 * ROW];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, li = lane & 15;
+  const int j = blockIdx.x * 4 + wid, head = blockIdx.y;
+  int lo = 0, hi = S - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] / 16 + 2 * mid <= j) lo = mid;
+    else hi = mid - 1;
+  }
+  const int first = starts[lo], out0 = cu[lo], count = min(cu[lo + 1], n) - out0;
+  const int ahead = j - (out0 / 16 + 2 * lo);
+  if (count <= 0 || first < 0 || out0 < 0 || ahead < 0) return;
+  const int tile = (first >> 4) + ahead;
+  // (tiles behind the sequence's end, or behind its table's: nothing to do)
+  if (tile * 16 >= first + count || tile >= width * (bs >> 4)) return;
+  const int page = min(max(tables[lo * table_stride + tile * 16 / bs], 0), num_blocks - 1);
+  const int off = tile * 16 % bs;
+  const int64_t ph = static_cast<int64_t>(page) * Hkv + head;
+  const int64_t base = (ph * bs + off) * D;
+  const float* sc = scales + ph * 2 * bs + off;
+  uint4 kr[LOADS], vr[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    kr[i] = ld16_nt(kc + base + i * 1024 + lane * 16);
+    vr[i] = ld16_nt(vc + base + i * 1024 + lane * 16);
+  }
+  const float ks = sc[li];
+  const float4 vs4 = *reinterpret_cast<const float4*>(sc + bs + 4 * g);
+  const float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
+  uint16_t* mine = rows[wid];
+  auto emit = [&](uint16_t* dst) {   // (a wave's own rows: its LDS writes and reads are in order)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const int ch = lane + 64 * i, t = ch / (D / 8), at = tile * 16 + t - first;
+      const uint4 w = ld16(mine + t * ROW + ch % (D / 8) * 8);
+      if (at >= 0 && at < count) st16(dst + ((static_cast<int64_t>(out0) + at) * Hkv + head) * D + ch % (D / 8) * 8, w);
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const uint32_t w[4] = {kr[i].x, kr[i].y, kr[i].z, kr[i].w};
+    uint32_t o[8];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint2 b = kv_widen4<FMT>(w[x]);
+      o[2 * x] = pack2(__uint_as_float(b.x << 16) * ks, __uint_as_float(b.x & 0xFFFF0000u) * ks);
+      o[2 * x + 1] = pack2(__uint_as_float(b.y << 16) * ks, __uint_as_float(b.y & 0xFFFF0000u) * ks);
+    }
+    uint16_t* dst = mine + li * ROW + 16 * (4 * i + g);
+    st16(dst, make_uint4(o[0], o[1], o[2], o[3]));
+    st16(dst + 8, make_uint4(o[4], o[5], o[6], o[7]));
+  }
+  emit(k);
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint2 b = kv_widen4<FMT>(w[x]);
+      const int d = 64 * i + 16 * x + li;
+      mine[(4 * g + 0) * ROW + d] = f2bf(__uint_as_float(b.x << 16) * vs[0]);
+      mine[(4 * g + 1) * ROW + d] = f2bf(__uint_as_float(b.x & 0xFFFF0000u) * vs[1]);
+      mine[(4 * g + 2) * ROW + d] = f2bf(__uint_as_float(b.y << 16) * vs[2]);
+      mine[(4 * g + 3) * ROW + d] = f2bf(__uint_as_float(b.y & 0xFFFF0000u) * vs[3]);
+    }
+  }
+  emit(v);
+}
+
+int kv_read(int fmt, const uint8_t* kc, const uint8_t* vc, const float* scales, const int32_t* tables, int64_t table_stride,
+            int width, const int32_t* starts, const int32_t* cu, int S, int n, int num_blocks, int Hkv, int D, int bs,
+            uint16_t* k, uint16_t* v, hipStream_t st) {
+  if (S <= 0 || n <= 0) return 0;
+  if (bs <= 0 || bs % KV_TILE || Hkv < 1 || num_blocks < 1 || width < 1) return -1;
+  const dim3 grid((n / 16 + 2 * S + 3) / 4, Hkv);
+#define XGK_READ(F, DD)                                                                                                  \
+  if (fmt == F && D == DD) {                                                                                             \
+    hipLaunchKernelGGL((kv_read_kernel<F, DD>), grid, dim3(256), 0, st, kc, vc, scales, tables, table_stride, width,     \
+                       starts, cu, S, n, num_blocks, Hkv, bs, k, v);                                                     \
+    return 0;                                                                                                            \
+  }
+  XGK_READ(KV_FP8, 128) XGK_READ(KV_FP8, 64) XGK_READ(KV_INT8, 128) XGK_READ(KV_INT8, 64)
+#undef XGK_READ
+  return -1;
+}
+
+}  // namespace xgk

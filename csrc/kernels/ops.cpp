@@ -62,6 +62,19 @@ int decode_attention(const uint16_t*, int64_t, const uint16_t*, const uint16_t*,
                      float*, float*, uint16_t*, int64_t, int, int, int, int, int, float, int, hipStream_t);
 int prefill_attention(const uint16_t*, int64_t, const uint16_t*, const uint16_t*, const int32_t*, int, const int32_t*,
                       const int32_t*, uint16_t*, int64_t, int, int, int, int, int, int, float, hipStream_t, int);
+int kv_append(int, uint16_t*, const uint16_t*, int64_t, const uint16_t*, int64_t, const int32_t*, const int32_t*, const float*,
+              uint8_t*, uint8_t*, float*, int64_t, int, int, int, int, int, hipStream_t);
+int kv_read(int, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t, int, const int32_t*, const int32_t*, int,
+            int, int, int, int, int, uint16_t*, uint16_t*, hipStream_t);
+int quant_decode_attention(int, const uint16_t*, int64_t, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t,
+                           int, const int32_t*, float*, float*, uint16_t*, int64_t, int, int, int, int, int, int, float, int,
+                           hipStream_t);
+int quant_prefill_attention(int, const uint16_t*, int64_t, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t,
+                            int, const int32_t*, const int32_t*, float*, float*, uint16_t*, int64_t, int, int, int, int, int,
+                            int, int, int, float, int, int, hipStream_t);
+int shared_prefix_attention(int, const uint16_t*, int64_t, const void*, const void*, const float*, const int32_t*, int64_t, int,
+                            const int32_t*, float*, float*, uint16_t*, int64_t, int, int, int, int, int, int, float,
+                            const int32_t*, int, const int32_t*, const int32_t*, int, int, int, hipStream_t);
 void argmax_logprob(const void*, int, int64_t, int, int, int32_t*, float*, hipStream_t, float* ws = nullptr,
                     int* cnt = nullptr);
 int argmax_ws_floats_per_row();
@@ -205,6 +218,49 @@ PYBIND11_MODULE(_kernels, m) {
      py::arg("D"), py::arg("bs"), py::arg("scale"), py::arg("st"), py::arg("gh") = 0);
   // ws / cnt (optional): the split-row form -- B x argmax_ws_floats_per_row() floats and B zeroed
   // ints (re-armed by every launch)
+  m.def("kv_append", [](int fmt, uintptr_t q, uintptr_t k, int64_t ks, uintptr_t v, int64_t vs, uintptr_t slots, uintptr_t pos,
+                        uintptr_t cs, uintptr_t kc, uintptr_t vc, uintptr_t scales, int64_t blocks, int T, int Hq, int Hkv, int D,
+                        int bs, uintptr_t st) {
+    check(xgk::kv_append(fmt, P<uint16_t>(q), P<const uint16_t>(k), ks, P<const uint16_t>(v), vs, P<const int32_t>(slots),
+                         P<const int32_t>(pos), P<const float>(cs), P<uint8_t>(kc), P<uint8_t>(vc), P<float>(scales), blocks, T,
+                         Hq, Hkv, D, bs, S(st)),
+          "kv_append");
+  });
+  m.def("kv_read", [](int fmt, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt, int64_t bts, int W, uintptr_t starts,
+                      uintptr_t cu, int S_, int n, int blocks, int Hkv, int D, int bs, uintptr_t k, uintptr_t v, uintptr_t st) {
+    check(xgk::kv_read(fmt, P<const uint8_t>(kc), P<const uint8_t>(vc), P<const float>(scales), P<const int32_t>(bt), bts, W,
+                       P<const int32_t>(starts), P<const int32_t>(cu), S_, n, blocks, Hkv, D, bs, P<uint16_t>(k), P<uint16_t>(v),
+                       S(st)),
+          "kv_read");
+  });
+  m.def("quant_decode_attention", [](int fmt, uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt,
+                                     int64_t bts, int W, uintptr_t sl, uintptr_t po, uintptr_t pl, uintptr_t out, int64_t os, int B,
+                                     int Hq, int Hkv, int D, int bs, int blocks, float scale, int splits, uintptr_t st) {
+    check(xgk::quant_decode_attention(fmt, P<const uint16_t>(q), qs, P<const uint8_t>(kc), P<const uint8_t>(vc),
+                                      P<const float>(scales), P<const int32_t>(bt), bts, W, P<const int32_t>(sl), P<float>(po),
+                                      P<float>(pl), P<uint16_t>(out), os, B, Hq, Hkv, D, bs, blocks, scale, splits, S(st)),
+          "quant_decode_attention");
+  });
+  m.def("quant_prefill_attention", [](int fmt, uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt,
+                                      int64_t bts, int W, uintptr_t qsl, uintptr_t sl, uintptr_t po, uintptr_t pl, uintptr_t out,
+                                      int64_t os, int T, int S_, int max_q, int Hq, int Hkv, int D, int bs, int blocks, float scale,
+                                      int rt, int splits, uintptr_t st) {
+    check(xgk::quant_prefill_attention(fmt, P<const uint16_t>(q), qs, P<const uint8_t>(kc), P<const uint8_t>(vc),
+                                       P<const float>(scales), P<const int32_t>(bt), bts, W, P<const int32_t>(qsl),
+                                       P<const int32_t>(sl), P<float>(po), P<float>(pl), P<uint16_t>(out), os, T, S_, max_q, Hq,
+                                       Hkv, D, bs, blocks, scale, rt, splits, S(st)),
+          "quant_prefill_attention");
+  });
+  m.def("shared_prefix_attention", [](int fmt, uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt,
+                                      int64_t bts, int W, uintptr_t sl, uintptr_t po, uintptr_t pl, uintptr_t out, int64_t os,
+                                      int B, int Hq, int Hkv, int D, int bs, int blocks, float scale, uintptr_t items, int n_items,
+                                      uintptr_t prefix, uintptr_t counts, int slots, int rt, int splits, uintptr_t st) {
+    check(xgk::shared_prefix_attention(fmt, P<const uint16_t>(q), qs, P<const void>(kc), P<const void>(vc), P<const float>(scales),
+                                       P<const int32_t>(bt), bts, W, P<const int32_t>(sl), P<float>(po), P<float>(pl),
+                                       P<uint16_t>(out), os, B, Hq, Hkv, D, bs, blocks, scale, P<const int32_t>(items), n_items,
+                                       P<const int32_t>(prefix), P<const int32_t>(counts), slots, rt, splits, S(st)),
+          "shared_prefix_attention");
+  });
   m.def("argmax_logprob", [](uintptr_t logits, int is_f32, int64_t stride, int B, int V, uintptr_t tok, uintptr_t lp,
                              uintptr_t st, uintptr_t ws, uintptr_t cnt) {
     xgk::argmax_logprob(P<const void>(logits), is_f32, stride, B, V, P<int32_t>(tok), P<float>(lp), S(st), P<float>(ws),

@@ -1,0 +1,602 @@
+// Attention of a block of query rows over paged keys, 8-bit (kv_quant.h) or bf16: decode, prompt portions, and the part of
+// a group of decode rows whose keys are in common (a shared prefix, read once for the group).
+//
+// The rows of one kv head are (token, query head of its G) pairs, token-major: a decode step has G rows a sequence, a
+// prompt portion G rows a token, a group of sequences with a common prefix G rows a member. A workgroup takes a block of
+// 16 RT rows and a range of keys; its four waves take 32-key tiles of the range in turn, each for all the rows:
+//   S^T[16 keys][16 rows] = K Q^T   v_mfma_f32_16x16x32_bf16; K fragments come from the cache as they lie (8-bit codes
+//     widened in registers), the key's scale joins softmax's scale afterwards: no rounding but the products' own
+//   softmax in base 2 by running maximum. The maximum is only raised (and the accumulators rescaled) when a score passes
+//     it by more than 2^8: fp32 sums and bf16 weights are relative, so weights up to 2^8 cost no precision
+//   O^T[D][16 rows] += V^T P^T      the same instruction over 32 keys. The S^T accumulators are the P^T fragment where
+//     the 8 keys of lane group g are 4 g + {0..3} of both 16-key halves; the cache holds V in that order (bf16: V is
+//     turned through LDS). V's scale joins the weight before its rounding to bf16 (2^-9, as everywhere here)
+// The waves' states join through LDS, splits of a long range through decode_join_kernel: (O / l, log2-sum-exp) in fp32.
+//
+// Waves share no tile, so the key loop has no barrier, and K / V go from HBM to registers: one tile's loads are on their
+// way while another is worked on. Rows without keys give zeros. Keys outside a row's range are never read into its result,
+// whatever the cache holds there.
+#include <type_traits>
+
+#include "kv_quant.h"
+
+namespace xgk {
+
+constexpr float RAISE = 8.f;          // in base 2
+constexpr float LOWEST = -1e30f;      // a maximum before any key: exp2(-inf - LOWEST) is 0
+
+struct RowsArgs {
+  const uint16_t* q;
+  int64_t q_stride;
+  const uint8_t* k;       // codes, or bf16 rows [num_blocks, Hkv, bs, D]
+  const uint8_t* v;
+  const float* scales;    // 8-bit
+  const int32_t* tables;
+  int64_t table_stride;
+  int width, num_blocks;
+  const int32_t* seq_lens;
+  float* part_out;        // [tokens, Hq, slots, D], slots > 1
+  float* part_lse;        // [tokens, Hq, slots]
+  uint16_t* out;
+  int64_t out_stride;
+  int Hq, Hkv, G, bs;
+  float scale;            // softmax's, in base 2
+  int slots;              // parts of a row (1: `out` is written here)
+};
+
+// what one workgroup does
+struct RowsBlock {
+  int tok0, ntok;         // tokens of its rows' list
+  int block;              // which 16 RT of the list's ntok G rows
+  int table;              // row of `tables`
+  int kbeg, kend;         // keys
+  int slot;               // of the rows' parts
+  int causal0;            // >= 0: token i sees keys < causal0 + i + 1; -1: keys < seq_lens of its own, and of kend
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_exp2f(x);
+#else
+  return x;
+#endif
+}
+
+// joined over the four lanes that hold one row: lane ^ 16, ^ 32
+template <typename F>
+__device__ __forceinline__ float join_groups(float v, F f) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+#endif
+  return v;
+}
+
+template <int FMT, int D, int RT>
+struct RowsCfg {
+  static constexpr bool WIDE = FMT == KV_BF16;
+  static constexpr int KK = D / 32;                  // matrix instructions over the head size
+  static constexpr int MT = D / 16;                  // 16-dim tiles of the output
+  static constexpr int LOADS = WIDE ? D / 32 : D / 64;   // 16-byte loads a lane, 16 tokens of K or V
+  static constexpr bool Q_LDS = RT == 4;             // registers: 64 of the rows' fragments would not fit beside the sums
+  static constexpr int OROW = D + 4;                 // row of the joining buffer (padded: banks)
+  static constexpr int JOIN = 4 * 16 * OROW * 4;     // bytes
+  static constexpr int TURN = WIDE ? 4 * 32 * D * 2 : 0;
+  static constexpr int SPACE = JOIN > TURN ? JOIN : TURN;
+};
+
+template <int FMT, int D, int RT>
+__device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space, uint16_t* q_lds,
+                                            float (*m_lds)[16 * RT], float (*l_lds)[16 * RT]) {
+  using C = RowsCfg<FMT, D, RT>;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, li = lane & 15;
+  const int nrows = w.ntok * p.G, row0 = w.block * 16 * RT;
+
+  // rows: fragments of Q, and the keys that each sees
+  int limit[RT];
+  int least = w.kend;   // every row sees the keys below
+  bf16x8_t qf[C::Q_LDS ? 1 : RT][C::KK];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + rt * 16 + li;
+    const bool real = r < nrows;
+    const int tok = real ? r / p.G : 0, head = kvh * p.G + (real ? r - tok * p.G : 0);
+    limit[rt] = 0;
+    if (real) {
+      limit[rt] = min(w.kend, w.causal0 >= 0 ? w.causal0 + tok + 1 : p.seq_lens[w.tok0 + tok]);
+      least = min(least, limit[rt]);
+    }
+    const uint16_t* qp = p.q + static_cast<int64_t>(w.tok0 + tok) * p.q_stride + static_cast<int64_t>(head) * D;
+    if constexpr (!C::Q_LDS) {
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk) {
+        // the dims of this lane's K fragment kk
+        const int d = C::WIDE ? 32 * kk + 8 * g : 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
+        qf[rt][kk] = as_frag(real ? ld16(qp + d) : make_uint4(0, 0, 0, 0));
+      }
+    } else if (rt == wid) {   // (wave rt brings row tile rt: RT is 4)
+#pragma unroll
+      for (int kk = 0; kk < C::KK; ++kk) {
+        const int d = C::WIDE ? 32 * kk + 8 * g : 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
+        st16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8, real ? ld16(qp + d) : make_uint4(0, 0, 0, 0));
+      }
+    }
+  }
+  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
+  if constexpr (C::Q_LDS) __syncthreads();
+
+  float m[RT], l[RT];
+  f32x4_t acc[RT][C::MT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = LOWEST;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < C::MT; ++mt) acc[rt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int tpp = p.bs >> 4;                       // tiles a page
+  const int t_end = (w.kend + 31) >> 5, last = (w.kend + 15) / 16 - 1;
+  const int32_t* table = p.tables + w.table * p.table_stride;
+  uint4 kr[2][C::LOADS], vr[2][C::LOADS];
+  float4 ks[2], vs[2];
+  // half a tile's address: clamped to the last tile that holds a key, and into the cache
+  auto place = [&](int t, int a) {
+    const int tile = min(2 * t + a, last);
+    const int pg = tile / tpp;
+    const int page = min(max(table[pg], 0), p.num_blocks - 1);
+    return make_int2(page, (tile - pg * tpp) * 16);
+  };
+  auto load_k = [&](int t) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int2 at = place(t, a);
+      const int64_t ph = static_cast<int64_t>(at.x) * p.Hkv + kvh;
+      if constexpr (C::WIDE) {
+        const uint16_t* base = reinterpret_cast<const uint16_t*>(p.k) + (ph * p.bs + at.y + li) * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = ld16_nt(base + 32 * i);
+      } else {
+        const uint8_t* base = p.k + (ph * p.bs + at.y) * D + lane * 16;
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = ld16_nt(base + 1024 * i);
+        ks[a] = *reinterpret_cast<const float4*>(p.scales + ph * 2 * p.bs + at.y + 4 * g);
+      }
+    }
+  };
+  auto load_v = [&](int t) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int2 at = place(t, a);
+      const int64_t ph = static_cast<int64_t>(at.x) * p.Hkv + kvh;
+      if constexpr (C::WIDE) {
+        const uint16_t* base = reinterpret_cast<const uint16_t*>(p.v) + (ph * p.bs + at.y) * D + lane * 8;
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = ld16_nt(base + 512 * i);   // 4 (D 128) or 8 whole rows a load
+      } else {
+        const uint8_t* base = p.v + (ph * p.bs + at.y) * D + lane * 16;
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = ld16_nt(base + 1024 * i);
+        vs[a] = *reinterpret_cast<const float4*>(p.scales + ph * 2 * p.bs + p.bs + at.y + 4 * g);
+      }
+    }
+  };
+
+  auto work = [&](int t, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    f32x4_t s[2][RT];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[a][rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < C::LOADS; ++i) {
+        bf16x8_t kf[C::WIDE ? 1 : 2];
+        if constexpr (C::WIDE) {
+          kf[0] = as_frag(kr[a][i]);
+        } else {
+          kf[0] = kv_widen8<FMT>(kr[a][i].x, kr[a][i].y);
+          kf[1] = kv_widen8<FMT>(kr[a][i].z, kr[a][i].w);
+        }
+#pragma unroll
+        for (int x = 0; x < (C::WIDE ? 1 : 2); ++x) {
+          const int kk = C::WIDE ? i : 2 * i + x;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const bf16x8_t qx = C::Q_LDS ? as_frag(ld16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8)) : qf[C::Q_LDS ? 0 : rt][kk];
+            s[a][rt] = mfma16x16x32(kf[x], qx, s[a][rt]);
+          }
+        }
+      }
+    }
+    float kf[2][4];
+    bool in[2][4];      // a key of the range: its V (and scale) may be used
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const float f[4] = {ks[a].x, ks[a].y, ks[a].z, ks[a].w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        kf[a][r] = C::WIDE ? p.scale : f[r] * p.scale;
+        const int key = 32 * t + 16 * a + 4 * g + r;
+        in[a][r] = !MASK || (key >= w.kbeg && key < w.kend);
+      }
+    }
+    if (t + 4 < t_end) load_k(t + 4);
+    float top[RT];
+    bool raise = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[a][rt][r] *= kf[a][r];
+          if (MASK && !(in[a][r] && 32 * t + 16 * a + 4 * g + r < limit[rt])) s[a][rt][r] = -INFINITY;
+        }
+      top[rt] = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
+                      fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
+      raise = raise || top[rt] > m[rt] + RAISE;
+    }
+    if (__any(raise)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float mn = fmaxf(m[rt], join_groups(top[rt], [](float x, float y) { return fmaxf(x, y); }));
+        const float alpha = exp2_fast(m[rt] - mn);
+        m[rt] = mn;
+        l[rt] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[rt][mt][r] *= alpha;
+      }
+    }
+    bf16x8_t pf[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      uint32_t o[4];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const float f[4] = {vs[a].x, vs[a].y, vs[a].z, vs[a].w};
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = exp2_fast(s[a][rt][r] - m[rt]);
+          l[rt] += e[r];
+          if constexpr (!C::WIDE) {
+            e[r] *= f[r];
+            // (the scale of a key that this row does not see may be anything)
+            if (MASK && !(in[a][r] && 32 * t + 16 * a + 4 * g + r < limit[rt])) e[r] = 0.f;
+          }
+        }
+        o[2 * a] = pack2(e[0], e[1]);
+        o[2 * a + 1] = pack2(e[2], e[3]);
+      }
+      pf[rt] = as_frag(make_uint4(o[0], o[1], o[2], o[3]));
+    }
+    if constexpr (C::WIDE) {
+      uint16_t* turn = reinterpret_cast<uint16_t*>(space) + wid * 32 * D;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) {
+          const int row = 16 * a + (lane + 64 * i) / (D / 8), ch = (lane + 64 * i) % (D / 8);
+          uint4 x = vr[a][i];
+          if (MASK) {
+            const int key = 32 * t + row;
+            if (key < w.kbeg || key >= w.kend) x = make_uint4(0, 0, 0, 0);
+          }
+          st16(turn + row * D + (ch ^ (((row & 7) << 1) & (D / 8 - 1))) * 8, x);
+        }
+      if (t + 4 < t_end) load_v(t + 4);
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt) {
+        const int row = 4 * g + (li >> 2), col = mt * 16 + 4 * (li & 3);
+        const uint16_t* src = turn + row * D + ((col >> 3) ^ (((row & 7) << 1) & (D / 8 - 1))) * 8 + (col & 7);
+        const uint2 lo = __builtin_bit_cast(uint2, lds_read_tr16(src)), hi = __builtin_bit_cast(uint2, lds_read_tr16(src + 16 * D));
+        const bf16x8_t vf = as_frag(make_uint4(lo.x, lo.y, hi.x, hi.y));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vf, pf[rt], acc[rt][mt]);
+      }
+    } else {
+      uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};   // codes of keys outside the range: anything, E4M3's NaN too
+      if (MASK) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          keep[a] = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) keep[a] |= in[a][r] ? 0xFFu << (8 * r) : 0u;
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt) {
+        const uint4 &va = vr[0][mt >> 2], &vb = vr[1][mt >> 2];
+        const uint32_t ca = (mt & 3) == 0 ? va.x : (mt & 3) == 1 ? va.y : (mt & 3) == 2 ? va.z : va.w;
+        const uint32_t cb = (mt & 3) == 0 ? vb.x : (mt & 3) == 1 ? vb.y : (mt & 3) == 2 ? vb.z : vb.w;
+        const bf16x8_t vf = MASK ? kv_widen8<FMT>(ca & keep[0], cb & keep[1]) : kv_widen8<FMT>(ca, cb);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vf, pf[rt], acc[rt][mt]);
+      }
+      if (t + 4 < t_end) load_v(t + 4);
+    }
+  };
+
+  const int t0 = (w.kbeg >> 5) + wid;
+  if (t0 < t_end) {
+    load_k(t0);
+    load_v(t0);
+  }
+  for (int t = t0; t < t_end; t += 4) {
+    if (32 * t < w.kbeg || 32 * t + 32 > least) work(t, std::true_type{});
+    else work(t, std::false_type{});
+  }
+
+  // ---- the four waves' states: O^T[16 mt + 4 g + r][row li] of each row tile
+  float* o_lds = reinterpret_cast<float*>(space);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float sum = join_groups(l[rt], [](float x, float y) { return x + y; });
+    if (g == 0) {
+      m_lds[wid][rt * 16 + li] = m[rt];
+      l_lds[wid][rt * 16 + li] = sum;
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    __syncthreads();   // (the rows' last reads of this buffer)
+#pragma unroll
+    for (int mt = 0; mt < C::MT; ++mt)
+      *reinterpret_cast<float4*>(o_lds + (wid * 16 + li) * C::OROW + mt * 16 + 4 * g) =
+          make_float4(acc[rt][mt][0], acc[rt][mt][1], acc[rt][mt][2], acc[rt][mt][3]);
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 16 * D / 4; idx += 256) {
+      const int i = idx / (D / 4), d = idx % (D / 4) * 4, r = row0 + rt * 16 + i;
+      if (r >= nrows) continue;
+      float M = LOWEST;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) M = fmaxf(M, m_lds[x][rt * 16 + i]);
+      float sum = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float e = exp2_fast(m_lds[x][rt * 16 + i] - M);
+        const float4 a = *reinterpret_cast<const float4*>(o_lds + (x * 16 + i) * C::OROW + d);
+        sum += l_lds[x][rt * 16 + i] * e;
+        o.x += a.x * e; o.y += a.y * e; o.z += a.z * e; o.w += a.w * e;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;   // (a row that sees no key)
+      const int tok = r / p.G, head = kvh * p.G + r - tok * p.G;
+      const int64_t at = static_cast<int64_t>(w.tok0 + tok);
+      if (p.slots == 1) {
+        *reinterpret_cast<uint2*>(p.out + at * p.out_stride + static_cast<int64_t>(head) * D + d) =
+            make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+      } else {
+        const int64_t part = (at * p.Hq + head) * p.slots + w.slot;
+        *reinterpret_cast<float4*>(p.part_out + part * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (d == 0) p.part_lse[part] = sum == 0.f ? -INFINITY : M + __log2f(sum);
+      }
+    }
+  }
+}
+
+#define XGK_ROWS_LDS(FMT, D, RT)                                                                         \
+  __shared__ __attribute__((aligned(16))) uint8_t space[RowsCfg<FMT, D, RT>::SPACE];                    \
+  __shared__ __attribute__((aligned(16))) uint16_t q_lds[RowsCfg<FMT, D, RT>::Q_LDS ? 64 * D : 8];      \
+  __shared__ float m_lds[4][16 * RT], l_lds[4][16 * RT]
+
+// share `split` of `splits` of the 32-key tiles of [kbeg, kend)
+__device__ __forceinline__ void share(int& kbeg, int& kend, int split, int splits) {
+  if (splits <= 1) return;
+  const int first = kbeg >> 5, tiles = max(0, ((kend + 31) >> 5) - first), each = (tiles + splits - 1) / splits;
+  kbeg = max(kbeg, 32 * (first + split * each));
+  kend = min(kend, 32 * (first + min(tiles, (split + 1) * each)));
+}
+
+// One new token of each sequence. Grid (Hkv, B heads' blocks of 16, splits). starts: keys below belong to another launch.
+template <int FMT, int D>
+__global__ void __launch_bounds__(256) rows_decode_kernel(RowsArgs p, const int32_t* starts, int blocks, int splits, int slot0) {
+  XGK_ROWS_LDS(FMT, D, 1);
+  const int b = blockIdx.y / blocks;
+  RowsBlock w;
+  w.tok0 = w.table = b;
+  w.ntok = 1;
+  w.block = blockIdx.y - b * blocks;
+  w.kend = min(max(p.seq_lens[b], 0), p.width * p.bs);
+  w.kbeg = starts ? min(max(starts[b], 0), w.kend) : 0;
+  share(w.kbeg, w.kend, blockIdx.z, splits);
+  if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
+  w.slot = slot0 + blockIdx.z;
+  w.causal0 = -1;
+  attend_rows<FMT, D, 1>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+}
+
+// Prompt portions, causal. Grid (Hkv, blocks of rows of the longest, sequences splits). Late blocks see the most keys: first.
+template <int FMT, int D, int RT>
+__global__ void __launch_bounds__(256) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
+  XGK_ROWS_LDS(FMT, D, RT);
+  const int s = blockIdx.z / splits;
+  RowsBlock w;
+  w.tok0 = min(max(qsl[s], 0), tokens);
+  w.ntok = min(max(qsl[s + 1], 0), tokens) - w.tok0;
+  w.block = gridDim.y - 1 - blockIdx.y;
+  if (w.ntok <= 0 || w.block * 16 * RT >= w.ntok * p.G) return;
+  w.table = s;
+  const int len = min(p.seq_lens[s], p.width * p.bs);
+  w.causal0 = max(p.seq_lens[s] - w.ntok, 0);   // tokens before the portion
+  const int last_tok = min(w.ntok - 1, ((w.block + 1) * 16 * RT - 1) / p.G);
+  w.kbeg = 0;
+  w.kend = max(0, min(len, w.causal0 + last_tok + 1));
+  share(w.kbeg, w.kend, blockIdx.z - s * splits, splits);
+  if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
+  w.slot = blockIdx.z - s * splits;
+  attend_rows<FMT, D, RT>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+}
+
+// The common keys of groups of decode rows. items [n][8]: first sequence, sequences, block of rows, first key, end key, slot.
+template <int FMT, int D, int RT>
+__global__ void __launch_bounds__(256) rows_prefix_kernel(RowsArgs p, const int32_t* items) {
+  XGK_ROWS_LDS(FMT, D, RT);
+  const int32_t* it = items + blockIdx.y * 8;
+  RowsBlock w;
+  w.tok0 = w.table = it[0];
+  w.ntok = it[1];
+  w.block = it[2];
+  w.kend = min(it[4], p.width * p.bs);
+  w.kbeg = min(it[3], w.kend);
+  if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
+  w.slot = it[5];
+  w.causal0 = -1;
+  attend_rows<FMT, D, RT>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+}
+
+// Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). counts (with first_free): the first counts[token]
+// slots and those from first_free on hold parts; else all. qsl: tokens outside [qsl[0], qsl[S]) have none. A thread has four dims; a batch's loads all go out together.
+template <int D>
+__global__ void __launch_bounds__(256) rows_join_kernel(const float* __restrict__ part_out, const float* __restrict__ part_lse,
+                                                        uint16_t* __restrict__ out, int64_t out_stride, int rows, int Hq,
+                                                        int slots, const int32_t* __restrict__ counts, int first_free,
+                                                        const int32_t* __restrict__ qsl, int S) {
+  constexpr int TPR = D / 4, BATCH = 8;
+  const int row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
+  if (row >= rows) return;
+  const int tok = row / Hq, head = row - tok * Hq;
+  if (qsl && (tok < qsl[0] || tok >= qsl[S])) return;
+  const int front = counts ? min(max(counts[tok], 0), first_free) : slots;
+  const int n = counts ? front + slots - first_free : slots;
+  const float* lse = part_lse + static_cast<int64_t>(row) * slots;
+  const float* po = part_out + static_cast<int64_t>(row) * slots * D + d;
+  float M = LOWEST, sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < n; s0 += BATCH) {
+    float e[BATCH];
+    float4 x[BATCH];
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int j = min(s0 + i, n - 1), s = j < front ? j : j - front + first_free;
+      e[i] = lse[s];
+      x[i] = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * D);
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if (s0 + i >= n) e[i] = -INFINITY;
+      top = fmaxf(top, e[i]);
+    }
+    const float old = exp2_fast(M - top);
+    M = top;
+    sum *= old;
+    o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float f = exp2_fast(e[i] - M);
+      sum += f;
+      o.x += f * x[i].x; o.y += f * x[i].y; o.z += f * x[i].z; o.w += f * x[i].w;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(out + tok * out_stride + static_cast<int64_t>(head) * D + d) =
+      make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+}
+
+static bool rows_ok(const RowsArgs& p, int D) {
+  return p.bs > 0 && p.bs % KV_TILE == 0 && p.Hkv >= 1 && p.Hq % p.Hkv == 0 && (D == 64 || D == 128) && p.width >= 1 &&
+         p.num_blocks >= 1 && p.slots >= 1 && (p.slots == 1 || (p.part_out && p.part_lse)) && p.q_stride % 8 == 0 &&
+         p.out_stride % 4 == 0;
+}
+
+static void join(const RowsArgs& p, int D, int tokens, const int32_t* counts, int first_free, const int32_t* qsl, int S,
+                 hipStream_t st) {
+  const int rows = tokens * p.Hq, per = 256 / (D / 4);
+  if (D == 128)
+    hipLaunchKernelGGL(rows_join_kernel<128>, dim3((rows + per - 1) / per), dim3(256), 0, st, p.part_out, p.part_lse, p.out,
+                       p.out_stride, rows, p.Hq, p.slots, counts, first_free, qsl, S);
+  else
+    hipLaunchKernelGGL(rows_join_kernel<64>, dim3((rows + per - 1) / per), dim3(256), 0, st, p.part_out, p.part_lse, p.out,
+                       p.out_stride, rows, p.Hq, p.slots, counts, first_free, qsl, S);
+}
+
+#define XGK_FMT_DIM(DO)                                                                                              \
+  if (fmt == KV_FP8 && D == 128) DO(KV_FP8, 128) else if (fmt == KV_FP8) DO(KV_FP8, 64)                               \
+  else if (fmt == KV_INT8 && D == 128) DO(KV_INT8, 128) else if (fmt == KV_INT8) DO(KV_INT8, 64)
+
+// Decode over an 8-bit cache. Returns 0, or -1 for what it does not take.
+int quant_decode_attention(int fmt, const uint16_t* q, int64_t q_stride, const uint8_t* k, const uint8_t* v, const float* scales,
+                           const int32_t* tables, int64_t table_stride, int width, const int32_t* seq_lens, float* part_out,
+                           float* part_lse, uint16_t* out, int64_t out_stride, int B, int Hq, int Hkv, int D, int bs,
+                           int num_blocks, float scale, int splits, hipStream_t st) {
+  if (B <= 0) return 0;
+  const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits};
+  const int blocks = (p.G + 15) / 16;
+  if (!rows_ok(p, D) || static_cast<int64_t>(B) * blocks > 65535 || splits > 65535) return -1;
+#define XGK_GO(F, DD)                                                                                                   \
+  {                                                                                                                     \
+    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, nullptr, blocks, \
+                       splits, 0);                                                                                      \
+  }
+  XGK_FMT_DIM(XGK_GO) else return -1;
+#undef XGK_GO
+  if (splits > 1) join(p, D, B, nullptr, 0, nullptr, 0, st);
+  return 0;
+}
+
+// Causal attention of packed prompt portions over an 8-bit cache; 16 RT rows a workgroup.
+int quant_prefill_attention(int fmt, const uint16_t* q, int64_t q_stride, const uint8_t* k, const uint8_t* v, const float* scales,
+                            const int32_t* tables, int64_t table_stride, int width, const int32_t* qsl, const int32_t* seq_lens,
+                            float* part_out, float* part_lse, uint16_t* out, int64_t out_stride, int tokens, int S, int max_q,
+                            int Hq, int Hkv, int D, int bs, int num_blocks, float scale, int RT, int splits, hipStream_t st) {
+  if (tokens <= 0 || S <= 0 || max_q <= 0) return 0;
+  const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits};
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 4)) return -1;
+  const int64_t blocks = (static_cast<int64_t>(max_q) * p.G + 16 * RT - 1) / (16 * RT);
+  if (blocks > 65535 || static_cast<int64_t>(S) * splits > 65535) return -1;
+  const dim3 grid(Hkv, static_cast<unsigned>(blocks), S * splits);
+#define XGK_GO(F, DD)                                                                                                        \
+  {                                                                                                                          \
+    if (RT == 1) hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 1>), grid, dim3(256), 0, st, p, qsl, tokens, splits);         \
+    else if (RT == 2) hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 2>), grid, dim3(256), 0, st, p, qsl, tokens, splits);    \
+    else hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 4>), grid, dim3(256), 0, st, p, qsl, tokens, splits);                 \
+  }
+  XGK_FMT_DIM(XGK_GO) else return -1;
+#undef XGK_GO
+  if (splits > 1) join(p, D, tokens, nullptr, 0, qsl, S, st);
+  return 0;
+}
+
+// Decode rows in groups with a common prefix. items: rows_prefix_kernel's, prefix: keys of each row that the items cover,
+// counts: its parts of them (at most prefix_slots), splits: parts of the rest.
+int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const void* k, const void* v, const float* scales,
+                            const int32_t* tables, int64_t table_stride, int width, const int32_t* seq_lens, float* part_out,
+                            float* part_lse, uint16_t* out, int64_t out_stride, int B, int Hq, int Hkv, int D, int bs,
+                            int num_blocks, float scale, const int32_t* items, int n_items, const int32_t* prefix,
+                            const int32_t* counts, int prefix_slots, int RT, int splits, hipStream_t st) {
+  if (B <= 0) return 0;
+  const RowsArgs p{q, q_stride, static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), scales, tables, table_stride,
+                   width, num_blocks, seq_lens, part_out, part_lse, out, out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs,
+                   scale * 1.44269504088896341f, prefix_slots + splits};
+  const int blocks = (p.G + 15) / 16;
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 4) || splits < 1 || splits > 65535 || prefix_slots < 0 || n_items < 0 ||
+      n_items > 65535 || static_cast<int64_t>(B) * blocks > 65535)
+    return -1;
+#define XGK_GO(F, DD)                                                                                                      \
+  {                                                                                                                        \
+    if (n_items > 0) {                                                                                                     \
+      if (RT == 1) hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 1>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);     \
+      else if (RT == 2) hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 2>), dim3(Hkv, n_items), dim3(256), 0, st, p, items); \
+      else hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 4>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);             \
+    }                                                                                                                      \
+    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, prefix, blocks,     \
+                       splits, prefix_slots);                                                                              \
+  }
+  XGK_FMT_DIM(XGK_GO)
+  else if (fmt == KV_BF16 && D == 128) XGK_GO(KV_BF16, 128) else if (fmt == KV_BF16) XGK_GO(KV_BF16, 64) else return -1;
+#undef XGK_GO
+  if (p.slots > 1) join(p, D, B, counts, prefix_slots, nullptr, 0, st);
+  return 0;
+}
+
+}  // namespace xgk

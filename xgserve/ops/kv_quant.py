@@ -1,0 +1,512 @@
+"""The 8-bit paged KV cache, the attentions over it, and decode attention of sequences that share a prefix.
+
+`QuantKVCache` holds keys and values of one layer in pages as 8-bit codes with one fp32 scale per token, kv head and side. A row
+x of D bf16 numbers whose largest magnitude is a is held as
+
+    int8   code = round(127 x / a), ties to even              value = code a / 127
+    fp8    code = round(448 x / a) to E4M3, ties to even      value = code a / 448
+
+(half a step of 2^-8 of a at most for int8, 2^-4 of each number for fp8). A row of zeros reads back as zeros; a row that holds
+an infinity or NaN reads back as NaN throughout, and so does what attends to it.
+
+All GPU calls go to the current stream of the current device, allocate nothing but their outputs and (without a workspace)
+the parts of a split, and can be captured; a workspace belongs to one call at a time, so captured graphs that may run at the
+same time, or eager calls beside them, each need their own. Page numbers of a table are kept within the cache.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from ._native import kernels, on_current_device, ptr, stream_ptr, use_native
+from .attention import DecodeWorkspace, _attend
+from .rope import _rotate
+
+KV_BF16, KV_FP8, KV_INT8 = 0, 1, 2
+KV_FORMATS = {"fp8": KV_FP8, "int8": KV_INT8}
+LARGEST = {"fp8": 448.0, "int8": 127.0}
+TILE = 16           # tokens whose codes lie together in the order of the matrix instructions (csrc/kernels/kv_quant.h)
+MAX_SPLITS = 64
+SPLIT_WGS = 512     # workgroups that fill the chip: two a CU
+SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _int32(t: torch.Tensor, name: str, dims: int, device) -> None:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    _need(t.dim() == dims and (t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1),
+          f"{name} must have {dims} dimension(s), contiguous in the last")
+    _need(t.device == device, f"{name} is on {t.device}, the cache on {device}")
+
+
+# ---------------------------------------------------------------------------------------------------------------- the cache
+@dataclass
+class QuantKVCache:
+    """One layer's keys and values in pages. `k`, `v`: codes [num_blocks, Hkv, block_size, D] uint8, where the 16 D codes of 16 tokens
+    lie in tile order (`kv_quant_read` gives rows); `scales` [num_blocks, Hkv, 2, block_size] fp32: the keys', then the values'. A
+    page is the same bytes wherever it lies, so whole pages may be copied, saved and moved."""
+    k: torch.Tensor
+    v: torch.Tensor
+    scales: torch.Tensor
+    fmt: str
+
+    @classmethod
+    def alloc(cls, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, fmt: str = "fp8",
+              device="cuda") -> "QuantKVCache":
+        """An empty cache: every row reads back as zeros."""
+        shape = (num_blocks, num_kv_heads, block_size, head_dim)
+        return cls(torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device),
+                   torch.zeros(num_blocks, num_kv_heads, 2, block_size, dtype=torch.float32, device=device), fmt)
+
+    def __post_init__(self):
+        _need(self.fmt in KV_FORMATS, f"format must be one of {sorted(KV_FORMATS)}, got {self.fmt!r}")
+        _need(self.k.dim() == 4 and self.k.shape == self.v.shape, "k and v must be [num_blocks, Hkv, block_size, D] alike")
+        nb, hkv, bs, d = self.k.shape
+        _need(nb >= 1 and hkv >= 1, "a cache has at least one page and one head")
+        _need(d in (64, 128), f"heads of 64 or 128 numbers, got {d}")
+        _need(bs >= TILE and bs % TILE == 0, f"pages of a multiple of {TILE} tokens, got {bs}")
+        _need(nb * bs < 1 << 31, "slots are 32-bit numbers")
+        if self.k.dtype != torch.uint8 or self.v.dtype != torch.uint8 or self.scales.dtype != torch.float32:
+            raise TypeError("codes are uint8 and scales float32")
+        _need(tuple(self.scales.shape) == (nb, hkv, 2, bs), "scales must be [num_blocks, Hkv, 2, block_size]")
+        _need(all(t.is_contiguous() for t in (self.k, self.v, self.scales)), "a cache is contiguous")
+        _need(self.k.device == self.v.device == self.scales.device, "a cache is on one device")
+
+    num_blocks = property(lambda self: self.k.shape[0])
+    num_kv_heads = property(lambda self: self.k.shape[1])
+    block_size = property(lambda self: self.k.shape[2])
+    head_dim = property(lambda self: self.k.shape[3])
+    device = property(lambda self: self.k.device)
+
+    def nbytes(self) -> int:
+        return self.k.numel() + self.v.numel() + 4 * self.scales.numel()
+
+
+def _native(cache_tensor: torch.Tensor) -> bool:
+    if not use_native(cache_tensor):
+        return False
+    _need(on_current_device(cache_tensor), f"the cache is on {cache_tensor.device}, which is not the current device")
+    return True
+
+
+# ------------------------------------------------------------------------------------------------------ plain (CPU) forms
+_ORDERS = {}
+
+
+def _order(D: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Bytes of codes (t, d) of a tile, keys' and values', [16, D]."""
+    key = (D, str(device))
+    if key not in _ORDERS:
+        t, d = torch.arange(TILE)[:, None], torch.arange(D)[None]
+        k = ((d // 16) * 16 + t) * 16 + d % 16
+        v = ((d // 64) * 64 + 16 * (t // 4) + d % 16) * 16 + (d // 16) % 4 * 4 + t % 4
+        _ORDERS[key] = (k.to(device), v.to(device))
+    return _ORDERS[key]
+
+
+def quantize_rows_ref(x: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes (uint8 bytes) and fp32 scales of rows [..., D]."""
+    a = x.abs().amax(-1, keepdim=True).double()
+    bad = ~torch.isfinite(x).all(-1, keepdim=True)
+    y = torch.where(bad | (a == 0), 0.0, x.double() * LARGEST[fmt] / torch.where(bad | (a == 0), 1.0, a))
+    codes = y.float().to(torch.float8_e4m3fn) if fmt == "fp8" else y.round().to(torch.int8)
+    scale = torch.where(bad, math.nan, a).float() / torch.tensor(LARGEST[fmt], device=x.device)
+    return codes.view(torch.uint8), scale[..., 0]
+
+
+def _tile_index(cache: QuantKVCache, slots: torch.Tensor):
+    """Pages, offsets in a page, and bytes of the page's rows of a head, keys' and values' [n, D], of slots."""
+    slots = slots.long()
+    pages, offs = slots // cache.block_size, slots % cache.block_size
+    ko, vo = _order(cache.head_dim, cache.device)
+    base = ((offs // TILE) * TILE * cache.head_dim)[:, None]
+    return pages, offs, base + ko[offs % TILE], base + vo[offs % TILE]
+
+
+def kv_quant_append_ref(k, v, cache: QuantKVCache, slot_mapping) -> None:
+    real = (slot_mapping >= 0) & (slot_mapping.long() < cache.num_blocks * cache.block_size)
+    if not bool(real.any()):
+        return
+    pages, offs, ko, vo = _tile_index(cache, slot_mapping[real])
+    flat = (cache.num_blocks, cache.num_kv_heads, cache.block_size * cache.head_dim)
+    heads = torch.arange(cache.num_kv_heads, device=cache.device)
+    for side, (x, codes, order) in enumerate(((k, cache.k, ko), (v, cache.v, vo))):
+        c, s = quantize_rows_ref(x[real], cache.fmt)
+        codes.view(flat)[pages[:, None, None], heads[None, :, None], order[:, None, :]] = c
+        cache.scales[pages, :, side, offs] = s
+
+
+def _rows_ref(cache: QuantKVCache, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 rows [n, Hkv, D] of slots."""
+    pages, offs, ko, vo = _tile_index(cache, slots)
+    flat = (cache.num_blocks, cache.num_kv_heads, cache.block_size * cache.head_dim)
+    heads = torch.arange(cache.num_kv_heads, device=cache.device)
+    out = []
+    for side, (codes, order) in enumerate(((cache.k, ko), (cache.v, vo))):
+        c = codes.view(flat)[pages[:, None, None], heads[None, :, None], order[:, None, :]]
+        c = c.view(torch.float8_e4m3fn if cache.fmt == "fp8" else torch.int8).float()
+        out.append(c * cache.scales[pages, :, side, offs][..., None])
+    return out[0], out[1]
+
+
+def _slots_ref(table_row: torch.Tensor, bs: int, lo: int, hi: int, num_blocks: int) -> torch.Tensor:
+    at = torch.arange(lo, hi, device=table_row.device)
+    return table_row.long()[at // bs].clamp(0, num_blocks - 1) * bs + at % bs
+
+
+def _any_rows_ref(kv, table_row, lo: int, hi: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    if isinstance(kv, QuantKVCache):
+        return _rows_ref(kv, _slots_ref(table_row, kv.block_size, lo, hi, kv.num_blocks))
+    bs, nb = kv[0].shape[2], kv[0].shape[0]
+    slots = _slots_ref(table_row, bs, lo, hi, nb)
+    return tuple(x[slots // bs, :, slots % bs].float() for x in kv)
+
+
+def _attend_causal(q, k, v, first: int, scale: float) -> torch.Tensor:
+    """q [n, Hq, D] at positions first .. over fp32 rows; a value that is NaN reaches the queries that see it and no others."""
+    n, Hq, _ = q.shape
+    pos = torch.arange(first, first + n, device=q.device)
+    bad = v.isnan().any(-1)                                           # [L, Hkv]
+    out = _attend(q, k, v.masked_fill(bad[..., None], 0.0), pos, scale)
+    reached = (bad.cumsum(0) > 0)[pos.clamp(max=k.shape[0] - 1)] if k.shape[0] else bad.new_zeros(n, bad.shape[1])
+    return out.masked_fill(reached.repeat_interleave(Hq // bad.shape[1], 1)[..., None], math.nan)
+
+
+# --------------------------------------------------------------------------------------------------------- write and read
+def _check_rows(x: torch.Tensor, name: str, cache: QuantKVCache, T: int) -> None:
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {x.dtype}")
+    H, D = cache.num_kv_heads, cache.head_dim
+    _need(x.dim() == 3 and tuple(x.shape) == (T, H, D), f"{name} must be [{T}, {H}, {D}], got {tuple(x.shape)}")
+    _need(x.device == cache.device, f"{name} is on {x.device}, the cache on {cache.device}")
+    if T:
+        _need(x.stride(2) == 1 and (H == 1 or x.stride(1) == D), f"{name}'s heads must be contiguous within a token")
+        _need(x.stride(0) % (D // 16) == 0 and x.data_ptr() % (D // 8) == 0, f"{name}'s tokens must begin at multiples of {D // 8} bytes")
+
+
+def kv_quant_append(k: torch.Tensor, v: torch.Tensor, cache: QuantKVCache, slot_mapping: torch.Tensor) -> None:
+    """Writes rows k, v [T, Hkv, D] bf16 (tokens may be strided: views into the projection's rows) to the cache's slots
+    slot_mapping [T] int32; tokens with a slot below 0 or behind the cache are left out. A slot may occur once in a call."""
+    T = k.shape[0]
+    _check_rows(k, "k", cache, T)
+    _check_rows(v, "v", cache, T)
+    _int32(slot_mapping, "slot_mapping", 1, cache.device)
+    _need(slot_mapping.shape[0] == T, f"slot_mapping must have {T} entries")
+    if T == 0:
+        return
+    if not _native(cache.k):
+        return kv_quant_append_ref(k, v, cache, slot_mapping)
+    _append(cache, None, k, v, slot_mapping, None, None, 0)
+
+
+def _append(cache, q, k, v, slots, positions, cos_sin, Hq) -> None:
+    kernels().kv_append(KV_FORMATS[cache.fmt], ptr(q), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(),
+                        ptr(positions), ptr(cos_sin), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
+                        cache.num_blocks, k.shape[0], Hq, cache.num_kv_heads, cache.head_dim, cache.block_size, stream_ptr())
+
+
+def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, cache: QuantKVCache,
+                  slot_mapping: torch.Tensor, num_heads: int, apply_rope: bool = True) -> None:
+    """`rope_cache` for an 8-bit cache: rows qkv [T, (Hq + 2 Hkv) D] bf16, q rotated in place, k rotated (to bf16, as the bf16
+    cache holds it) and v written to the cache in 8 bits. positions [T] int32 within cos_sin [max_pos, D] fp32."""
+    H, D, T = cache.num_kv_heads, cache.head_dim, qkv.shape[0]
+    _need(qkv.dim() == 2 and qkv.shape[1] >= (num_heads + 2 * H) * D and (T == 0 or qkv.stride(1) == 1),
+          "qkv must be [T, (Hq + 2 Hkv) D], contiguous in the last dimension")
+    k = qkv[:, num_heads * D:(num_heads + H) * D].unflatten(1, (H, D))
+    v = qkv[:, (num_heads + H) * D:(num_heads + 2 * H) * D].unflatten(1, (H, D))
+    if not apply_rope:
+        return kv_quant_append(k, v, cache, slot_mapping)
+    _check_rows(k, "qkv", cache, T)
+    _int32(slot_mapping, "slot_mapping", 1, cache.device)
+    _int32(positions, "positions", 1, cache.device)
+    _need(slot_mapping.shape[0] == T and positions.shape[0] == T, f"slot_mapping and positions must have {T} entries")
+    if cos_sin.dtype != torch.float32:
+        raise TypeError("cos_sin must be float32")
+    _need(cos_sin.dim() == 2 and cos_sin.shape[1] == D and cos_sin.is_contiguous() and cos_sin.device == cache.device,
+          f"cos_sin must be a contiguous [max_pos, {D}] table beside the cache")
+    if T == 0:
+        return
+    if not _native(cache.k):
+        cs = cos_sin[positions.long()]
+        cos, sin = cs[:, None, :D // 2], cs[:, None, D // 2:]
+        q = qkv[:, :num_heads * D].unflatten(1, (num_heads, D))
+        q.copy_(_rotate(q.float(), cos, sin).to(qkv.dtype))
+        return kv_quant_append_ref(_rotate(k.float(), cos, sin).to(torch.bfloat16), v, cache, slot_mapping)
+    _append(cache, qkv, k, v, slot_mapping, positions, cos_sin, num_heads)
+
+
+def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch.Tensor, cu_tokens: torch.Tensor, num_tokens: int,
+                  out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cached rows as bf16: tokens starts[s] .. starts[s] + cu_tokens[s + 1] - cu_tokens[s] of each sequence, packed
+    -> k, v [num_tokens, Hkv, D]. block_tables [S, W], starts [S], cu_tokens [S + 1] (from 0, not falling) int32; num_tokens =
+    cu_tokens[S]. Tokens behind a sequence's table have no row: theirs stay as they were in `out`."""
+    _int32(block_tables, "block_tables", 2, cache.device)
+    _int32(starts, "starts", 1, cache.device)
+    _int32(cu_tokens, "cu_tokens", 1, cache.device)
+    S, W = block_tables.shape
+    _need(starts.shape[0] == S and cu_tokens.shape[0] == S + 1, "starts must have an entry a sequence, cu_tokens one more")
+    _need(num_tokens >= 0, "num_tokens must not be negative")
+    shape = (num_tokens, cache.num_kv_heads, cache.head_dim)
+    if out is None:
+        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    else:
+        k, v = out
+        for t in (k, v):
+            _need(t.dtype == torch.bfloat16 and tuple(t.shape) == shape and t.is_contiguous() and t.device == cache.device
+                  and t.data_ptr() % 16 == 0, f"out must be two contiguous, aligned bfloat16 {list(shape)} beside the cache")
+    if num_tokens == 0 or S == 0 or W == 0:
+        return k, v
+    if not _native(cache.k):
+        for s in range(S):
+            lo, a, b = int(starts[s]), int(cu_tokens[s]), min(int(cu_tokens[s + 1]), num_tokens)
+            n = min(b - a, W * cache.block_size - lo)
+            if n > 0:
+                k[a:a + n], v[a:a + n] = _rows_ref(cache, _slots_ref(block_tables[s], cache.block_size, lo, lo + n, cache.num_blocks))
+        return k, v
+    kernels().kv_read(KV_FORMATS[cache.fmt], cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
+                      block_tables.data_ptr(), block_tables.stride(0), W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens,
+                      cache.num_blocks, cache.num_kv_heads, cache.head_dim, cache.block_size, k.data_ptr(), v.data_ptr(),
+                      stream_ptr())
+    return k, v
+
+
+# -------------------------------------------------------------------------------------------------------------- attention
+def _check_q(q: torch.Tensor, Hkv: int, D: int, device) -> None:
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"q must be bfloat16, got {q.dtype}")
+    _need(q.dim() == 3 and q.shape[2] == D and q.shape[1] >= 1 and q.shape[1] % Hkv == 0,
+          f"q must be [tokens, a multiple of {Hkv} heads, {D}], got {tuple(q.shape)}")
+    _need(q.device == device, f"q is on {q.device}, the cache on {device}")
+    if q.shape[0]:
+        _need(q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == D), "q's heads must be contiguous within a token")
+        _need(q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0, "q's tokens must begin at multiples of 16 bytes")
+
+
+def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.dtype != q.dtype:
+        raise TypeError(f"out must be {q.dtype}, got {out.dtype}")
+    _need(out.shape == q.shape and out.device == q.device, f"out must be {list(q.shape)} beside q")
+    if q.shape[0]:
+        _need(out.stride(2) == 1 and (q.shape[1] == 1 or out.stride(1) == q.shape[2]) and out.stride(0) % 4 == 0
+              and out.data_ptr() % 8 == 0, "out's heads must be contiguous within a token, and tokens begin at multiples of 8 bytes")
+    return out
+
+
+def _check_tables(block_tables, seq_lens, device, S: int) -> None:
+    _int32(block_tables, "block_tables", 2, device)
+    _int32(seq_lens, "seq_lens", 1, device)
+    _need(block_tables.shape[0] == S and seq_lens.shape[0] == S, f"block_tables and seq_lens must have {S} rows")
+    _need(block_tables.shape[1] >= 1 or S == 0, "block_tables must have a column")
+
+
+def _splits(wgs: int, max_keys: int) -> int:
+    """Parts of the key range: enough workgroups to fill the chip, each with a tile for each of its waves."""
+    want = -(-SPLIT_WGS // max(1, wgs))
+    return max(1, min(want, -(-max_keys // SPLIT_KEYS), MAX_SPLITS))
+
+
+def _parts(workspace: Optional[DecodeWorkspace], tokens: int, Hq: int, D: int, slots: int, device):
+    """Pointers (and the owner) of the parts' buffers."""
+    if slots <= 1:
+        return None, 0, 0
+    if workspace is None:
+        workspace = DecodeWorkspace(tokens, Hq, D, slots, device)
+    _need(workspace.part_lse.device == device and workspace.part_lse.numel() >= tokens * Hq * slots
+          and workspace.part_out.numel() >= tokens * Hq * slots * D,
+          f"the workspace is too small for {slots} parts of {tokens} tokens of {Hq} heads of {D}, or on another device")
+    return workspace, workspace.part_out.data_ptr(), workspace.part_lse.data_ptr()
+
+
+def _num_splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
+    if num_splits is None:
+        return _splits(wgs, max_keys)
+    _need(1 <= num_splits <= MAX_SPLITS, f"num_splits must be 1 to {MAX_SPLITS}, got {num_splits}")
+    return int(num_splits)
+
+
+def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                           num_splits: Optional[int] = None, workspace: Optional[DecodeWorkspace] = None,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`decode_attention` over an 8-bit cache: q [B, Hq, D] bf16 (tokens may be strided), one new token of each sequence, whose own
+    key is in the cache already -> [B, Hq, D]. block_tables [B, W], seq_lens [B] int32; a length of 0 gives zeros, one behind the
+    table means the whole table. num_splits: parts of the key range (None: by the batch and the table's width)."""
+    Hkv, D, bs, dev = cache.num_kv_heads, cache.head_dim, cache.block_size, cache.device
+    _check_q(q, Hkv, D, dev)
+    B, Hq, _ = q.shape
+    _check_tables(block_tables, seq_lens, dev, B)
+    out = _check_out(out, q)
+    W = block_tables.shape[1]
+    splits = _num_splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs)
+    if B == 0:
+        return out
+    if not _native(cache.k):
+        for b in range(B):
+            L = min(int(seq_lens[b]), W * bs)
+            out[b] = 0
+            if L > 0:
+                k, v = _any_rows_ref(cache, block_tables[b], 0, L)
+                out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
+        return out
+    keep, po, pl = _parts(workspace, B, Hq, D, splits, dev)
+    kernels().quant_decode_attention(KV_FORMATS[cache.fmt], q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
+                                     cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
+                                     seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs,
+                                     cache.num_blocks, float(scale), splits, stream_ptr())
+    return out
+
+
+def _row_tiles(rows: int) -> int:
+    """16-row tiles of a workgroup: as many as the rows fill."""
+    return 1 if rows <= 16 else 2
+
+
+def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
+                            seq_lens: torch.Tensor, max_q_len: int, scale: float, num_splits: Optional[int] = None,
+                            workspace: Optional[DecodeWorkspace] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`prefill_attention` over an 8-bit cache: q [T, Hq, D] bf16 packed; sequence s has the tokens query_start_loc[s] ..
+    query_start_loc[s + 1], the last of its seq_lens[s], and each sees the keys up to its own, all of them in the cache already.
+    max_q_len: at least the tokens of the longest portion. Rows of no sequence stay as they were in `out`."""
+    Hkv, D, bs, dev = cache.num_kv_heads, cache.head_dim, cache.block_size, cache.device
+    _check_q(q, Hkv, D, dev)
+    T, Hq, _ = q.shape
+    S = seq_lens.shape[0]
+    _check_tables(block_tables, seq_lens, dev, S)
+    _int32(query_start_loc, "query_start_loc", 1, dev)
+    _need(query_start_loc.shape[0] == S + 1, "query_start_loc must have one entry more than seq_lens")
+    _need(0 <= max_q_len, "max_q_len must not be negative")
+    out = _check_out(out, q)
+    if T == 0 or S == 0 or max_q_len == 0:
+        return out
+    W, G = block_tables.shape[1], Hq // Hkv
+    max_q_len = min(max_q_len, T)
+    rt = _row_tiles(max_q_len * G)
+    splits = _num_splits(num_splits, S * Hkv * -(-max_q_len * G // (16 * rt)), W * bs)
+    _need(S * splits <= 65535 and -(-max_q_len * G // (16 * rt)) <= 65535, "at most 65535 sequences (times splits), or blocks of rows")
+    if not _native(cache.k):
+        for s in range(S):
+            a, b = int(query_start_loc[s]), int(query_start_loc[s + 1])
+            n, L = min(b - a, max_q_len), int(seq_lens[s])
+            if n > 0:
+                k, v = _any_rows_ref(cache, block_tables[s], 0, min(L, W * bs))
+                out[a:a + n] = _attend_causal(q[a:a + n], k, v, max(L - (b - a), 0), scale).to(q.dtype)
+        return out
+    keep, po, pl = _parts(workspace, T, Hq, D, splits, dev)
+    kernels().quant_prefill_attention(KV_FORMATS[cache.fmt], q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
+                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
+                                      query_start_loc.data_ptr(), seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), T, S,
+                                      int(max_q_len), Hq, Hkv, D, bs, cache.num_blocks, float(scale), rt, splits, stream_ptr())
+    return out
+
+
+# ----------------------------------------------------------------------------------------------------------- shared prefixes
+@dataclass
+class SharedPrefixPlan:
+    """Which sequences of a decode batch share which prefix, and the launch's work (`shared_prefix_plan`)."""
+    num_seqs: int
+    num_heads: int
+    num_kv_heads: int
+    row_tiles: int               # 16-row tiles of a workgroup of the common part
+    slots: int                   # most parts that a prefix is cut into
+    items: torch.Tensor          # [n, 8] int32: first sequence, sequences, block of rows, first key, end key, slot
+    prefix: torch.Tensor         # [num_seqs] int32: keys that the common part covers
+    counts: torch.Tensor         # [num_seqs] int32: its parts
+    group_sizes: Tuple[int, ...]
+    prefix_lens: Tuple[int, ...]
+
+
+def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], num_heads: int, num_kv_heads: int,
+                       device="cuda") -> SharedPrefixPlan:
+    """Plan of a decode batch whose sequences come in groups: group_sizes[g] sequences in a row of the batch share their first
+    prefix_lens[g] tokens (0: nothing shared). A program makes it when the batch changes, not for every step; it holds for any
+    lengths of the sequences and for all layers."""
+    sizes, lens = [int(n) for n in group_sizes], [int(n) for n in prefix_lens]
+    _need(len(sizes) == len(lens), "a prefix length for each group")
+    _need(all(n >= 1 for n in sizes) and all(0 <= n < 1 << 30 for n in lens), "groups of at least one sequence, lengths of at least 0")
+    _need(num_kv_heads >= 1 and num_heads >= 1 and num_heads % num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
+    G = num_heads // num_kv_heads
+    rt = _row_tiles(max([n * G for n, p in zip(sizes, lens) if p > 0], default=0))
+    blocks = [-(-n * G // (16 * rt)) for n in sizes]
+    tiles = [-(-p // 32) for p in lens]
+    total = sum(b * t for b, t in zip(blocks, tiles)) * num_kv_heads
+    each = max(4, -(-total // SPLIT_WGS))      # 32-key tiles of a workgroup
+    items: List[List[int]] = []
+    prefix, counts, at = [], [], 0
+    for n, p, b, t in zip(sizes, lens, blocks, tiles):
+        parts = min(MAX_SPLITS, -(-t // each))
+        share = -(-t // parts) * 32 if parts else 0
+        parts = -(-p // share) if parts else 0
+        # (the blocks of one range of keys side by side: they read the same bytes)
+        items += [[at, n, i, j * share, min(p, (j + 1) * share), j, 0, 0] for j in range(parts) for i in range(b)]
+        prefix += [p] * n
+        counts += [parts] * n
+        at += n
+    _need(len(items) <= 65535, "too many groups")
+
+    def put(rows, width):
+        return torch.tensor(rows, dtype=torch.int32).reshape(-1, *width).to(device)
+
+    return SharedPrefixPlan(at, num_heads, num_kv_heads, rt, max(counts, default=0), put(items, (8,)), put(prefix, ()), put(counts, ()),
+                            tuple(sizes), tuple(lens))
+
+
+def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch.Tensor, torch.Tensor]], block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, plan: SharedPrefixPlan, scale: float, num_splits: Optional[int] = None,
+                            workspace: Optional[DecodeWorkspace] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode attention q [B, Hq, D] bf16 of sequences in groups with a common prefix, whose keys are read once for the group: of a
+    group, the first prefix_lens[g] keys of every sequence are those of its first sequence's table, the rest its own table's; a
+    sequence shorter than the prefix sees as much of it as it is long. kv: a `QuantKVCache`, or the bf16 pages (k, v) [NB, Hkv, bs,
+    D]. num_splits: parts of the keys behind the prefix. A workspace needs plan.slots + num_splits parts."""
+    quant = isinstance(kv, QuantKVCache)
+    if quant:
+        kc, vc, nb, Hkv, bs, D, fmt = kv.k, kv.v, kv.num_blocks, kv.num_kv_heads, kv.block_size, kv.head_dim, KV_FORMATS[kv.fmt]
+    else:
+        kc, vc = kv
+        if kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16:
+            raise TypeError("kv must be a QuantKVCache or bfloat16 pages")
+        _need(kc.dim() == 4 and kc.shape == vc.shape and kc.is_contiguous() and vc.is_contiguous() and kc.device == vc.device
+              and kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0, "pages must be contiguous [NB, Hkv, bs, D] alike")
+        (nb, Hkv, bs, D), fmt = kc.shape, KV_BF16
+        _need(D in (64, 128) and bs >= TILE and bs % TILE == 0 and nb >= 1,
+              f"heads of 64 or 128 numbers in pages of a multiple of {TILE} tokens")
+    dev = kc.device
+    _check_q(q, Hkv, D, dev)
+    B, Hq, _ = q.shape
+    _check_tables(block_tables, seq_lens, dev, B)
+    _need((plan.num_seqs, plan.num_heads, plan.num_kv_heads) == (B, Hq, Hkv),
+          f"the plan is for {plan.num_seqs} sequences of {plan.num_heads} / {plan.num_kv_heads} heads, not {B} of {Hq} / {Hkv}")
+    _need(plan.prefix.device == dev, f"the plan is on {plan.prefix.device}, the cache on {dev}")
+    W = block_tables.shape[1]
+    _need(max(plan.prefix_lens, default=0) <= W * bs, "a prefix is longer than the tables")
+    out = _check_out(out, q)
+    splits = _num_splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs - min(plan.prefix_lens, default=0))
+    if B == 0:
+        return out
+    if not _native(kc):
+        at = 0
+        for n, p in zip(plan.group_sizes, plan.prefix_lens):
+            for b in range(at, at + n):
+                L = max(0, min(int(seq_lens[b]), W * bs))
+                out[b] = 0
+                if L > 0:
+                    front, back = _any_rows_ref(kv, block_tables[at], 0, min(p, L)), _any_rows_ref(kv, block_tables[b], min(p, L), L)
+                    k, v = (torch.cat(x) for x in zip(front, back))
+                    out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
+            at += n
+        return out
+    keep, po, pl = _parts(workspace, B, Hq, D, plan.slots + splits, dev)
+    kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride(0), kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
+                                      block_tables.data_ptr(), block_tables.stride(0), W, seq_lens.data_ptr(), po, pl,
+                                      out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, float(scale), plan.items.data_ptr(),
+                                      plan.items.shape[0], plan.prefix.data_ptr(), plan.counts.data_ptr(), plan.slots,
+                                      plan.row_tiles, splits, stream_ptr())
+    return out
