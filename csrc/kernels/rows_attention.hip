@@ -23,7 +23,7 @@
 namespace xgk {
 
 constexpr float RAISE = 8.f;          // in base 2
-constexpr float LOWEST = -1e30f;      // a maximum before any key: exp2(-inf - LOWEST) is 0
+constexpr float LOWEST = -1e30f;      // the maximum of no key: exp2(LOWEST - any) is 0
 
 struct RowsArgs {
   const uint16_t* q;
@@ -87,7 +87,7 @@ struct RowsCfg {
   static constexpr int SPACE = JOIN > TURN ? JOIN : TURN;
 };
 
-template <int FMT, int D, int RT>
+template <int FMT, int D, int RT, bool ONCE>
 __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space, uint16_t* q_lds,
                                             float (*m_lds)[16 * RT], float (*l_lds)[16 * RT]) {
   using C = RowsCfg<FMT, D, RT>;
@@ -129,21 +129,23 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   least = __builtin_amdgcn_readfirstlane(least);
   if constexpr (C::Q_LDS) __syncthreads();
 
-  float m[RT], l[RT];
+  float m[RT], l[RT], high[RT];   // running maximum and sum; what a score has to pass to raise it: anything, before the first key
   f32x4_t acc[RT][C::MT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = LOWEST;
-    l[rt] = 0.f;
+    m[rt] = l[rt] = 0.f;
+    high[rt] = -INFINITY;
 #pragma unroll
     for (int mt = 0; mt < C::MT; ++mt) acc[rt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
   const int tpp = p.bs >> 4;                       // tiles a page
-  const int t_end = (w.kend + 31) >> 5, last = (w.kend + 15) / 16 - 1;
+  const int t_end = (w.kend + 31) >> 5, last = max((w.kend + 15) / 16 - 1, 0);
   const int32_t* table = p.tables + w.table * p.table_stride;
   uint4 kr[2][C::LOADS], vr[2][C::LOADS];
   float4 ks[2], vs[2];
+  // a decode step reads its keys once (non-temporal); blocks of rows over the same keys find them in the L2
+  auto load16 = [](const void* at) { return ONCE ? ld16_nt(at) : ld16(at); };
   // half a tile's address: clamped to the last tile that holds a key, and into the cache
   auto place = [&](int t, int a) {
     const int tile = min(2 * t + a, last);
@@ -159,11 +161,11 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
       if constexpr (C::WIDE) {
         const uint16_t* base = reinterpret_cast<const uint16_t*>(p.k) + (ph * p.bs + at.y + li) * D + 8 * g;
 #pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = ld16_nt(base + 32 * i);
+        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = load16(base + 32 * i);
       } else {
         const uint8_t* base = p.k + (ph * p.bs + at.y) * D + lane * 16;
 #pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = ld16_nt(base + 1024 * i);
+        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = load16(base + 1024 * i);
         ks[a] = *reinterpret_cast<const float4*>(p.scales + ph * 2 * p.bs + at.y + 4 * g);
       }
     }
@@ -176,56 +178,53 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
       if constexpr (C::WIDE) {
         const uint16_t* base = reinterpret_cast<const uint16_t*>(p.v) + (ph * p.bs + at.y) * D + lane * 8;
 #pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = ld16_nt(base + 512 * i);   // 4 (D 128) or 8 whole rows a load
+        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = load16(base + 512 * i);   // 4 (D 128) or 8 whole rows a load
       } else {
         const uint8_t* base = p.v + (ph * p.bs + at.y) * D + lane * 16;
 #pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = ld16_nt(base + 1024 * i);
+        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = load16(base + 1024 * i);
         vs[a] = *reinterpret_cast<const float4*>(p.scales + ph * 2 * p.bs + p.bs + at.y + 4 * g);
       }
     }
   };
 
-  auto work = [&](int t, auto masked) {
-    constexpr bool MASK = decltype(masked)::value;
+  const int t0 = (w.kbeg >> 5) + wid;
+  load_k(t0);   // (of no tile: clamped, and unused)
+  load_v(t0);
+#pragma unroll 1
+  for (int t = t0; t < t_end; t += 4) {
+    const bool edge = 32 * t < w.kbeg || 32 * t + 32 > least;   // some row does not see some key
+    auto sees = [&](int rt, int a, int r) {
+      const int key = 32 * t + 16 * a + 4 * g + r;
+      return key >= w.kbeg && key < limit[rt];
+    };
     f32x4_t s[2][RT];
+    float kf[2][4];
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[a][rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < C::LOADS; ++i) {
-        bf16x8_t kf[C::WIDE ? 1 : 2];
-        if constexpr (C::WIDE) {
-          kf[0] = as_frag(kr[a][i]);
-        } else {
-          kf[0] = kv_widen8<FMT>(kr[a][i].x, kr[a][i].y);
-          kf[1] = kv_widen8<FMT>(kr[a][i].z, kr[a][i].w);
-        }
 #pragma unroll
         for (int x = 0; x < (C::WIDE ? 1 : 2); ++x) {
           const int kk = C::WIDE ? i : 2 * i + x;
+          bf16x8_t kx;
+          if constexpr (C::WIDE) kx = as_frag(kr[a][i]);
+          else kx = x == 0 ? kv_widen8<FMT>(kr[a][i].x, kr[a][i].y) : kv_widen8<FMT>(kr[a][i].z, kr[a][i].w);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             const bf16x8_t qx = C::Q_LDS ? as_frag(ld16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8)) : qf[C::Q_LDS ? 0 : rt][kk];
-            s[a][rt] = mfma16x16x32(kf[x], qx, s[a][rt]);
+            s[a][rt] = mfma16x16x32(kx, qx, s[a][rt]);
           }
         }
       }
-    }
-    float kf[2][4];
-    bool in[2][4];      // a key of the range: its V (and scale) may be used
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
       const float f[4] = {ks[a].x, ks[a].y, ks[a].z, ks[a].w};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        kf[a][r] = C::WIDE ? p.scale : f[r] * p.scale;
-        const int key = 32 * t + 16 * a + 4 * g + r;
-        in[a][r] = !MASK || (key >= w.kbeg && key < w.kend);
-      }
+      for (int r = 0; r < 4; ++r) kf[a][r] = C::WIDE ? p.scale : f[r] * p.scale;
     }
-    if (t + 4 < t_end) load_k(t + 4);
+    load_k(t + 4);
+    // scores less the running maximum; where one is above it by more than RAISE, the maximum of this tile becomes the new one
     float top[RT];
     bool raise = false;
 #pragma unroll
@@ -233,21 +232,31 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[a][rt][r] *= kf[a][r];
-          if (MASK && !(in[a][r] && 32 * t + 16 * a + 4 * g + r < limit[rt])) s[a][rt][r] = -INFINITY;
-        }
+        for (int r = 0; r < 4; ++r) s[a][rt][r] = fmaf(s[a][rt][r], kf[a][r], -m[rt]);
+      if (edge) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][rt][r] = sees(rt, a, r) ? s[a][rt][r] : -INFINITY;
+      }
       top[rt] = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
                       fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
-      raise = raise || top[rt] > m[rt] + RAISE;
+      raise = raise || top[rt] > high[rt];
     }
     if (__any(raise)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float mn = fmaxf(m[rt], join_groups(top[rt], [](float x, float y) { return fmaxf(x, y); }));
-        const float alpha = exp2_fast(m[rt] - mn);
-        m[rt] = mn;
+        const bool first = high[rt] == -INFINITY;
+        float up = join_groups(top[rt], [](float x, float y) { return fmaxf(x, y); });
+        if (first) high[rt] = up == -INFINITY ? up : RAISE;
+        up = first && up != -INFINITY ? up : fmaxf(up, 0.f);
+        const float alpha = first ? 1.f : exp2_fast(-up);
+        m[rt] += up;
         l[rt] *= alpha;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][rt][r] -= up;
 #pragma unroll
         for (int mt = 0; mt < C::MT; ++mt)
 #pragma unroll
@@ -257,26 +266,31 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
     bf16x8_t pf[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      uint32_t o[4];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const float f[4] = {vs[a].x, vs[a].y, vs[a].z, vs[a].w};
-        float e[4];
+      for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          e[r] = exp2_fast(s[a][rt][r] - m[rt]);
-          l[rt] += e[r];
-          if constexpr (!C::WIDE) {
-            e[r] *= f[r];
-            // (the scale of a key that this row does not see may be anything)
-            if (MASK && !(in[a][r] && 32 * t + 16 * a + 4 * g + r < limit[rt])) e[r] = 0.f;
-          }
+          s[a][rt][r] = exp2_fast(s[a][rt][r]);
+          l[rt] += s[a][rt][r];
         }
-        o[2 * a] = pack2(e[0], e[1]);
-        o[2 * a + 1] = pack2(e[2], e[3]);
+      if constexpr (!C::WIDE) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const float f[4] = {vs[a].x, vs[a].y, vs[a].z, vs[a].w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][rt][r] *= f[r];
+        }
+        if (edge) {   // (the scale of a key that a row does not see may be anything)
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[a][rt][r] = sees(rt, a, r) ? s[a][rt][r] : 0.f;
+        }
       }
-      pf[rt] = as_frag(make_uint4(o[0], o[1], o[2], o[3]));
+      pf[rt] = as_frag(make_uint4(pack2(s[0][rt][0], s[0][rt][1]), pack2(s[0][rt][2], s[0][rt][3]),
+                                  pack2(s[1][rt][0], s[1][rt][1]), pack2(s[1][rt][2], s[1][rt][3])));
     }
+    // V of keys outside the range: anything (E4M3's NaN too), so zeros
     if constexpr (C::WIDE) {
       uint16_t* turn = reinterpret_cast<uint16_t*>(space) + wid * 32 * D;
 #pragma unroll
@@ -284,54 +298,41 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
 #pragma unroll
         for (int i = 0; i < C::LOADS; ++i) {
           const int row = 16 * a + (lane + 64 * i) / (D / 8), ch = (lane + 64 * i) % (D / 8);
-          uint4 x = vr[a][i];
-          if (MASK) {
-            const int key = 32 * t + row;
-            if (key < w.kbeg || key >= w.kend) x = make_uint4(0, 0, 0, 0);
-          }
-          st16(turn + row * D + (ch ^ (((row & 7) << 1) & (D / 8 - 1))) * 8, x);
+          if (edge && (32 * t + row < w.kbeg || 32 * t + row >= w.kend)) vr[a][i] = make_uint4(0, 0, 0, 0);
+          st16(turn + row * D + (ch ^ (((row & 7) << 1) & (D / 8 - 1))) * 8, vr[a][i]);
         }
-      if (t + 4 < t_end) load_v(t + 4);
+      load_v(t + 4);
+    } else if (edge) {
 #pragma unroll
-      for (int mt = 0; mt < C::MT; ++mt) {
+      for (int a = 0; a < 2; ++a) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = 32 * t + 16 * a + 4 * g + r;
+          keep |= key >= w.kbeg && key < w.kend ? 0xFFu << (8 * r) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = make_uint4(vr[a][i].x & keep, vr[a][i].y & keep, vr[a][i].z & keep, vr[a][i].w & keep);
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < C::MT; ++mt) {
+      bf16x8_t vf;
+      if constexpr (C::WIDE) {
+        const uint16_t* turn = reinterpret_cast<const uint16_t*>(space) + wid * 32 * D;
         const int row = 4 * g + (li >> 2), col = mt * 16 + 4 * (li & 3);
         const uint16_t* src = turn + row * D + ((col >> 3) ^ (((row & 7) << 1) & (D / 8 - 1))) * 8 + (col & 7);
         const uint2 lo = __builtin_bit_cast(uint2, lds_read_tr16(src)), hi = __builtin_bit_cast(uint2, lds_read_tr16(src + 16 * D));
-        const bf16x8_t vf = as_frag(make_uint4(lo.x, lo.y, hi.x, hi.y));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vf, pf[rt], acc[rt][mt]);
-      }
-    } else {
-      uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};   // codes of keys outside the range: anything, E4M3's NaN too
-      if (MASK) {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          keep[a] = 0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) keep[a] |= in[a][r] ? 0xFFu << (8 * r) : 0u;
-        }
-      }
-#pragma unroll
-      for (int mt = 0; mt < C::MT; ++mt) {
+        vf = as_frag(make_uint4(lo.x, lo.y, hi.x, hi.y));
+      } else {
         const uint4 &va = vr[0][mt >> 2], &vb = vr[1][mt >> 2];
-        const uint32_t ca = (mt & 3) == 0 ? va.x : (mt & 3) == 1 ? va.y : (mt & 3) == 2 ? va.z : va.w;
-        const uint32_t cb = (mt & 3) == 0 ? vb.x : (mt & 3) == 1 ? vb.y : (mt & 3) == 2 ? vb.z : vb.w;
-        const bf16x8_t vf = MASK ? kv_widen8<FMT>(ca & keep[0], cb & keep[1]) : kv_widen8<FMT>(ca, cb);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vf, pf[rt], acc[rt][mt]);
+        vf = kv_widen8<FMT>((mt & 3) == 0 ? va.x : (mt & 3) == 1 ? va.y : (mt & 3) == 2 ? va.z : va.w,
+                            (mt & 3) == 0 ? vb.x : (mt & 3) == 1 ? vb.y : (mt & 3) == 2 ? vb.z : vb.w);
       }
-      if (t + 4 < t_end) load_v(t + 4);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vf, pf[rt], acc[rt][mt]);
     }
-  };
-
-  const int t0 = (w.kbeg >> 5) + wid;
-  if (t0 < t_end) {
-    load_k(t0);
-    load_v(t0);
-  }
-  for (int t = t0; t < t_end; t += 4) {
-    if (32 * t < w.kbeg || 32 * t + 32 > least) work(t, std::true_type{});
-    else work(t, std::false_type{});
+    if constexpr (!C::WIDE) load_v(t + 4);
   }
 
   // ---- the four waves' states: O^T[16 mt + 4 g + r][row li] of each row tile
@@ -340,7 +341,7 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   for (int rt = 0; rt < RT; ++rt) {
     const float sum = join_groups(l[rt], [](float x, float y) { return x + y; });
     if (g == 0) {
-      m_lds[wid][rt * 16 + li] = m[rt];
+      m_lds[wid][rt * 16 + li] = sum == 0.f ? LOWEST : m[rt];
       l_lds[wid][rt * 16 + li] = sum;
     }
   }
@@ -397,7 +398,7 @@ __device__ __forceinline__ void share(int& kbeg, int& kend, int split, int split
 
 // One new token of each sequence. Grid (Hkv, B heads' blocks of 16, splits). starts: keys below belong to another launch.
 template <int FMT, int D>
-__global__ void __launch_bounds__(256) rows_decode_kernel(RowsArgs p, const int32_t* starts, int blocks, int splits, int slot0) {
+__global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, const int32_t* starts, int blocks, int splits, int slot0) {
   XGK_ROWS_LDS(FMT, D, 1);
   const int b = blockIdx.y / blocks;
   RowsBlock w;
@@ -410,12 +411,12 @@ __global__ void __launch_bounds__(256) rows_decode_kernel(RowsArgs p, const int3
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
   w.slot = slot0 + blockIdx.z;
   w.causal0 = -1;
-  attend_rows<FMT, D, 1>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  attend_rows<FMT, D, 1, true>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
 }
 
 // Prompt portions, causal. Grid (Hkv, blocks of rows of the longest, sequences splits). Late blocks see the most keys: first.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
+__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
   XGK_ROWS_LDS(FMT, D, RT);
   const int s = blockIdx.z / splits;
   RowsBlock w;
@@ -432,12 +433,12 @@ __global__ void __launch_bounds__(256) rows_prompt_kernel(RowsArgs p, const int3
   share(w.kbeg, w.kend, blockIdx.z - s * splits, splits);
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
   w.slot = blockIdx.z - s * splits;
-  attend_rows<FMT, D, RT>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
 }
 
 // The common keys of groups of decode rows. items [n][8]: first sequence, sequences, block of rows, first key, end key, slot.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256) rows_prefix_kernel(RowsArgs p, const int32_t* items) {
+__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_prefix_kernel(RowsArgs p, const int32_t* items) {
   XGK_ROWS_LDS(FMT, D, RT);
   const int32_t* it = items + blockIdx.y * 8;
   RowsBlock w;
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(256) rows_prefix_kernel(RowsArgs p, const int3
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
   w.slot = it[5];
   w.causal0 = -1;
-  attend_rows<FMT, D, RT>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
 }
 
 // Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). counts (with first_free): the first counts[token]

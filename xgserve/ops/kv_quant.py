@@ -365,9 +365,9 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     return out
 
 
-def _row_tiles(rows: int) -> int:
-    """16-row tiles of a workgroup: as many as the rows fill."""
-    return 1 if rows <= 16 else 2
+def _row_tiles(rows: int, D: int) -> int:
+    """16-row tiles of a workgroup: as many as the rows fill and the registers hold."""
+    return 1 if rows <= 16 else 2 if rows <= 32 or D == 128 else 4
 
 
 def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
@@ -389,7 +389,7 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
         return out
     W, G = block_tables.shape[1], Hq // Hkv
     max_q_len = min(max_q_len, T)
-    rt = _row_tiles(max_q_len * G)
+    rt = _row_tiles(max_q_len * G, D)
     splits = _num_splits(num_splits, S * Hkv * -(-max_q_len * G // (16 * rt)), W * bs)
     _need(S * splits <= 65535 and -(-max_q_len * G // (16 * rt)) <= 65535, "at most 65535 sequences (times splits), or blocks of rows")
     if not _native(cache.k):
@@ -434,7 +434,7 @@ def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], n
     _need(all(n >= 1 for n in sizes) and all(0 <= n < 1 << 30 for n in lens), "groups of at least one sequence, lengths of at least 0")
     _need(num_kv_heads >= 1 and num_heads >= 1 and num_heads % num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
     G = num_heads // num_kv_heads
-    rt = _row_tiles(max([n * G for n, p in zip(sizes, lens) if p > 0], default=0))
+    rt = _row_tiles(max([n * G for n, p in zip(sizes, lens) if p > 0], default=0), 128)
     blocks = [-(-n * G // (16 * rt)) for n in sizes]
     tiles = [-(-p // 32) for p in lens]
     total = sum(b * t for b, t in zip(blocks, tiles)) * num_kv_heads
