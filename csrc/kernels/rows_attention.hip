@@ -42,7 +42,26 @@ struct RowsArgs {
   int Hq, Hkv, G, bs;
   float scale;            // softmax's, in base 2
   int slots;              // parts of a row (1: `out` is written here)
+  uint32_t page_magic;    // page_of
 };
+
+// tables are not written while a kernel reads them: scalar loads
+template <typename T>
+using Constant = const __attribute__((address_space(4))) T*;
+template <typename T>
+__device__ __forceinline__ Constant<T> constant(const T* p) {
+  return (Constant<T>)(uintptr_t)p;
+}
+
+// tile / (tiles a page), without a division: (2 tile + 1) / 2 over the tiles of a page, whose inverse in 31 bits is rounded up,
+// is in the right page while tile times (tiles a page) is below 2^30 (rows_ok)
+__device__ __forceinline__ int page_of(int tile, uint32_t magic) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __umulhi(2 * static_cast<uint32_t>(tile) + 1, magic);
+#else
+  return 0;
+#endif
+}
 
 // what one workgroup does
 struct RowsBlock {
@@ -80,12 +99,126 @@ struct RowsCfg {
   static constexpr int KK = D / 32;                  // matrix instructions over the head size
   static constexpr int MT = D / 16;                  // 16-dim tiles of the output
   static constexpr int LOADS = WIDE ? D / 32 : D / 64;   // 16-byte loads a lane, 16 tokens of K or V
-  static constexpr bool Q_LDS = RT == 4;             // registers: 64 of the rows' fragments would not fit beside the sums
+  static constexpr bool Q_LDS = false;   // 32 registers fewer: three waves a SIMD instead of two
   static constexpr int OROW = D + 4;                 // row of the joining buffer (padded: banks)
   static constexpr int JOIN = 4 * 16 * OROW * 4;     // bytes
   static constexpr int TURN = WIDE ? 4 * 32 * D * 2 : 0;
   static constexpr int SPACE = JOIN > TURN ? JOIN : TURN;
 };
+
+// Products q k of 32 keys -> scores less their rows' running maxima, which rise (and sums and outputs shrink) where a score is more
+// than RAISE above its row's. kf, vs: the keys' and values' factors. EDGE: some row does not see some key of the 32 from key0 on:
+// its score becomes -inf. A value that is not finite then reaches the rows that see it by their scores, and no other by its factor.
+template <bool EDGE, bool WIDE, int NA, int RT, int MT>
+__device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[NA], float4 (&vs)[NA], float scale, int key0, int kbeg,
+                                       int kend, const int (&limit)[RT], float (&m)[RT], float (&l)[RT], float (&high)[RT],
+                                       f32x4_t (&acc)[RT][MT]) {
+  float top[RT];
+  bool raise = false;
+#pragma unroll
+  for (int a = 0; a < NA; ++a) {
+    const float f[4] = {ks[a].x, ks[a].y, ks[a].z, ks[a].w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float k = WIDE ? scale : f[r] * scale;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[a][rt][r] = fmaf(s[a][rt][r], k, -m[rt]);
+    }
+  }
+  if constexpr (EDGE) {
+    const int base = key0 + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      float f[4] = {vs[a].x, vs[a].y, vs[a].z, vs[a].w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = base + 16 * a + r;
+        const bool odd = !WIDE && !(fabsf(f[r]) < INFINITY);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float x = odd ? NAN : s[a][rt][r];
+          s[a][rt][r] = key >= kbeg && key < limit[rt] ? x : -INFINITY;
+        }
+        if (odd || key < kbeg || key >= kend) f[r] = 0.f;
+      }
+      if constexpr (!WIDE) vs[a] = make_float4(f[0], f[1], f[2], f[3]);
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    top[rt] = fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3]));
+#pragma unroll
+    for (int a = 1; a < NA; ++a)
+      top[rt] = fmaxf(top[rt], fmaxf(fmaxf(s[a][rt][0], s[a][rt][1]), fmaxf(s[a][rt][2], s[a][rt][3])));
+    raise = raise || top[rt] > high[rt];
+  }
+  if (__any(raise)) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const bool first = high[rt] == -INFINITY;
+      float up = join_groups(top[rt], [](float x, float y) { return fmaxf(x, y); });
+      if (first) high[rt] = up == -INFINITY ? up : RAISE;
+      up = first && up != -INFINITY ? up : fmaxf(up, 0.f);
+      const float alpha = first ? 1.f : exp2_fast(-up);
+      m[rt] += up;
+      l[rt] *= alpha;
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[a][rt][r] -= up;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[rt][mt][r] *= alpha;
+    }
+  }
+}
+
+// ... -> weights, the P^T fragments of pairs of tiles. vs: the values' factors.
+template <bool WIDE, int NA, int RT>
+__device__ __forceinline__ void weights(f32x4_t (&s)[NA][RT], const float4 (&vs)[NA], float (&l)[RT], bf16x8_t (&pf)[NA / 2][RT]) {
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+    for (int pair = 0; pair < NA / 2; ++pair) {
+      uint32_t o[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int a = 2 * pair + x;
+        const float f[4] = {vs[a].x, vs[a].y, vs[a].z, vs[a].w};
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = exp2_fast(s[a][rt][r]);
+          l[rt] += e[r];
+          if constexpr (!WIDE) e[r] *= f[r];
+        }
+        o[2 * x] = pack2(e[0], e[1]);
+        o[2 * x + 1] = pack2(e[2], e[3]);
+      }
+      pf[pair][rt] = as_frag(make_uint4(o[0], o[1], o[2], o[3]));
+    }
+  }
+}
+
+// Row r of a block's list: its fragments of Q (the dims of the K fragments), the keys it sees; `least` sinks to these.
+template <int FMT, int D>
+__device__ __forceinline__ void load_row(const RowsArgs& p, const RowsBlock& w, int kvh, int r, int g, bf16x8_t (&qf)[D / 32],
+                                         int& limit, int& least) {
+  const bool real = r < w.ntok * p.G;
+  const int tok = real ? r / p.G : 0, head = kvh * p.G + (real ? r - tok * p.G : 0);
+  limit = 0;
+  if (real) {
+    limit = min(w.kend, w.causal0 >= 0 ? w.causal0 + tok + 1 : p.seq_lens[w.tok0 + tok]);
+    least = min(least, limit);
+  }
+  const uint16_t* qp = p.q + static_cast<int64_t>(w.tok0 + tok) * p.q_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+  for (int kk = 0; kk < D / 32; ++kk) {
+    const int d = FMT == KV_BF16 ? 32 * kk + 8 * g : 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
+    qf[kk] = as_frag(real ? ld16(qp + d) : make_uint4(0, 0, 0, 0));
+  }
+}
 
 template <int FMT, int D, int RT, bool ONCE>
 __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space, uint16_t* q_lds,
@@ -98,36 +231,18 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   // rows: fragments of Q, and the keys that each sees
   int limit[RT];
   int least = w.kend;   // every row sees the keys below
-  bf16x8_t qf[C::Q_LDS ? 1 : RT][C::KK];
+  bf16x8_t qf[RT][C::KK];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = row0 + rt * 16 + li;
-    const bool real = r < nrows;
-    const int tok = real ? r / p.G : 0, head = kvh * p.G + (real ? r - tok * p.G : 0);
-    limit[rt] = 0;
-    if (real) {
-      limit[rt] = min(w.kend, w.causal0 >= 0 ? w.causal0 + tok + 1 : p.seq_lens[w.tok0 + tok]);
-      least = min(least, limit[rt]);
-    }
-    const uint16_t* qp = p.q + static_cast<int64_t>(w.tok0 + tok) * p.q_stride + static_cast<int64_t>(head) * D;
-    if constexpr (!C::Q_LDS) {
+  for (int rt = 0; rt < RT; ++rt) load_row<FMT, D>(p, w, kvh, row0 + rt * 16 + li, g, qf[rt], limit[rt], least);
+  if constexpr (C::Q_LDS) {   // (every wave the same)
 #pragma unroll
-      for (int kk = 0; kk < C::KK; ++kk) {
-        // the dims of this lane's K fragment kk
-        const int d = C::WIDE ? 32 * kk + 8 * g : 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
-        qf[rt][kk] = as_frag(real ? ld16(qp + d) : make_uint4(0, 0, 0, 0));
-      }
-    } else if (rt == wid) {   // (wave rt brings row tile rt: RT is 4)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int kk = 0; kk < C::KK; ++kk) {
-        const int d = C::WIDE ? 32 * kk + 8 * g : 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
-        st16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8, real ? ld16(qp + d) : make_uint4(0, 0, 0, 0));
-      }
-    }
+      for (int kk = 0; kk < C::KK; ++kk) st16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8, __builtin_bit_cast(uint4, qf[rt][kk]));
+    __syncthreads();
   }
   for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
   least = __builtin_amdgcn_readfirstlane(least);
-  if constexpr (C::Q_LDS) __syncthreads();
 
   float m[RT], l[RT], high[RT];   // running maximum and sum; what a score has to pass to raise it: anything, before the first key
   f32x4_t acc[RT][C::MT];
@@ -141,65 +256,59 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
 
   const int tpp = p.bs >> 4;                       // tiles a page
   const int t_end = (w.kend + 31) >> 5, last = max((w.kend + 15) / 16 - 1, 0);
-  const int32_t* table = p.tables + w.table * p.table_stride;
+  const Constant<int32_t> table = constant(p.tables + w.table * p.table_stride);
   uint4 kr[2][C::LOADS], vr[2][C::LOADS];
   float4 ks[2], vs[2];
   // a decode step reads its keys once (non-temporal); blocks of rows over the same keys find them in the L2
   auto load16 = [](const void* at) { return ONCE ? ld16_nt(at) : ld16(at); };
-  // half a tile's address: clamped to the last tile that holds a key, and into the cache
-  auto place = [&](int t, int a) {
-    const int tile = min(2 * t + a, last);
-    const int pg = tile / tpp;
-    const int page = min(max(table[pg], 0), p.num_blocks - 1);
-    return make_int2(page, (tile - pg * tpp) * 16);
-  };
-  auto load_k = [&](int t) {
+  // where the halves of a tile lie: clamped to the last tile that holds a key, and into the cache. The page numbers of the
+  // tile after the next are asked for while the next one's loads go out, so no load waits for its address. Addresses are scalar
+  // work of each tile (a third of the loop's instructions where they came from the indexes each time): one offset for K and V
+  const uint32_t elem = C::WIDE ? 2 : 1;
+  const uint32_t page_bytes = static_cast<uint32_t>(p.Hkv) * p.bs * D * elem, page_scales = static_cast<uint32_t>(p.Hkv) * 2 * p.bs;
+  const uint8_t* k_head = p.k + static_cast<int64_t>(kvh) * p.bs * D * elem;
+  const uint8_t* v_head = p.v + static_cast<int64_t>(kvh) * p.bs * D * elem;
+  const float* s_head = p.scales + static_cast<int64_t>(kvh) * 2 * p.bs;
+  int page[2], off[2];
+  auto find = [&](int t) {
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const int2 at = place(t, a);
-      const int64_t ph = static_cast<int64_t>(at.x) * p.Hkv + kvh;
-      if constexpr (C::WIDE) {
-        const uint16_t* base = reinterpret_cast<const uint16_t*>(p.k) + (ph * p.bs + at.y + li) * D + 8 * g;
-#pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = load16(base + 32 * i);
-      } else {
-        const uint8_t* base = p.k + (ph * p.bs + at.y) * D + lane * 16;
-#pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) kr[a][i] = load16(base + 1024 * i);
-        ks[a] = *reinterpret_cast<const float4*>(p.scales + ph * 2 * p.bs + at.y + 4 * g);
-      }
+      const int tile = min(2 * t + a, last), pg = page_of(tile, p.page_magic);
+      page[a] = table[pg];
+      off[a] = (tile - pg * tpp) * 16;
     }
   };
-  auto load_v = [&](int t) {
+  uint64_t at[2];                // bytes of the half's tile from k_head, v_head
+  const float* factor[2];        // its first scale
+  auto settle = [&]() {
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const int2 at = place(t, a);
-      const int64_t ph = static_cast<int64_t>(at.x) * p.Hkv + kvh;
-      if constexpr (C::WIDE) {
-        const uint16_t* base = reinterpret_cast<const uint16_t*>(p.v) + (ph * p.bs + at.y) * D + lane * 8;
-#pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = load16(base + 512 * i);   // 4 (D 128) or 8 whole rows a load
-      } else {
-        const uint8_t* base = p.v + (ph * p.bs + at.y) * D + lane * 16;
-#pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = load16(base + 1024 * i);
-        vs[a] = *reinterpret_cast<const float4*>(p.scales + ph * 2 * p.bs + p.bs + at.y + 4 * g);
-      }
+      const uint32_t pg = min(max(page[a], 0), p.num_blocks - 1);
+      at[a] = static_cast<uint64_t>(pg) * page_bytes + static_cast<uint32_t>(off[a]) * D * elem;
+      if constexpr (!C::WIDE) factor[a] = s_head + static_cast<uint64_t>(pg) * page_scales + static_cast<uint32_t>(off[a]);
     }
   };
-
-  const int t0 = (w.kbeg >> 5) + wid;
-  load_k(t0);   // (of no tile: clamped, and unused)
-  load_v(t0);
-#pragma unroll 1
-  for (int t = t0; t < t_end; t += 4) {
-    const bool edge = 32 * t < w.kbeg || 32 * t + 32 > least;   // some row does not see some key
-    auto sees = [&](int rt, int a, int r) {
-      const int key = 32 * t + 16 * a + 4 * g + r;
-      return key >= w.kbeg && key < limit[rt];
-    };
-    f32x4_t s[2][RT];
-    float kf[2][4];
+  auto load_k = [&]() {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const uint8_t* base = k_head + at[a];
+#pragma unroll
+      for (int i = 0; i < C::LOADS; ++i)
+        kr[a][i] = load16(base + (C::WIDE ? static_cast<uint32_t>(li * D * 2 + 16 * g + 64 * i) : static_cast<uint32_t>(lane * 16 + 1024 * i)));
+      if constexpr (!C::WIDE) ks[a] = *reinterpret_cast<const float4*>(factor[a] + 4 * g);
+    }
+  };
+  auto load_v = [&]() {          // (bf16: 4 (D 128) or 8 whole rows a load)
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const uint8_t* base = v_head + at[a];
+#pragma unroll
+      for (int i = 0; i < C::LOADS; ++i) vr[a][i] = load16(base + static_cast<uint32_t>(lane * 16 + 1024 * i));
+      if constexpr (!C::WIDE) vs[a] = *reinterpret_cast<const float4*>(factor[a] + p.bs + 4 * g);
+    }
+  };
+  // S^T of the tile whose K is in registers
+  auto product = [&](f32x4_t (&s)[2][RT]) {
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
 #pragma unroll
@@ -214,126 +323,97 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
           else kx = x == 0 ? kv_widen8<FMT>(kr[a][i].x, kr[a][i].y) : kv_widen8<FMT>(kr[a][i].z, kr[a][i].w);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            const bf16x8_t qx = C::Q_LDS ? as_frag(ld16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8)) : qf[C::Q_LDS ? 0 : rt][kk];
+            const bf16x8_t qx = C::Q_LDS ? as_frag(ld16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8)) : qf[rt][kk];
             s[a][rt] = mfma16x16x32(kx, qx, s[a][rt]);
           }
         }
       }
-      const float f[4] = {ks[a].x, ks[a].y, ks[a].z, ks[a].w};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) kf[a][r] = C::WIDE ? p.scale : f[r] * p.scale;
     }
-    load_k(t + 4);
-    // scores less the running maximum; where one is above it by more than RAISE, the maximum of this tile becomes the new one
-    float top[RT];
-    bool raise = false;
+  };
+  // scores of tile t, whose V is in registers
+  auto judge = [&](int t, f32x4_t (&s)[2][RT], const float4 (&factors)[2], auto edge) {
+    scores<decltype(edge)::value, C::WIDE, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, w.kend, limit, m, l, high, acc);
+    if constexpr (decltype(edge)::value) {   // V of keys outside the range: anything (E4M3's NaN too), so zeros
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
+      for (int a = 0; a < 2; ++a) {
+        if constexpr (C::WIDE) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+          for (int i = 0; i < C::LOADS; ++i) {
+            const int key = 32 * t + 16 * a + (lane + 64 * i) / (D / 8);
+            if (key < w.kbeg || key >= w.kend) vr[a][i] = make_uint4(0, 0, 0, 0);
+          }
+        } else {
+          uint32_t keep = 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[a][rt][r] = fmaf(s[a][rt][r], kf[a][r], -m[rt]);
-      if (edge) {
+          for (int r = 0; r < 4; ++r) {
+            const int key = 32 * t + 16 * a + 4 * g + r;
+            keep |= key >= w.kbeg && key < w.kend ? 0xFFu << (8 * r) : 0u;
+          }
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[a][rt][r] = sees(rt, a, r) ? s[a][rt][r] : -INFINITY;
-      }
-      top[rt] = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
-                      fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
-      raise = raise || top[rt] > high[rt];
-    }
-    if (__any(raise)) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const bool first = high[rt] == -INFINITY;
-        float up = join_groups(top[rt], [](float x, float y) { return fmaxf(x, y); });
-        if (first) high[rt] = up == -INFINITY ? up : RAISE;
-        up = first && up != -INFINITY ? up : fmaxf(up, 0.f);
-        const float alpha = first ? 1.f : exp2_fast(-up);
-        m[rt] += up;
-        l[rt] *= alpha;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[a][rt][r] -= up;
-#pragma unroll
-        for (int mt = 0; mt < C::MT; ++mt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[rt][mt][r] *= alpha;
-      }
-    }
-    bf16x8_t pf[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[a][rt][r] = exp2_fast(s[a][rt][r]);
-          l[rt] += s[a][rt][r];
-        }
-      if constexpr (!C::WIDE) {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const float f[4] = {vs[a].x, vs[a].y, vs[a].z, vs[a].w};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[a][rt][r] *= f[r];
-        }
-        if (edge) {   // (the scale of a key that a row does not see may be anything)
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[a][rt][r] = sees(rt, a, r) ? s[a][rt][r] : 0.f;
+          for (int i = 0; i < C::LOADS; ++i) vr[a][i] = make_uint4(vr[a][i].x & keep, vr[a][i].y & keep, vr[a][i].z & keep, vr[a][i].w & keep);
         }
       }
-      pf[rt] = as_frag(make_uint4(pack2(s[0][rt][0], s[0][rt][1]), pack2(s[0][rt][2], s[0][rt][3]),
-                                  pack2(s[1][rt][0], s[1][rt][1]), pack2(s[1][rt][2], s[1][rt][3])));
     }
-    // V of keys outside the range: anything (E4M3's NaN too), so zeros
+  };
+  // The wave's tiles t0 + 4 i, in an order that leaves those at the edges (some row does not see some key) to a loop of their own:
+  // what they ask for would be selects in every tile's way, and two bodies in one loop copy the sums from one to the other
+  const int t0 = (w.kbeg >> 5) + wid, n = t0 < t_end ? (t_end - t0 + 3) >> 2 : 0;
+  const int ahead = n > 0 && 32 * t0 < w.kbeg ? 1 : 0;                         // the first tile is one: it goes last
+  const int whole = max(0, min(n, ((least >> 5) - t0 + 3) >> 2) - ahead);      // tiles that every row sees
+  auto nth = [&](int j) {                                                      // (behind the last: anything)
+    const int i = j + ahead;
+    return t0 + 4 * (i < n ? i : 0);
+  };
+  if (n > 0) {
+    find(nth(0));
+    settle();
+    load_k();
+    load_v();
+    find(nth(1));
+  }
+  auto step = [&](int j, auto edge) {
+    f32x4_t s[2][RT];
+    product(s);
+    const float4 factors[2] = {ks[0], ks[1]};
+    settle();
+    load_k();
+    judge(nth(j), s, factors, edge);
+    bf16x8_t pf[1][RT];
+    weights<C::WIDE, 2, RT>(s, vs, l, pf);
+    uint16_t* turn = reinterpret_cast<uint16_t*>(space) + wid * 32 * D;
     if constexpr (C::WIDE) {
-      uint16_t* turn = reinterpret_cast<uint16_t*>(space) + wid * 32 * D;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int i = 0; i < C::LOADS; ++i) {
           const int row = 16 * a + (lane + 64 * i) / (D / 8), ch = (lane + 64 * i) % (D / 8);
-          if (edge && (32 * t + row < w.kbeg || 32 * t + row >= w.kend)) vr[a][i] = make_uint4(0, 0, 0, 0);
           st16(turn + row * D + (ch ^ (((row & 7) << 1) & (D / 8 - 1))) * 8, vr[a][i]);
         }
-      load_v(t + 4);
-    } else if (edge) {
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        uint32_t keep = 0;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = 32 * t + 16 * a + 4 * g + r;
-          keep |= key >= w.kbeg && key < w.kend ? 0xFFu << (8 * r) : 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < C::LOADS; ++i) vr[a][i] = make_uint4(vr[a][i].x & keep, vr[a][i].y & keep, vr[a][i].z & keep, vr[a][i].w & keep);
-      }
+      load_v();
     }
 #pragma unroll
     for (int mt = 0; mt < C::MT; ++mt) {
-      bf16x8_t vf;
+      bf16x8_t vx;
       if constexpr (C::WIDE) {
-        const uint16_t* turn = reinterpret_cast<const uint16_t*>(space) + wid * 32 * D;
         const int row = 4 * g + (li >> 2), col = mt * 16 + 4 * (li & 3);
         const uint16_t* src = turn + row * D + ((col >> 3) ^ (((row & 7) << 1) & (D / 8 - 1))) * 8 + (col & 7);
         const uint2 lo = __builtin_bit_cast(uint2, lds_read_tr16(src)), hi = __builtin_bit_cast(uint2, lds_read_tr16(src + 16 * D));
-        vf = as_frag(make_uint4(lo.x, lo.y, hi.x, hi.y));
+        vx = as_frag(make_uint4(lo.x, lo.y, hi.x, hi.y));
       } else {
         const uint4 &va = vr[0][mt >> 2], &vb = vr[1][mt >> 2];
-        vf = kv_widen8<FMT>((mt & 3) == 0 ? va.x : (mt & 3) == 1 ? va.y : (mt & 3) == 2 ? va.z : va.w,
+        vx = kv_widen8<FMT>((mt & 3) == 0 ? va.x : (mt & 3) == 1 ? va.y : (mt & 3) == 2 ? va.z : va.w,
                             (mt & 3) == 0 ? vb.x : (mt & 3) == 1 ? vb.y : (mt & 3) == 2 ? vb.z : vb.w);
       }
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vf, pf[rt], acc[rt][mt]);
+      for (int rt = 0; rt < RT; ++rt) acc[rt][mt] = mfma16x16x32(vx, pf[0][rt], acc[rt][mt]);
     }
-    if constexpr (!C::WIDE) load_v(t + 4);
-  }
+    if constexpr (!C::WIDE) load_v();
+    find(nth(j + 2));
+  };
+#pragma unroll 1
+  for (int j = 0; j < whole; ++j) step(j, std::false_type{});
+#pragma unroll 1
+  for (int j = whole; j < n; ++j) step(j, std::true_type{});
 
   // ---- the four waves' states: O^T[16 mt + 4 g + r][row li] of each row tile
   float* o_lds = reinterpret_cast<float*>(space);
@@ -383,9 +463,238 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   }
 }
 
+// ---- many rows: 128 a workgroup, 32 a wave, all over the same keys ------------------------------------------------------
+// The widening of 8-bit codes is vector work, and that (with the softmax) bounds blocks of many rows, not the products: here a
+// stage of 64 keys is widened once for the workgroup's 128 rows and laid in LDS in fragment order, two stages in turn, one
+// barrier a stage. Each wave has rows of its own, so nothing is joined at the end. Ranges begin at multiples of 32 keys.
+template <int FMT, int D>
+struct BlockCfg {
+  static constexpr bool WIDE = FMT == KV_BF16;
+  static constexpr int ROWS = 128, KEYS = 64, RT = 2;
+  static constexpr int KK = D / 32, MT = D / 16;
+  static constexpr int SIDE = KEYS * D * 2;               // bytes of a stage's K, or V
+  static constexpr int STAGE = 2 * SIDE + 2 * KEYS * 4;   // and the scales
+  static constexpr int SPACE = 2 * STAGE;
+  static constexpr int RAW = WIDE ? D / 32 : D / 64;      // 16-byte loads a lane for its 16 keys of K, and as many of V
+};
+
+template <int FMT, int D>
+__device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space) {
+  using C = BlockCfg<FMT, D>;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, li = lane & 15;
+  const int row0 = w.block * C::ROWS + wid * 32;
+  int limit[C::RT], least = w.kend;
+  bf16x8_t qf[C::RT][C::KK];
+#pragma unroll
+  for (int rt = 0; rt < C::RT; ++rt) load_row<FMT, D>(p, w, kvh, row0 + rt * 16 + li, g, qf[rt], limit[rt], least);
+  int most = max(limit[0], limit[1]);
+  for (int o = 1; o < 16; o <<= 1) {
+    least = min(least, __shfl_xor(least, o, 64));
+    most = max(most, __shfl_xor(most, o, 64));
+  }
+  most = __builtin_amdgcn_readfirstlane(most);   // no row of the wave sees the keys from here on
+  int* of_waves = reinterpret_cast<int*>(space);
+  if (lane == 0) of_waves[wid] = least;
+  __syncthreads();
+  least = __builtin_amdgcn_readfirstlane(min(min(of_waves[0], of_waves[1]), min(of_waves[2], of_waves[3])));
+  __syncthreads();
+
+  float m[C::RT], l[C::RT], high[C::RT];
+  f32x4_t acc[C::RT][C::MT];
+#pragma unroll
+  for (int rt = 0; rt < C::RT; ++rt) {
+    m[rt] = l[rt] = 0.f;
+    high[rt] = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < C::MT; ++mt) acc[rt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int tpp = p.bs >> 4, last = max((w.kend + 15) / 16 - 1, 0);
+  const int stages = w.kend > w.kbeg ? (w.kend - w.kbeg + C::KEYS - 1) / C::KEYS : 0;
+  const Constant<int32_t> table = constant(p.tables + w.table * p.table_stride);
+  const uint32_t elem = C::WIDE ? 2 : 1;
+  const uint32_t page_bytes = static_cast<uint32_t>(p.Hkv) * p.bs * D * elem, page_scales = static_cast<uint32_t>(p.Hkv) * 2 * p.bs;
+  const uint8_t* k_head = p.k + static_cast<int64_t>(kvh) * p.bs * D * elem;
+  const uint8_t* v_head = p.v + static_cast<int64_t>(kvh) * p.bs * D * elem;
+  const float* s_head = p.scales + static_cast<int64_t>(kvh) * 2 * p.bs;
+  // Of a stage's four tiles, wave w brings K (and the scales) of tile w; of V, 8-bit codes of 128 dims: half w & 1 of the dims of both
+  // tiles of pair w >> 1, which a fragment has side by side; else tile w. Page numbers are asked for a stage ahead of the loads.
+  constexpr bool PAIRED = !C::WIDE && D == 128;
+  int page[2], off[2];
+  auto find = [&](int stage) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int tile = min((w.kbeg >> 4) + 4 * stage + (wid & 2) + a, last), pg = page_of(tile, p.page_magic);
+      page[a] = table[pg];
+      off[a] = (tile - pg * tpp) * 16;
+    }
+  };
+  uint4 kraw[C::RAW], vraw[C::RAW];
+  float factor = 0.f;
+  auto fetch = [&]() {
+    uint64_t at[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      page[a] = min(max(page[a], 0), p.num_blocks - 1);
+      at[a] = static_cast<uint64_t>(static_cast<uint32_t>(page[a])) * page_bytes + static_cast<uint32_t>(off[a]) * D * elem;
+    }
+    const int own = wid & 1;
+    const uint8_t* kb = k_head + (own ? at[1] : at[0]);
+#pragma unroll
+    for (int i = 0; i < C::RAW; ++i)
+      kraw[i] = ld16(kb + (C::WIDE ? static_cast<uint32_t>(li * D * 2 + 16 * g + 64 * i) : static_cast<uint32_t>(lane * 16 + 1024 * i)));
+    if constexpr (PAIRED) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) vraw[a] = ld16(v_head + at[a] + static_cast<uint32_t>(own * 1024 + lane * 16));
+    } else {
+      const uint8_t* vb = v_head + (own ? at[1] : at[0]);
+#pragma unroll
+      for (int i = 0; i < C::RAW; ++i) vraw[i] = ld16(vb + static_cast<uint32_t>(lane * 16 + 1024 * i));
+    }
+    if constexpr (!C::WIDE) {   // lanes 0 .. 15: the keys', 16 .. 31: the values'
+      const float* sc = s_head + static_cast<uint64_t>(static_cast<uint32_t>(own ? page[1] : page[0])) * page_scales +
+                        static_cast<uint32_t>(own ? off[1] : off[0]);
+      factor = sc[static_cast<uint32_t>((g & 1) * p.bs + li)];
+    }
+  };
+  auto kept = [&](int key) { return key >= w.kbeg && key < w.kend; };
+  auto lay = [&](int stage, auto edge) {
+    uint8_t* kd = space + (stage & 1) * C::STAGE;
+    uint8_t* vd = kd + C::SIDE;
+    const int key0 = w.kbeg + stage * C::KEYS;
+    if constexpr (C::WIDE) {
+#pragma unroll
+      for (int i = 0; i < C::RAW; ++i) {
+        st16(kd + ((wid * C::KK + i) * 64 + lane) * 16, kraw[i]);
+        const int row = 16 * wid + (lane + 64 * i) / (D / 8), ch = (lane + 64 * i) % (D / 8);
+        uint4 x = vraw[i];
+        if (decltype(edge)::value && !kept(key0 + row)) x = make_uint4(0, 0, 0, 0);
+        st16(vd + (row * (D / 8) + (ch ^ (((row & 7) << 1) & (D / 8 - 1)))) * 16, x);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::RAW; ++i) {
+        st16(kd + ((wid * C::KK + 2 * i) * 64 + lane) * 16, __builtin_bit_cast(uint4, kv_widen8<FMT>(kraw[i].x, kraw[i].y)));
+        st16(kd + ((wid * C::KK + 2 * i + 1) * 64 + lane) * 16, __builtin_bit_cast(uint4, kv_widen8<FMT>(kraw[i].z, kraw[i].w)));
+      }
+      if constexpr (decltype(edge)::value) {   // V of keys outside the range may be anything (E4M3's NaN too): zeros
+#pragma unroll
+        for (int a = 0; a < C::RAW; ++a) {
+          const int tile = PAIRED ? (wid & 2) + a : wid;
+          uint32_t keep = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) keep |= kept(key0 + 16 * tile + 4 * g + r) ? 0xFFu << (8 * r) : 0u;
+          vraw[a] = make_uint4(vraw[a].x & keep, vraw[a].y & keep, vraw[a].z & keep, vraw[a].w & keep);
+        }
+      }
+      if constexpr (PAIRED) {
+        const uint32_t x[4] = {vraw[0].x, vraw[0].y, vraw[0].z, vraw[0].w}, y[4] = {vraw[1].x, vraw[1].y, vraw[1].z, vraw[1].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st16(vd + (((wid >> 1) * C::MT + (wid & 1) * 4 + i) * 64 + lane) * 16, __builtin_bit_cast(uint4, kv_widen8<FMT>(x[i], y[i])));
+      } else {
+        const uint32_t x[4] = {vraw[0].x, vraw[0].y, vraw[0].z, vraw[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint2*>(vd + (((wid >> 1) * C::MT + i) * 64 + lane) * 16 + (wid & 1) * 8) = kv_widen4<FMT>(x[i]);
+      }
+      if (lane < 32) reinterpret_cast<float*>(kd + 2 * C::SIDE)[g * C::KEYS + wid * 16 + li] = factor;
+    }
+  };
+  if (stages > 0) {
+    find(0);
+    fetch();
+    find(1);   // (stages behind the last: clamped to its last tile, and unused)
+    lay(0, std::true_type{});
+    fetch();
+    find(2);
+  }
+  __syncthreads();
+  auto step = [&](int stage, auto edge) {
+    lay(stage + 1, edge);
+    fetch();
+    find(stage + 3);
+    const uint8_t* kd = space + (stage & 1) * C::STAGE;
+    const uint8_t* vd = kd + C::SIDE;
+    const float* sd = reinterpret_cast<const float*>(kd + 2 * C::SIDE) + 4 * g;
+    const int key0 = w.kbeg + stage * C::KEYS;
+    if (!decltype(edge)::value || key0 < most) {
+      f32x4_t s[4][C::RT];
+      float4 ks[4], vs[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+#pragma unroll
+        for (int rt = 0; rt < C::RT; ++rt) s[a][rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < C::KK; ++kk) {
+          const bf16x8_t kx = as_frag(ld16(kd + ((a * C::KK + kk) * 64 + lane) * 16));
+#pragma unroll
+          for (int rt = 0; rt < C::RT; ++rt) s[a][rt] = mfma16x16x32(kx, qf[rt][kk], s[a][rt]);
+        }
+        if constexpr (!C::WIDE) {
+          ks[a] = *reinterpret_cast<const float4*>(sd + 16 * a);
+          vs[a] = *reinterpret_cast<const float4*>(sd + C::KEYS + 16 * a);
+        }
+      }
+      scores<decltype(edge)::value, C::WIDE, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, w.kend, limit, m, l, high, acc);
+      bf16x8_t pf[2][C::RT];
+      weights<C::WIDE, 4, C::RT>(s, vs, l, pf);
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
+          bf16x8_t vx;
+          if constexpr (C::WIDE) {
+            const int row = 32 * half + 4 * g + (li >> 2), col = mt * 16 + 4 * (li & 3);
+            const uint16_t* src = reinterpret_cast<const uint16_t*>(vd) + row * D +
+                                  ((col >> 3) ^ (((row & 7) << 1) & (D / 8 - 1))) * 8 + (col & 7);
+            const uint2 lo = __builtin_bit_cast(uint2, lds_read_tr16(src)), hi = __builtin_bit_cast(uint2, lds_read_tr16(src + 16 * D));
+            vx = as_frag(make_uint4(lo.x, lo.y, hi.x, hi.y));
+          } else {
+            vx = as_frag(ld16(vd + ((half * C::MT + mt) * 64 + lane) * 16));
+          }
+#pragma unroll
+          for (int rt = 0; rt < C::RT; ++rt) acc[rt][mt] = mfma16x16x32(vx, pf[half][rt], acc[rt][mt]);
+        }
+    }
+    __syncthreads();
+  };
+  // stages that every row sees (and whose next one ends within the range), then the others: two loops, as above
+  const int whole = max(0, min(min((least - w.kbeg) / C::KEYS, stages), (w.kend - w.kbeg) / C::KEYS - 1));
+#pragma unroll 1
+  for (int stage = 0; stage < whole; ++stage) step(stage, std::false_type{});
+#pragma unroll 1
+  for (int stage = whole; stage < stages; ++stage) step(stage, std::true_type{});
+
+#pragma unroll
+  for (int rt = 0; rt < C::RT; ++rt) {
+    const int r = row0 + rt * 16 + li;
+    const float sum = join_groups(l[rt], [](float x, float y) { return x + y; });
+    if (r >= w.ntok * p.G) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int tok = r / p.G, head = kvh * p.G + r - tok * p.G;
+    const int64_t at = static_cast<int64_t>(w.tok0 + tok);
+    if (p.slots == 1) {
+      uint16_t* dst = p.out + at * p.out_stride + static_cast<int64_t>(head) * D + 4 * g;
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt)
+        *reinterpret_cast<uint2*>(dst + 16 * mt) = make_uint2(pack2(acc[rt][mt][0] * inv, acc[rt][mt][1] * inv),
+                                                              pack2(acc[rt][mt][2] * inv, acc[rt][mt][3] * inv));
+    } else {
+      const int64_t part = (at * p.Hq + head) * p.slots + w.slot;
+#pragma unroll
+      for (int mt = 0; mt < C::MT; ++mt)
+        *reinterpret_cast<float4*>(p.part_out + part * D + 16 * mt + 4 * g) =
+            make_float4(acc[rt][mt][0] * inv, acc[rt][mt][1] * inv, acc[rt][mt][2] * inv, acc[rt][mt][3] * inv);
+      if (g == 0) p.part_lse[part] = sum == 0.f ? -INFINITY : m[rt] + __log2f(sum);
+    }
+  }
+}
+
 #define XGK_ROWS_LDS(FMT, D, RT)                                                                         \
   __shared__ __attribute__((aligned(16))) uint8_t space[RowsCfg<FMT, D, RT>::SPACE];                    \
-  __shared__ __attribute__((aligned(16))) uint16_t q_lds[RowsCfg<FMT, D, RT>::Q_LDS ? 64 * D : 8];      \
+  __shared__ __attribute__((aligned(16))) uint16_t q_lds[RowsCfg<FMT, D, RT>::Q_LDS ? 16 * RT * D : 8]; \
   __shared__ float m_lds[4][16 * RT], l_lds[4][16 * RT]
 
 // share `split` of `splits` of the 32-key tiles of [kbeg, kend)
@@ -416,8 +725,7 @@ __global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, const i
 
 // Prompt portions, causal. Grid (Hkv, blocks of rows of the longest, sequences splits). Late blocks see the most keys: first.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
-  XGK_ROWS_LDS(FMT, D, RT);
+__global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
   const int s = blockIdx.z / splits;
   RowsBlock w;
   w.tok0 = min(max(qsl[s], 0), tokens);
@@ -433,13 +741,18 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_prompt_kernel(RowsA
   share(w.kbeg, w.kend, blockIdx.z - s * splits, splits);
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
   w.slot = blockIdx.z - s * splits;
-  attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  if constexpr (RT == 8) {
+    __shared__ __attribute__((aligned(16))) uint8_t space[BlockCfg<FMT, D>::SPACE];
+    attend_block<FMT, D>(p, w, blockIdx.x, space);
+  } else {
+    XGK_ROWS_LDS(FMT, D, RT);
+    attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  }
 }
 
 // The common keys of groups of decode rows. items [n][8]: first sequence, sequences, block of rows, first key, end key, slot.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_prefix_kernel(RowsArgs p, const int32_t* items) {
-  XGK_ROWS_LDS(FMT, D, RT);
+__global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prefix_kernel(RowsArgs p, const int32_t* items) {
   const int32_t* it = items + blockIdx.y * 8;
   RowsBlock w;
   w.tok0 = w.table = it[0];
@@ -450,7 +763,13 @@ __global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_prefix_kernel(RowsA
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
   w.slot = it[5];
   w.causal0 = -1;
-  attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  if constexpr (RT == 8) {
+    __shared__ __attribute__((aligned(16))) uint8_t space[BlockCfg<FMT, D>::SPACE];
+    attend_block<FMT, D>(p, w, blockIdx.x, space);
+  } else {
+    XGK_ROWS_LDS(FMT, D, RT);
+    attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  }
 }
 
 // Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). counts (with first_free): the first counts[token]
@@ -505,8 +824,9 @@ __global__ void __launch_bounds__(256) rows_join_kernel(const float* __restrict_
 static bool rows_ok(const RowsArgs& p, int D) {
   return p.bs > 0 && p.bs % KV_TILE == 0 && p.Hkv >= 1 && p.Hq % p.Hkv == 0 && (D == 64 || D == 128) && p.width >= 1 &&
          p.num_blocks >= 1 && p.slots >= 1 && (p.slots == 1 || (p.part_out && p.part_lse)) && p.q_stride % 8 == 0 &&
-         p.out_stride % 4 == 0;
+         p.out_stride % 4 == 0 && static_cast<int64_t>(p.width) * (p.bs / KV_TILE) * (p.bs / KV_TILE) < 1 << 30;
 }
+static uint32_t page_magic(int bs) { return bs >= KV_TILE ? (1u << 31) / (bs / KV_TILE) + 1 : 1; }
 
 static void join(const RowsArgs& p, int D, int tokens, const int32_t* counts, int first_free, const int32_t* qsl, int S,
                  hipStream_t st) {
@@ -530,7 +850,7 @@ int quant_decode_attention(int fmt, const uint16_t* q, int64_t q_stride, const u
                            int num_blocks, float scale, int splits, hipStream_t st) {
   if (B <= 0) return 0;
   const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
-                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits};
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits, page_magic(bs)};
   const int blocks = (p.G + 15) / 16;
   if (!rows_ok(p, D) || static_cast<int64_t>(B) * blocks > 65535 || splits > 65535) return -1;
 #define XGK_GO(F, DD)                                                                                                   \
@@ -551,8 +871,8 @@ int quant_prefill_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
                             int Hq, int Hkv, int D, int bs, int num_blocks, float scale, int RT, int splits, hipStream_t st) {
   if (tokens <= 0 || S <= 0 || max_q <= 0) return 0;
   const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
-                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits};
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 4)) return -1;
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits, page_magic(bs)};
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8)) return -1;
   const int64_t blocks = (static_cast<int64_t>(max_q) * p.G + 16 * RT - 1) / (16 * RT);
   if (blocks > 65535 || static_cast<int64_t>(S) * splits > 65535) return -1;
   const dim3 grid(Hkv, static_cast<unsigned>(blocks), S * splits);
@@ -560,7 +880,7 @@ int quant_prefill_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
   {                                                                                                                          \
     if (RT == 1) hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 1>), grid, dim3(256), 0, st, p, qsl, tokens, splits);         \
     else if (RT == 2) hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 2>), grid, dim3(256), 0, st, p, qsl, tokens, splits);    \
-    else hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 4>), grid, dim3(256), 0, st, p, qsl, tokens, splits);                 \
+    else hipLaunchKernelGGL((rows_prompt_kernel<F, DD, 8>), grid, dim3(256), 0, st, p, qsl, tokens, splits);                 \
   }
   XGK_FMT_DIM(XGK_GO) else return -1;
 #undef XGK_GO
@@ -578,9 +898,9 @@ int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
   if (B <= 0) return 0;
   const RowsArgs p{q, q_stride, static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), scales, tables, table_stride,
                    width, num_blocks, seq_lens, part_out, part_lse, out, out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs,
-                   scale * 1.44269504088896341f, prefix_slots + splits};
+                   scale * 1.44269504088896341f, prefix_slots + splits, page_magic(bs)};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 4) || splits < 1 || splits > 65535 || prefix_slots < 0 || n_items < 0 ||
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8) || splits < 1 || splits > 65535 || prefix_slots < 0 || n_items < 0 ||
       n_items > 65535 || static_cast<int64_t>(B) * blocks > 65535)
     return -1;
 #define XGK_GO(F, DD)                                                                                                      \
@@ -588,7 +908,7 @@ int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
     if (n_items > 0) {                                                                                                     \
       if (RT == 1) hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 1>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);     \
       else if (RT == 2) hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 2>), dim3(Hkv, n_items), dim3(256), 0, st, p, items); \
-      else hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 4>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);             \
+      else hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 8>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);             \
     }                                                                                                                      \
     hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, prefix, blocks,     \
                        splits, prefix_slots);                                                                              \

@@ -79,22 +79,44 @@ class QuantKVCache:
         _need(tuple(self.scales.shape) == (nb, hkv, 2, bs), "scales must be [num_blocks, Hkv, 2, block_size]")
         _need(all(t.is_contiguous() for t in (self.k, self.v, self.scales)), "a cache is contiguous")
         _need(self.k.device == self.v.device == self.scales.device, "a cache is on one device")
-
-    num_blocks = property(lambda self: self.k.shape[0])
-    num_kv_heads = property(lambda self: self.k.shape[1])
-    block_size = property(lambda self: self.k.shape[2])
-    head_dim = property(lambda self: self.k.shape[3])
-    device = property(lambda self: self.k.device)
+        self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = self.dims = nb, hkv, bs, d
+        self.device, self.code = self.k.device, KV_FORMATS[self.fmt]
+        self.index = self.k.get_device()   # -1: host
 
     def nbytes(self) -> int:
         return self.k.numel() + self.v.numel() + 4 * self.scales.numel()
 
 
 def _native(cache_tensor: torch.Tensor) -> bool:
-    if not use_native(cache_tensor):
+    if not cache_tensor.is_cuda or not use_native(cache_tensor):
         return False
-    _need(on_current_device(cache_tensor), f"the cache is on {cache_tensor.device}, which is not the current device")
+    if not on_current_device(cache_tensor):
+        raise ValueError(f"the cache is on {cache_tensor.device}, which is not the current device")
     return True
+
+
+# Arguments are looked over twice: `_plain_*` ask once whether all is as it nearly always is (a call of a decode step is
+# mostly host time), and where it is not, `_check_*` allow it or say what is wrong.
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _plain_heads(t: torch.Tensor, index: int, D: int, step: int, align: int) -> bool:
+    """[tokens, heads, D] bf16 whose tokens begin at multiples of `step` elements, the first of `align` bytes."""
+    st = t.stride()
+    return (len(st) == 3 and st[2] == 1 and st[1] == D and st[0] % step == 0 and t.shape[2] == D and t.dtype is _BF16
+            and t.get_device() == index and t.data_ptr() % align == 0)
+
+
+def _plain_lists(index: int, n: int, *lists: torch.Tensor) -> bool:
+    for t in lists:
+        if t.dtype is not _I32 or t.shape != (n,) or t.stride() != (1,) or t.get_device() != index:
+            return False
+    return True
+
+
+def _plain_table(t: torch.Tensor, index: int, rows: int) -> bool:
+    st = t.stride()
+    return len(st) == 2 and st[1] == 1 and t.shape[0] == rows and t.dtype is _I32 and t.get_device() == index and t.shape[1] > 0
 
 
 # ------------------------------------------------------------------------------------------------------ plain (CPU) forms
@@ -195,11 +217,13 @@ def _check_rows(x: torch.Tensor, name: str, cache: QuantKVCache, T: int) -> None
 def kv_quant_append(k: torch.Tensor, v: torch.Tensor, cache: QuantKVCache, slot_mapping: torch.Tensor) -> None:
     """Writes rows k, v [T, Hkv, D] bf16 (tokens may be strided: views into the projection's rows) to the cache's slots
     slot_mapping [T] int32; tokens with a slot below 0 or behind the cache are left out. A slot may occur once in a call."""
-    T = k.shape[0]
-    _check_rows(k, "k", cache, T)
-    _check_rows(v, "v", cache, T)
-    _int32(slot_mapping, "slot_mapping", 1, cache.device)
-    _need(slot_mapping.shape[0] == T, f"slot_mapping must have {T} entries")
+    T, index, D = k.shape[0], cache.index, cache.head_dim
+    if not (_plain_heads(k, index, D, D // 16, D // 8) and _plain_heads(v, index, D, D // 16, D // 8) and k.shape == v.shape
+            and k.shape[1] == cache.num_kv_heads and _plain_lists(index, T, slot_mapping)):
+        _check_rows(k, "k", cache, T)
+        _check_rows(v, "v", cache, T)
+        _int32(slot_mapping, "slot_mapping", 1, cache.device)
+        _need(slot_mapping.shape[0] == T, f"slot_mapping must have {T} entries")
     if T == 0:
         return
     if not _native(cache.k):
@@ -208,9 +232,10 @@ def kv_quant_append(k: torch.Tensor, v: torch.Tensor, cache: QuantKVCache, slot_
 
 
 def _append(cache, q, k, v, slots, positions, cos_sin, Hq) -> None:
-    kernels().kv_append(KV_FORMATS[cache.fmt], ptr(q), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(),
-                        ptr(positions), ptr(cos_sin), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
-                        cache.num_blocks, k.shape[0], Hq, cache.num_kv_heads, cache.head_dim, cache.block_size, stream_ptr())
+    nb, Hkv, bs, D = cache.dims
+    kernels().kv_append(cache.code, ptr(q), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(), ptr(positions),
+                        ptr(cos_sin), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), nb, k.shape[0], Hq, Hkv, D,
+                        bs, stream_ptr())
 
 
 def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, cache: QuantKVCache,
@@ -248,15 +273,19 @@ def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch
     """Cached rows as bf16: tokens starts[s] .. starts[s] + cu_tokens[s + 1] - cu_tokens[s] of each sequence, packed
     -> k, v [num_tokens, Hkv, D]. block_tables [S, W], starts [S], cu_tokens [S + 1] (from 0, not falling) int32; num_tokens =
     cu_tokens[S]. Tokens behind a sequence's table have no row: theirs stay as they were in `out`."""
-    _int32(block_tables, "block_tables", 2, cache.device)
-    _int32(starts, "starts", 1, cache.device)
-    _int32(cu_tokens, "cu_tokens", 1, cache.device)
-    S, W = block_tables.shape
-    _need(starts.shape[0] == S and cu_tokens.shape[0] == S + 1, "starts must have an entry a sequence, cu_tokens one more")
-    _need(num_tokens >= 0, "num_tokens must not be negative")
-    shape = (num_tokens, cache.num_kv_heads, cache.head_dim)
+    nb, Hkv, bs, D = cache.dims
+    S, index = starts.shape[0], cache.index
+    if not (_plain_table(block_tables, index, S) and _plain_lists(index, S, starts) and _plain_lists(index, S + 1, cu_tokens)
+            and num_tokens >= 0):
+        _int32(block_tables, "block_tables", 2, cache.device)
+        _int32(starts, "starts", 1, cache.device)
+        _int32(cu_tokens, "cu_tokens", 1, cache.device)
+        _need(block_tables.shape[0] == S and cu_tokens.shape[0] == S + 1, "starts must have an entry a sequence, cu_tokens one more")
+        _need(num_tokens >= 0, "num_tokens must not be negative")
+    W, shape = block_tables.shape[1], (num_tokens, Hkv, D)
     if out is None:
-        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+        k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for t in (k, v):
@@ -271,10 +300,9 @@ def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch
             if n > 0:
                 k[a:a + n], v[a:a + n] = _rows_ref(cache, _slots_ref(block_tables[s], cache.block_size, lo, lo + n, cache.num_blocks))
         return k, v
-    kernels().kv_read(KV_FORMATS[cache.fmt], cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
-                      block_tables.data_ptr(), block_tables.stride(0), W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens,
-                      cache.num_blocks, cache.num_kv_heads, cache.head_dim, cache.block_size, k.data_ptr(), v.data_ptr(),
-                      stream_ptr())
+    kernels().kv_read(cache.code, cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), block_tables.data_ptr(),
+                      block_tables.stride(0), W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens, nb, Hkv, D, bs,
+                      k.data_ptr(), v.data_ptr(), stream_ptr())
     return k, v
 
 
@@ -292,7 +320,7 @@ def _check_q(q: torch.Tensor, Hkv: int, D: int, device) -> None:
 
 def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.dtype != q.dtype:
         raise TypeError(f"out must be {q.dtype}, got {out.dtype}")
     _need(out.shape == q.shape and out.device == q.device, f"out must be {list(q.shape)} beside q")
@@ -309,29 +337,35 @@ def _check_tables(block_tables, seq_lens, device, S: int) -> None:
     _need(block_tables.shape[1] >= 1 or S == 0, "block_tables must have a column")
 
 
-def _splits(wgs: int, max_keys: int) -> int:
+def _check_decode(q, Hkv: int, D: int, index: int, device, block_tables, seq_lens) -> None:
+    """q, tables and lengths of a step with one new token of each sequence."""
+    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 and _plain_table(block_tables, index, q.shape[0])
+            and _plain_lists(index, q.shape[0], seq_lens)):
+        _check_q(q, Hkv, D, device)
+        _check_tables(block_tables, seq_lens, device, q.shape[0])
+
+
+def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
     """Parts of the key range: enough workgroups to fill the chip, each with a tile for each of its waves."""
-    want = -(-SPLIT_WGS // max(1, wgs))
-    return max(1, min(want, -(-max_keys // SPLIT_KEYS), MAX_SPLITS))
+    if num_splits is None:
+        return max(1, min(-(-SPLIT_WGS // max(1, wgs)), -(-max_keys // SPLIT_KEYS), MAX_SPLITS))
+    if not 1 <= num_splits <= MAX_SPLITS:
+        raise ValueError(f"num_splits must be 1 to {MAX_SPLITS}, got {num_splits}")
+    return int(num_splits)
 
 
-def _parts(workspace: Optional[DecodeWorkspace], tokens: int, Hq: int, D: int, slots: int, device):
-    """Pointers (and the owner) of the parts' buffers."""
+def _parts(workspace: Optional[DecodeWorkspace], rows: int, D: int, slots: int, device):
+    """The parts' buffer and the addresses of outputs and log-sums in it; rows: tokens times query heads."""
     if slots <= 1:
         return None, 0, 0
     if workspace is None:
-        workspace = DecodeWorkspace(tokens, Hq, D, slots, device)
-    _need(workspace.part_lse.device == device and workspace.part_lse.numel() >= tokens * Hq * slots
-          and workspace.part_out.numel() >= tokens * Hq * slots * D,
-          f"the workspace is too small for {slots} parts of {tokens} tokens of {Hq} heads of {D}, or on another device")
+        buf = torch.empty(rows * slots * (D + 1), dtype=torch.float32, device=device)
+        at = buf.data_ptr()
+        return buf, at, at + 4 * rows * slots * D
+    if (workspace.part_lse.device != device or workspace.part_lse.numel() < rows * slots
+            or workspace.part_out.numel() < rows * slots * D):
+        raise ValueError(f"the workspace is too small for {slots} parts of {rows} rows of {D}, or on another device")
     return workspace, workspace.part_out.data_ptr(), workspace.part_lse.data_ptr()
-
-
-def _num_splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
-    if num_splits is None:
-        return _splits(wgs, max_keys)
-    _need(1 <= num_splits <= MAX_SPLITS, f"num_splits must be 1 to {MAX_SPLITS}, got {num_splits}")
-    return int(num_splits)
 
 
 def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, seq_lens: torch.Tensor, scale: float,
@@ -340,13 +374,12 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     """`decode_attention` over an 8-bit cache: q [B, Hq, D] bf16 (tokens may be strided), one new token of each sequence, whose own
     key is in the cache already -> [B, Hq, D]. block_tables [B, W], seq_lens [B] int32; a length of 0 gives zeros, one behind the
     table means the whole table. num_splits: parts of the key range (None: by the batch and the table's width)."""
-    Hkv, D, bs, dev = cache.num_kv_heads, cache.head_dim, cache.block_size, cache.device
-    _check_q(q, Hkv, D, dev)
+    (nb, Hkv, bs, D), dev = cache.dims, cache.device
+    _check_decode(q, Hkv, D, cache.index, dev, block_tables, seq_lens)
     B, Hq, _ = q.shape
-    _check_tables(block_tables, seq_lens, dev, B)
     out = _check_out(out, q)
     W = block_tables.shape[1]
-    splits = _num_splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs)
+    splits = _splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs)
     if B == 0:
         return out
     if not _native(cache.k):
@@ -357,17 +390,17 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
                 k, v = _any_rows_ref(cache, block_tables[b], 0, L)
                 out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
         return out
-    keep, po, pl = _parts(workspace, B, Hq, D, splits, dev)
-    kernels().quant_decode_attention(KV_FORMATS[cache.fmt], q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
+    keep, po, pl = _parts(workspace, B * Hq, D, splits, dev)
+    kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
-                                     seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs,
-                                     cache.num_blocks, float(scale), splits, stream_ptr())
+                                     seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale,
+                                     splits, stream_ptr())
     return out
 
 
 def _row_tiles(rows: int, D: int) -> int:
     """16-row tiles of a workgroup: as many as the rows fill and the registers hold."""
-    return 1 if rows <= 16 else 2 if rows <= 32 or D == 128 else 4
+    return 1 if rows <= 16 else 2 if rows <= 32 else 8
 
 
 def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
@@ -376,22 +409,26 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
     """`prefill_attention` over an 8-bit cache: q [T, Hq, D] bf16 packed; sequence s has the tokens query_start_loc[s] ..
     query_start_loc[s + 1], the last of its seq_lens[s], and each sees the keys up to its own, all of them in the cache already.
     max_q_len: at least the tokens of the longest portion. Rows of no sequence stay as they were in `out`."""
-    Hkv, D, bs, dev = cache.num_kv_heads, cache.head_dim, cache.block_size, cache.device
-    _check_q(q, Hkv, D, dev)
-    T, Hq, _ = q.shape
+    (nb, Hkv, bs, D), dev, index = cache.dims, cache.device, cache.index
     S = seq_lens.shape[0]
-    _check_tables(block_tables, seq_lens, dev, S)
-    _int32(query_start_loc, "query_start_loc", 1, dev)
-    _need(query_start_loc.shape[0] == S + 1, "query_start_loc must have one entry more than seq_lens")
-    _need(0 <= max_q_len, "max_q_len must not be negative")
+    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 and _plain_table(block_tables, index, S)
+            and _plain_lists(index, S, seq_lens) and _plain_lists(index, S + 1, query_start_loc) and max_q_len >= 0):
+        _check_q(q, Hkv, D, dev)
+        _check_tables(block_tables, seq_lens, dev, S)
+        _int32(query_start_loc, "query_start_loc", 1, dev)
+        _need(query_start_loc.shape[0] == S + 1, "query_start_loc must have one entry more than seq_lens")
+        _need(0 <= max_q_len, "max_q_len must not be negative")
+    T, Hq, _ = q.shape
     out = _check_out(out, q)
     if T == 0 or S == 0 or max_q_len == 0:
         return out
     W, G = block_tables.shape[1], Hq // Hkv
     max_q_len = min(max_q_len, T)
     rt = _row_tiles(max_q_len * G, D)
-    splits = _num_splits(num_splits, S * Hkv * -(-max_q_len * G // (16 * rt)), W * bs)
-    _need(S * splits <= 65535 and -(-max_q_len * G // (16 * rt)) <= 65535, "at most 65535 sequences (times splits), or blocks of rows")
+    blocks = -(-max_q_len * G // (16 * rt))
+    splits = _splits(num_splits, S * Hkv * blocks, W * bs)
+    if S * splits > 65535 or blocks > 65535:
+        raise ValueError("at most 65535 sequences (times splits), and blocks of rows")
     if not _native(cache.k):
         for s in range(S):
             a, b = int(query_start_loc[s]), int(query_start_loc[s + 1])
@@ -400,11 +437,11 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
                 k, v = _any_rows_ref(cache, block_tables[s], 0, min(L, W * bs))
                 out[a:a + n] = _attend_causal(q[a:a + n], k, v, max(L - (b - a), 0), scale).to(q.dtype)
         return out
-    keep, po, pl = _parts(workspace, T, Hq, D, splits, dev)
-    kernels().quant_prefill_attention(KV_FORMATS[cache.fmt], q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
+    keep, po, pl = _parts(workspace, T * Hq, D, splits, dev)
+    kernels().quant_prefill_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
                                       cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
                                       query_start_loc.data_ptr(), seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), T, S,
-                                      int(max_q_len), Hq, Hkv, D, bs, cache.num_blocks, float(scale), rt, splits, stream_ptr())
+                                      max_q_len, Hq, Hkv, D, bs, nb, scale, rt, splits, stream_ptr())
     return out
 
 
@@ -422,6 +459,8 @@ class SharedPrefixPlan:
     counts: torch.Tensor         # [num_seqs] int32: its parts
     group_sizes: Tuple[int, ...]
     prefix_lens: Tuple[int, ...]
+    shortest: int                # prefix
+    longest: int
 
 
 def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], num_heads: int, num_kv_heads: int,
@@ -456,7 +495,7 @@ def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], n
         return torch.tensor(rows, dtype=torch.int32).reshape(-1, *width).to(device)
 
     return SharedPrefixPlan(at, num_heads, num_kv_heads, rt, max(counts, default=0), put(items, (8,)), put(prefix, ()), put(counts, ()),
-                            tuple(sizes), tuple(lens))
+                            tuple(sizes), tuple(lens), min(lens, default=0), max(lens, default=0))
 
 
 def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch.Tensor, torch.Tensor]], block_tables: torch.Tensor,
@@ -468,27 +507,28 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
     D]. num_splits: parts of the keys behind the prefix. A workspace needs plan.slots + num_splits parts."""
     quant = isinstance(kv, QuantKVCache)
     if quant:
-        kc, vc, nb, Hkv, bs, D, fmt = kv.k, kv.v, kv.num_blocks, kv.num_kv_heads, kv.block_size, kv.head_dim, KV_FORMATS[kv.fmt]
+        kc, vc, (nb, Hkv, bs, D), fmt = kv.k, kv.v, kv.dims, kv.code
     else:
         kc, vc = kv
-        if kc.dtype != torch.bfloat16 or vc.dtype != torch.bfloat16:
+        if kc.dtype is not torch.bfloat16 or vc.dtype is not torch.bfloat16:
             raise TypeError("kv must be a QuantKVCache or bfloat16 pages")
-        _need(kc.dim() == 4 and kc.shape == vc.shape and kc.is_contiguous() and vc.is_contiguous() and kc.device == vc.device
-              and kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0, "pages must be contiguous [NB, Hkv, bs, D] alike")
+        if not (kc.dim() == 4 and kc.shape == vc.shape and kc.is_contiguous() and vc.is_contiguous()
+                and kc.get_device() == vc.get_device() and kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0):
+            raise ValueError("pages must be contiguous [NB, Hkv, bs, D] alike")
         (nb, Hkv, bs, D), fmt = kc.shape, KV_BF16
-        _need(D in (64, 128) and bs >= TILE and bs % TILE == 0 and nb >= 1,
-              f"heads of 64 or 128 numbers in pages of a multiple of {TILE} tokens")
+        if D not in (64, 128) or bs < TILE or bs % TILE or nb < 1 or Hkv < 1:
+            raise ValueError(f"heads of 64 or 128 numbers in pages of a multiple of {TILE} tokens")
     dev = kc.device
-    _check_q(q, Hkv, D, dev)
+    _check_decode(q, Hkv, D, kc.get_device(), dev, block_tables, seq_lens)
     B, Hq, _ = q.shape
-    _check_tables(block_tables, seq_lens, dev, B)
-    _need((plan.num_seqs, plan.num_heads, plan.num_kv_heads) == (B, Hq, Hkv),
-          f"the plan is for {plan.num_seqs} sequences of {plan.num_heads} / {plan.num_kv_heads} heads, not {B} of {Hq} / {Hkv}")
-    _need(plan.prefix.device == dev, f"the plan is on {plan.prefix.device}, the cache on {dev}")
     W = block_tables.shape[1]
-    _need(max(plan.prefix_lens, default=0) <= W * bs, "a prefix is longer than the tables")
+    if plan.num_seqs != B or plan.num_heads != Hq or plan.num_kv_heads != Hkv:
+        raise ValueError(f"the plan is for {plan.num_seqs} sequences of {plan.num_heads} / {plan.num_kv_heads} heads, not {B} of {Hq} / {Hkv}")
+    if plan.prefix.device != dev or plan.longest > W * bs:
+        raise ValueError(f"the plan is on {plan.prefix.device}, the cache on {dev}" if plan.prefix.device != dev
+                         else "a prefix is longer than the tables")
     out = _check_out(out, q)
-    splits = _num_splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs - min(plan.prefix_lens, default=0))
+    splits = _splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs - plan.shortest)
     if B == 0:
         return out
     if not _native(kc):
@@ -503,10 +543,10 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
                     out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
             at += n
         return out
-    keep, po, pl = _parts(workspace, B, Hq, D, plan.slots + splits, dev)
+    keep, po, pl = _parts(workspace, B * Hq, D, plan.slots + splits, dev)
     kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride(0), kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
                                       block_tables.data_ptr(), block_tables.stride(0), W, seq_lens.data_ptr(), po, pl,
-                                      out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, float(scale), plan.items.data_ptr(),
+                                      out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale, plan.items.data_ptr(),
                                       plan.items.shape[0], plan.prefix.data_ptr(), plan.counts.data_ptr(), plan.slots,
                                       plan.row_tiles, splits, stream_ptr())
     return out
