@@ -126,6 +126,18 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
     }
     return;
   }
+  auto row_of = [&](int t, bool value, uint16_t (&x)[N]) {
+    const uint16_t* src = value ? p.v + static_cast<int64_t>(t) * p.v_stride : p.k + static_cast<int64_t>(t) * p.k_stride;
+    kv_load_row<N>(src + static_cast<int64_t>(head) * D + c * N, x);
+  };
+  auto turned = [&](int t, uint16_t (&x)[N]) {
+    if (ROPE) kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
+  };
+  // the window's own rows are on their way before its slots are known (a quad mostly begins with the window)
+  uint16_t xk[N], xv[N];
+  const int own = min(t0 + i, p.T - 1);
+  row_of(own, false, xk);
+  row_of(own, true, xv);
   // slots of the tokens around the window, -1 where there is none
   int s[10];
 #pragma unroll
@@ -145,11 +157,6 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
       for (int j = 0; j < 4; ++j)
         if (b + j >= 3 && b + j < 7) taken |= 1u << (b + j - 3);
     }
-  auto row_of = [&](int t, bool value, uint16_t (&x)[N]) {
-    const uint16_t* src = value ? p.v + static_cast<int64_t>(t) * p.v_stride : p.k + static_cast<int64_t>(t) * p.k_stride;
-    kv_load_row<N>(src + static_cast<int64_t>(head) * D + c * N, x);
-    if (ROPE && !value) kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
-  };
   auto tile_of = [&](int slot, int64_t& scale_at) {
     const int64_t page = slot / p.bs;
     const int off = slot % p.bs;
@@ -165,12 +172,17 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
     const int slot = p.slots[quad] + i;
     int64_t at;
     const int64_t tile = tile_of(slot, at);
-    uint16_t xk[N], xv[N];
-    row_of(quad + i, false, xk);
-    row_of(quad + i, true, xv);
+    uint16_t yk[N], yv[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) { yk[j] = xk[j]; yv[j] = xv[j]; }
+    if (quad != t0) {
+      row_of(quad + i, false, yk);
+      row_of(quad + i, true, yv);
+    }
+    turned(quad + i, yk);
     float sk, sv;
-    put_k(kv_quantise<FMT, N>(xk, sk), slot, tile);
-    const Codes<N> w = kv_quantise<FMT, N>(xv, sv);
+    put_k(kv_quantise<FMT, N>(yk, sk), slot, tile);
+    const Codes<N> w = kv_quantise<FMT, N>(yv, sv);
     if (c == 0) {
       p.scales[at] = sk;
       p.scales[at + p.bs] = sv;
@@ -197,9 +209,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
   if (!(taken >> i & 1) && slot >= 0) {   // (16 lanes are of one mind: the rotations within them stay whole)
     int64_t at;
     const int64_t tile = tile_of(slot, at);
-    uint16_t xk[N], xv[N];
-    row_of(t0 + i, false, xk);
-    row_of(t0 + i, true, xv);
+    turned(own, xk);
     float sk, sv;
     put_k(kv_quantise<FMT, N>(xk, sk), slot, tile);
     const Codes<N> w = kv_quantise<FMT, N>(xv, sv);

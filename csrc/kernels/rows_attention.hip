@@ -70,8 +70,9 @@ struct RowsBlock {
   int table;              // row of `tables`
   int kbeg, kend;         // keys
   int slot;               // of the rows' parts
-  int causal0;            // >= 0: token i sees keys < causal0 + i + 1; -1: keys < seq_lens of its own, and of kend
+  int causal0;            // >= 0: token i sees keys < causal0 + i + 1; OWN: those below its seq_lens; ALL: all (below kend, each)
 };
+enum : int { OWN = -1, ALL = -2 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -99,7 +100,6 @@ struct RowsCfg {
   static constexpr int KK = D / 32;                  // matrix instructions over the head size
   static constexpr int MT = D / 16;                  // 16-dim tiles of the output
   static constexpr int LOADS = WIDE ? D / 32 : D / 64;   // 16-byte loads a lane, 16 tokens of K or V
-  static constexpr bool Q_LDS = false;   // 32 registers fewer: three waves a SIMD instead of two
   static constexpr int OROW = D + 4;                 // row of the joining buffer (padded: banks)
   static constexpr int JOIN = 4 * 16 * OROW * 4;     // bytes
   static constexpr int TURN = WIDE ? 4 * 32 * D * 2 : 0;
@@ -209,8 +209,11 @@ __device__ __forceinline__ void load_row(const RowsArgs& p, const RowsBlock& w, 
   const int tok = real ? r / p.G : 0, head = kvh * p.G + (real ? r - tok * p.G : 0);
   limit = 0;
   if (real) {
-    limit = min(w.kend, w.causal0 >= 0 ? w.causal0 + tok + 1 : p.seq_lens[w.tok0 + tok]);
-    least = min(least, limit);
+    limit = w.kend;
+    if (w.causal0 != ALL) {
+      limit = min(limit, w.causal0 >= 0 ? w.causal0 + tok + 1 : p.seq_lens[w.tok0 + tok]);
+      least = min(least, limit);
+    }
   }
   const uint16_t* qp = p.q + static_cast<int64_t>(w.tok0 + tok) * p.q_stride + static_cast<int64_t>(head) * D;
 #pragma unroll
@@ -221,28 +224,12 @@ __device__ __forceinline__ void load_row(const RowsArgs& p, const RowsBlock& w, 
 }
 
 template <int FMT, int D, int RT, bool ONCE>
-__device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space, uint16_t* q_lds,
+__device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space,
                                             float (*m_lds)[16 * RT], float (*l_lds)[16 * RT]) {
   using C = RowsCfg<FMT, D, RT>;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, li = lane & 15;
   const int nrows = w.ntok * p.G, row0 = w.block * 16 * RT;
-
-  // rows: fragments of Q, and the keys that each sees
-  int limit[RT];
-  int least = w.kend;   // every row sees the keys below
-  bf16x8_t qf[RT][C::KK];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) load_row<FMT, D>(p, w, kvh, row0 + rt * 16 + li, g, qf[rt], limit[rt], least);
-  if constexpr (C::Q_LDS) {   // (every wave the same)
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int kk = 0; kk < C::KK; ++kk) st16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8, __builtin_bit_cast(uint4, qf[rt][kk]));
-    __syncthreads();
-  }
-  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
-  least = __builtin_amdgcn_readfirstlane(least);
 
   float m[RT], l[RT], high[RT];   // running maximum and sum; what a score has to pass to raise it: anything, before the first key
   f32x4_t acc[RT][C::MT];
@@ -259,8 +246,9 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   const Constant<int32_t> table = constant(p.tables + w.table * p.table_stride);
   uint4 kr[2][C::LOADS], vr[2][C::LOADS];
   float4 ks[2], vs[2];
-  // a decode step reads its keys once (non-temporal); blocks of rows over the same keys find them in the L2
-  auto load16 = [](const void* at) { return ONCE ? ld16_nt(at) : ld16(at); };
+  // a decode step reads its keys once (non-temporal); blocks of rows over the same keys find them in the L2. (bf16 K fragments are
+  // half lines, whose other half the next load finds in the L1: 43 us non-temporal 55, 64 rows behind a prefix of 4096)
+  auto load16 = [](const void* at) { return ONCE && !C::WIDE ? ld16_nt(at) : ld16(at); };
   // where the halves of a tile lie: clamped to the last tile that holds a key, and into the cache. The page numbers of the
   // tile after the next are asked for while the next one's loads go out, so no load waits for its address. Addresses are scalar
   // work of each tile (a third of the loop's instructions where they came from the indexes each time): one offset for K and V
@@ -307,6 +295,31 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
       if constexpr (!C::WIDE) vs[a] = *reinterpret_cast<const float4*>(factor[a] + p.bs + 4 * g);
     }
   };
+  // The wave's tiles t0 + 4 i, in an order that leaves those at the edges (some row does not see some key) to a loop of their own:
+  // what they ask for would be selects in every tile's way, and two bodies in one loop copy the sums from one to the other
+  const int t0 = (w.kbeg >> 5) + wid, n = t0 < t_end ? (t_end - t0 + 3) >> 2 : 0;
+  const int ahead = n > 0 && 32 * t0 < w.kbeg ? 1 : 0;                         // the first tile is one: it goes last
+  auto nth = [&](int j) {                                                      // (behind the last: anything)
+    const int i = j + ahead;
+    return t0 + 4 * (i < n ? i : 0);
+  };
+  if (n > 0) {
+    find(nth(0));
+    settle();
+    load_k();
+    load_v();
+    find(nth(1));
+  }
+  // rows: fragments of Q, and the keys that each sees (asked for after the first keys, which come from further away)
+  int limit[RT];
+  int least = w.kend;   // every row sees the keys below
+  bf16x8_t qf[RT][C::KK];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) load_row<FMT, D>(p, w, kvh, row0 + rt * 16 + li, g, qf[rt], limit[rt], least);
+  if (w.causal0 != ALL)
+    for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
+  const int whole = max(0, min(n, ((least >> 5) - t0 + 3) >> 2) - ahead);      // tiles that every row sees
   // S^T of the tile whose K is in registers
   auto product = [&](f32x4_t (&s)[2][RT]) {
 #pragma unroll
@@ -322,10 +335,7 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
           if constexpr (C::WIDE) kx = as_frag(kr[a][i]);
           else kx = x == 0 ? kv_widen8<FMT>(kr[a][i].x, kr[a][i].y) : kv_widen8<FMT>(kr[a][i].z, kr[a][i].w);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const bf16x8_t qx = C::Q_LDS ? as_frag(ld16(q_lds + ((rt * C::KK + kk) * 64 + lane) * 8)) : qf[rt][kk];
-            s[a][rt] = mfma16x16x32(kx, qx, s[a][rt]);
-          }
+          for (int rt = 0; rt < RT; ++rt) s[a][rt] = mfma16x16x32(kx, qf[rt][kk], s[a][rt]);
         }
       }
     }
@@ -355,22 +365,6 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
       }
     }
   };
-  // The wave's tiles t0 + 4 i, in an order that leaves those at the edges (some row does not see some key) to a loop of their own:
-  // what they ask for would be selects in every tile's way, and two bodies in one loop copy the sums from one to the other
-  const int t0 = (w.kbeg >> 5) + wid, n = t0 < t_end ? (t_end - t0 + 3) >> 2 : 0;
-  const int ahead = n > 0 && 32 * t0 < w.kbeg ? 1 : 0;                         // the first tile is one: it goes last
-  const int whole = max(0, min(n, ((least >> 5) - t0 + 3) >> 2) - ahead);      // tiles that every row sees
-  auto nth = [&](int j) {                                                      // (behind the last: anything)
-    const int i = j + ahead;
-    return t0 + 4 * (i < n ? i : 0);
-  };
-  if (n > 0) {
-    find(nth(0));
-    settle();
-    load_k();
-    load_v();
-    find(nth(1));
-  }
   auto step = [&](int j, auto edge) {
     f32x4_t s[2][RT];
     product(s);
@@ -694,7 +688,6 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
 
 #define XGK_ROWS_LDS(FMT, D, RT)                                                                         \
   __shared__ __attribute__((aligned(16))) uint8_t space[RowsCfg<FMT, D, RT>::SPACE];                    \
-  __shared__ __attribute__((aligned(16))) uint16_t q_lds[RowsCfg<FMT, D, RT>::Q_LDS ? 16 * RT * D : 8]; \
   __shared__ float m_lds[4][16 * RT], l_lds[4][16 * RT]
 
 // share `split` of `splits` of the 32-key tiles of [kbeg, kend)
@@ -705,22 +698,29 @@ __device__ __forceinline__ void share(int& kbeg, int& kend, int split, int split
   kend = min(kend, 32 * (first + min(tiles, (split + 1) * each)));
 }
 
-// One new token of each sequence. Grid (Hkv, B heads' blocks of 16, splits). starts: keys below belong to another launch.
+// One new token of sequence b, its heads' block `block` of 16: share `split` of `splits` of its keys, from `start` on.
 template <int FMT, int D>
-__global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, const int32_t* starts, int blocks, int splits, int slot0) {
-  XGK_ROWS_LDS(FMT, D, 1);
-  const int b = blockIdx.y / blocks;
+__device__ __forceinline__ void decode_block(const RowsArgs& p, int kvh, int b, int block, int start, int split, int splits, int slot,
+                                             uint8_t* space, float (*m_lds)[16], float (*l_lds)[16]) {
   RowsBlock w;
   w.tok0 = w.table = b;
   w.ntok = 1;
-  w.block = blockIdx.y - b * blocks;
+  w.block = block;
   w.kend = min(max(p.seq_lens[b], 0), p.width * p.bs);
-  w.kbeg = starts ? min(max(starts[b], 0), w.kend) : 0;
-  share(w.kbeg, w.kend, blockIdx.z, splits);
+  w.kbeg = min(max(start, 0), w.kend);
+  share(w.kbeg, w.kend, split, splits);
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
-  w.slot = slot0 + blockIdx.z;
-  w.causal0 = -1;
-  attend_rows<FMT, D, 1, true>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+  w.slot = slot;
+  w.causal0 = ALL;
+  attend_rows<FMT, D, 1, true>(p, w, kvh, space, m_lds, l_lds);
+}
+
+// One new token of each sequence. Grid (Hkv, B heads' blocks of 16, splits).
+template <int FMT, int D>
+__global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, int blocks, int splits) {
+  XGK_ROWS_LDS(FMT, D, 1);
+  const int b = blockIdx.y / blocks;
+  decode_block<FMT, D>(p, blockIdx.x, b, blockIdx.y - b * blocks, 0, blockIdx.z, splits, blockIdx.z, space, m_lds, l_lds);
 }
 
 // Prompt portions, causal. Grid (Hkv, blocks of rows of the longest, sequences splits). Late blocks see the most keys: first.
@@ -746,13 +746,23 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsA
     attend_block<FMT, D>(p, w, blockIdx.x, space);
   } else {
     XGK_ROWS_LDS(FMT, D, RT);
-    attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
+    attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, m_lds, l_lds);
   }
 }
 
-// The common keys of groups of decode rows. items [n][8]: first sequence, sequences, block of rows, first key, end key, slot.
+// Groups of decode rows with common keys, in one launch: first the common parts (items [n][8]: first sequence, sequences, block of
+// rows, first key, end key, slot), then each sequence's own keys. The first are bound by the vector and matrix work, the others by
+// HBM, and run beside each other. Grid (Hkv, n_items + B heads' blocks of 16, splits of the own keys).
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prefix_kernel(RowsArgs p, const int32_t* items) {
+__global__ void __launch_bounds__(256, 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
+                                                             int prefix_slots, int blocks, int splits) {
+  XGK_ROWS_LDS(FMT, D, RT);
+  if (blockIdx.y >= n_items) {
+    const int i = blockIdx.y - n_items, split = i % splits, row = i / splits, b = row / blocks;
+    decode_block<FMT, D>(p, blockIdx.x, b, row - b * blocks, prefix[b], split, splits, prefix_slots + split, space,
+                         reinterpret_cast<float(*)[16]>(m_lds), reinterpret_cast<float(*)[16]>(l_lds));
+    return;
+  }
   const int32_t* it = items + blockIdx.y * 8;
   RowsBlock w;
   w.tok0 = w.table = it[0];
@@ -762,59 +772,57 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prefix_kernel(RowsA
   w.kbeg = min(it[3], w.kend);
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
   w.slot = it[5];
-  w.causal0 = -1;
-  if constexpr (RT == 8) {
-    __shared__ __attribute__((aligned(16))) uint8_t space[BlockCfg<FMT, D>::SPACE];
-    attend_block<FMT, D>(p, w, blockIdx.x, space);
-  } else {
-    XGK_ROWS_LDS(FMT, D, RT);
-    attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, q_lds, m_lds, l_lds);
-  }
+  w.causal0 = OWN;
+  attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, m_lds, l_lds);
 }
 
 // Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). counts (with first_free): the first counts[token]
-// slots and those from first_free on hold parts; else all. qsl: tokens outside [qsl[0], qsl[S]) have none. A thread has four dims; a batch's loads all go out together.
+// slots and those from first_free on hold parts; else all. qsl: tokens outside [qsl[0], qsl[S]) have none. A workgroup has a row,
+// four dims a thread, and 1024 / D parts at once: 57 parts of 72 rows take 2.6 us, and took 8.3 with a row's parts one behind the
+// other in D / 4 threads.
 template <int D>
 __global__ void __launch_bounds__(256) rows_join_kernel(const float* __restrict__ part_out, const float* __restrict__ part_lse,
-                                                        uint16_t* __restrict__ out, int64_t out_stride, int rows, int Hq,
-                                                        int slots, const int32_t* __restrict__ counts, int first_free,
+                                                        uint16_t* __restrict__ out, int64_t out_stride, int Hq, int slots,
+                                                        const int32_t* __restrict__ counts, int first_free,
                                                         const int32_t* __restrict__ qsl, int S) {
-  constexpr int TPR = D / 4, BATCH = 8;
-  const int row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR, d = threadIdx.x % TPR * 4;
-  if (row >= rows) return;
-  const int tok = row / Hq, head = row - tok * Hq;
+  constexpr int TPR = D / 4, AT_ONCE = 256 / TPR;
+  __shared__ float sums[AT_ONCE], tops[AT_ONCE];
+  __shared__ __attribute__((aligned(16))) float outs[AT_ONCE][D];
+  const int64_t row = blockIdx.x;
+  const int tok = row / Hq, head = row - static_cast<int64_t>(tok) * Hq;
   if (qsl && (tok < qsl[0] || tok >= qsl[S])) return;
+  const int d = threadIdx.x % TPR * 4, mine = threadIdx.x / TPR;
   const int front = counts ? min(max(counts[tok], 0), first_free) : slots;
   const int n = counts ? front + slots - first_free : slots;
-  const float* lse = part_lse + static_cast<int64_t>(row) * slots;
-  const float* po = part_out + static_cast<int64_t>(row) * slots * D + d;
+  const float* lse = part_lse + row * slots;
+  const float* po = part_out + row * slots * D + d;
   float M = LOWEST, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < n; s0 += BATCH) {
-    float e[BATCH];
-    float4 x[BATCH];
-    float top = M;
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const int j = min(s0 + i, n - 1), s = j < front ? j : j - front + first_free;
-      e[i] = lse[s];
-      x[i] = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * D);
-    }
-#pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      if (s0 + i >= n) e[i] = -INFINITY;
-      top = fmaxf(top, e[i]);
-    }
-    const float old = exp2_fast(M - top);
+  for (int i = mine; i < n; i += AT_ONCE) {
+    const int s = i < front ? i : i - front + first_free;
+    const float e = lse[s];
+    const float4 x = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * D);
+    const float top = fmaxf(M, e), old = exp2_fast(M - top), f = exp2_fast(e - top);
     M = top;
-    sum *= old;
-    o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+    sum = sum * old + f;
+    o = make_float4(o.x * old + f * x.x, o.y * old + f * x.y, o.z * old + f * x.z, o.w * old + f * x.w);
+  }
+  if (d == 0) {
+    sums[mine] = sum;
+    tops[mine] = M;
+  }
+  *reinterpret_cast<float4*>(&outs[mine][d]) = o;
+  __syncthreads();
+  if (mine != 0) return;
+  for (int i = 1; i < AT_ONCE; ++i) M = fmaxf(M, tops[i]);
+  sum = 0.f;
+  o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const float f = exp2_fast(e[i] - M);
-      sum += f;
-      o.x += f * x[i].x; o.y += f * x[i].y; o.z += f * x[i].z; o.w += f * x[i].w;
-    }
+  for (int i = 0; i < AT_ONCE; ++i) {
+    const float f = exp2_fast(tops[i] - M);
+    const float4 x = *reinterpret_cast<const float4*>(&outs[i][d]);
+    sum += sums[i] * f;
+    o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *reinterpret_cast<uint2*>(out + tok * out_stride + static_cast<int64_t>(head) * D + d) =
@@ -830,13 +838,13 @@ static uint32_t page_magic(int bs) { return bs >= KV_TILE ? (1u << 31) / (bs / K
 
 static void join(const RowsArgs& p, int D, int tokens, const int32_t* counts, int first_free, const int32_t* qsl, int S,
                  hipStream_t st) {
-  const int rows = tokens * p.Hq, per = 256 / (D / 4);
+  const dim3 grid(static_cast<unsigned>(tokens) * p.Hq);
   if (D == 128)
-    hipLaunchKernelGGL(rows_join_kernel<128>, dim3((rows + per - 1) / per), dim3(256), 0, st, p.part_out, p.part_lse, p.out,
-                       p.out_stride, rows, p.Hq, p.slots, counts, first_free, qsl, S);
+    hipLaunchKernelGGL(rows_join_kernel<128>, grid, dim3(256), 0, st, p.part_out, p.part_lse, p.out, p.out_stride, p.Hq, p.slots,
+                       counts, first_free, qsl, S);
   else
-    hipLaunchKernelGGL(rows_join_kernel<64>, dim3((rows + per - 1) / per), dim3(256), 0, st, p.part_out, p.part_lse, p.out,
-                       p.out_stride, rows, p.Hq, p.slots, counts, first_free, qsl, S);
+    hipLaunchKernelGGL(rows_join_kernel<64>, grid, dim3(256), 0, st, p.part_out, p.part_lse, p.out, p.out_stride, p.Hq, p.slots,
+                       counts, first_free, qsl, S);
 }
 
 #define XGK_FMT_DIM(DO)                                                                                              \
@@ -855,8 +863,7 @@ int quant_decode_attention(int fmt, const uint16_t* q, int64_t q_stride, const u
   if (!rows_ok(p, D) || static_cast<int64_t>(B) * blocks > 65535 || splits > 65535) return -1;
 #define XGK_GO(F, DD)                                                                                                   \
   {                                                                                                                     \
-    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, nullptr, blocks, \
-                       splits, 0);                                                                                      \
+    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, blocks, splits); \
   }
   XGK_FMT_DIM(XGK_GO) else return -1;
 #undef XGK_GO
@@ -900,18 +907,18 @@ int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
                    width, num_blocks, seq_lens, part_out, part_lse, out, out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs,
                    scale * 1.44269504088896341f, prefix_slots + splits, page_magic(bs)};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8) || splits < 1 || splits > 65535 || prefix_slots < 0 || n_items < 0 ||
-      n_items > 65535 || static_cast<int64_t>(B) * blocks > 65535)
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2) || splits < 1 || prefix_slots < 0 || n_items < 0 ||
+      n_items + static_cast<int64_t>(B) * blocks * splits > 65535)
     return -1;
-#define XGK_GO(F, DD)                                                                                                      \
-  {                                                                                                                        \
-    if (n_items > 0) {                                                                                                     \
-      if (RT == 1) hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 1>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);     \
-      else if (RT == 2) hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 2>), dim3(Hkv, n_items), dim3(256), 0, st, p, items); \
-      else hipLaunchKernelGGL((rows_prefix_kernel<F, DD, 8>), dim3(Hkv, n_items), dim3(256), 0, st, p, items);             \
-    }                                                                                                                      \
-    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, prefix, blocks,     \
-                       splits, prefix_slots);                                                                              \
+  const dim3 grid(Hkv, n_items + B * blocks * splits);
+#define XGK_GO(F, DD)                                                                                                     \
+  {                                                                                                                       \
+    if (RT == 1)                                                                                                          \
+      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 1>), grid, dim3(256), 0, st, p, items, n_items, prefix, prefix_slots, \
+                         blocks, splits);                                                                                 \
+    else                                                                                                                  \
+      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 2>), grid, dim3(256), 0, st, p, items, n_items, prefix, prefix_slots, \
+                         blocks, splits);                                                                                 \
   }
   XGK_FMT_DIM(XGK_GO)
   else if (fmt == KV_BF16 && D == 128) XGK_GO(KV_BF16, 128) else if (fmt == KV_BF16) XGK_GO(KV_BF16, 64) else return -1;

@@ -393,8 +393,8 @@ def test_a_key_that_is_not_finite_reaches_only_those_who_see_it(dev, fmt):
     assert bool(out[1, 2:].isnan().all()) and bool(out[1, :2].isfinite().all()) and bool(out[2].isfinite().all())
     n = 60                                # tokens 40 .. 100 of each: those before the key do not see it
     qp = rows(3 * n, 4, 64, gen).to(dev)
-    got = ops.quant_prefill_attention(qp, cache, table, i32([0, n, 2 * n, 3 * n], dev), i32(lens, dev), n, 0.1).cpu()
-    for s in range(3):
+    for rt, s in ((rt, s) for rt in (1, 2, 8) for s in range(3)):
+        got = ops.quant_prefill_attention(qp, cache, table, i32([0, n, 2 * n, 3 * n], dev), i32(lens, dev), n, 0.1, row_tiles=rt).cpu()
         for i in range(n):
             seen = 40 + i + 1
             bad = [s == 0 and seen > 50, s == 1 and seen > 70]
@@ -410,8 +410,8 @@ def test_a_key_that_is_not_finite_reaches_only_those_who_see_it(dev, fmt):
 @DEVICES
 @FORMATS
 @pytest.mark.parametrize("Hq,Hkv,D,bs", [(32, 8, 128, 16), (8, 1, 128, 32), (12, 12, 64, 16), (6, 2, 64, 48), (20, 1, 128, 16)])
-@pytest.mark.parametrize("splits", [None, 1, 5])
-def test_prompts(dev, fmt, Hq, Hkv, D, bs, splits):
+@pytest.mark.parametrize("splits,rt", [(None, None), (1, 1), (1, 2), (5, 2), (1, 8), (3, 8)])
+def test_prompts(dev, fmt, Hq, Hkv, D, bs, splits, rt):
     gen = torch.Generator().manual_seed(Hq * 3 + D)
     new, ctx = [1, 0, 5, 33, 17, 64, 3, 130], [0, 9, 0, 31, 200, 64, 500, 2]
     lens = [a + b for a, b in zip(new, ctx)]
@@ -422,7 +422,8 @@ def test_prompts(dev, fmt, Hq, Hkv, D, bs, splits):
     q = rows(cu[-1] + 3, Hq, D, gen, 1.5).to(dev)
     scale = 1 / math.sqrt(D)
     out = torch.full_like(q, 9.0)
-    ops.quant_prefill_attention(q, cache, table, i32(cu, dev), i32(lens, dev), max(new), scale, num_splits=splits, out=out)
+    ops.quant_prefill_attention(q, cache, table, i32(cu, dev), i32(lens, dev), max(new), scale, num_splits=splits, out=out,
+                                row_tiles=rt)
     assert bool((out[:2] == 9).all()) and bool((out[cu[-1]:] == 9).all())
     for s, n in enumerate(new):
         a, b = cu[s], cu[s + 1]
@@ -586,6 +587,8 @@ def test_refusals():
                     ((q, c, bt[:1], cu, ln, 1), ValueError)):
         with pytest.raises(e):
             ops.quant_prefill_attention(*args, 0.1)
+    with pytest.raises(ValueError):
+        ops.quant_prefill_attention(q, c, bt, cu, ln, 1, 0.1, row_tiles=4)
 
     for a in (([1], [1, 2], 4, 2), ([0], [1], 4, 2), ([1], [-1], 4, 2), ([1], [1], 3, 2), ([1], [1], 4, 0)):
         with pytest.raises(ValueError):

@@ -30,8 +30,14 @@ KV_FORMATS = {"fp8": KV_FP8, "int8": KV_INT8}
 LARGEST = {"fp8": 448.0, "int8": 127.0}
 TILE = 16           # tokens whose codes lie together in the order of the matrix instructions (csrc/kernels/kv_quant.h)
 MAX_SPLITS = 64
+# us of decode, one part / the parts that this makes: 1 sequence of 640 keys 6.0 / 6.5, 1280 8.5 / 6.9, 5120 35.7 / 8.9; 16 of 640
+# 8.5 / 9.4, 5120 48.8 / 30.5; 48 of 1280 25.2 / 25.4 (8 kv heads of 128). Below SPLIT_FROM keys a second launch costs more
 SPLIT_WGS = 512     # workgroups that fill the chip: two a CU
 SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
+SPLIT_FROM = 1024
+# the common parts of shared prefixes: one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences behind
+# 4096 keys: 256 workgroups 26.9 us, 512 32.6, 1024 40.6)
+PREFIX_WGS = 256
 
 
 def _need(ok: bool, what: str) -> None:
@@ -348,7 +354,7 @@ def _check_decode(q, Hkv: int, D: int, index: int, device, block_tables, seq_len
 def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
     """Parts of the key range: enough workgroups to fill the chip, each with a tile for each of its waves."""
     if num_splits is None:
-        return max(1, min(-(-SPLIT_WGS // max(1, wgs)), -(-max_keys // SPLIT_KEYS), MAX_SPLITS))
+        return 1 if max_keys < SPLIT_FROM else max(1, min(-(-SPLIT_WGS // max(1, wgs)), -(-max_keys // SPLIT_KEYS), MAX_SPLITS))
     if not 1 <= num_splits <= MAX_SPLITS:
         raise ValueError(f"num_splits must be 1 to {MAX_SPLITS}, got {num_splits}")
     return int(num_splits)
@@ -398,17 +404,24 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     return out
 
 
-def _row_tiles(rows: int, D: int) -> int:
-    """16-row tiles of a workgroup: as many as the rows fill and the registers hold."""
-    return 1 if rows <= 16 else 2 if rows <= 32 else 8
+def _row_tiles(rows: int, lists: int) -> int:
+    """16-row tiles of a workgroup over `lists` lists of up to `rows` rows: one or two for all four waves, each with keys of its own, or
+    eight, two a wave, over the same keys. More rows read and widen the keys less often; fewer make more workgroups. us with 1, 2
+    and 8 (8 kv heads, G = 4): a prompt of 128 tokens 5.4 / 7.2 / 11.5, 512 14.1 / 11.5 / 20.4, 2048 76.3 / 56.6 / 60.3, four of
+    2000 behind 1500 tokens 515 / 380 / 342 (int8 714 / 474 / 358)."""
+    if lists * -(-rows // 128) >= 2 * SPLIT_WGS:
+        return 8
+    return 2 if lists * -(-rows // 32) >= SPLIT_WGS else 1
 
 
 def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
                             seq_lens: torch.Tensor, max_q_len: int, scale: float, num_splits: Optional[int] = None,
-                            workspace: Optional[DecodeWorkspace] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                            workspace: Optional[DecodeWorkspace] = None, out: Optional[torch.Tensor] = None,
+                            row_tiles: Optional[int] = None) -> torch.Tensor:
     """`prefill_attention` over an 8-bit cache: q [T, Hq, D] bf16 packed; sequence s has the tokens query_start_loc[s] ..
     query_start_loc[s + 1], the last of its seq_lens[s], and each sees the keys up to its own, all of them in the cache already.
-    max_q_len: at least the tokens of the longest portion. Rows of no sequence stay as they were in `out`."""
+    max_q_len: at least the tokens of the longest portion. Rows of no sequence stay as they were in `out`. row_tiles (tests / A/B
+    sweeps; None = `_row_tiles`): 1, 2 or 8."""
     (nb, Hkv, bs, D), dev, index = cache.dims, cache.device, cache.index
     S = seq_lens.shape[0]
     if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 and _plain_table(block_tables, index, S)
@@ -424,7 +437,9 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
         return out
     W, G = block_tables.shape[1], Hq // Hkv
     max_q_len = min(max_q_len, T)
-    rt = _row_tiles(max_q_len * G, D)
+    rt = _row_tiles(max_q_len * G, S * Hkv) if row_tiles is None else row_tiles
+    if rt not in (1, 2, 8):
+        raise ValueError(f"row_tiles must be 1, 2 or 8, got {rt}")
     blocks = -(-max_q_len * G // (16 * rt))
     splits = _splits(num_splits, S * Hkv * blocks, W * bs)
     if S * splits > 65535 or blocks > 65535:
@@ -473,11 +488,11 @@ def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], n
     _need(all(n >= 1 for n in sizes) and all(0 <= n < 1 << 30 for n in lens), "groups of at least one sequence, lengths of at least 0")
     _need(num_kv_heads >= 1 and num_heads >= 1 and num_heads % num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
     G = num_heads // num_kv_heads
-    rt = _row_tiles(max([n * G for n, p in zip(sizes, lens) if p > 0], default=0), 128)
+    rt = 2 if max([n * G for n, p in zip(sizes, lens) if p > 0], default=0) > 16 else 1
     blocks = [-(-n * G // (16 * rt)) for n in sizes]
     tiles = [-(-p // 32) for p in lens]
     total = sum(b * t for b, t in zip(blocks, tiles)) * num_kv_heads
-    each = max(4, -(-total // SPLIT_WGS))      # 32-key tiles of a workgroup
+    each = max(4, -(-total // PREFIX_WGS))      # 32-key tiles of a workgroup
     items: List[List[int]] = []
     prefix, counts, at = [], [], 0
     for n, p, b, t in zip(sizes, lens, blocks, tiles):
