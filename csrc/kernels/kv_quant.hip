@@ -32,32 +32,50 @@ struct KvAppend {
 template <int N>
 struct Codes { uint32_t w[N / 4]; };
 
-// codes of this lane's D / 16 numbers of a row that 16 lanes hold, and the row's scale
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
+// codes of this lane's D / 16 numbers (N / 2 pairs) of a row that 16 lanes hold, and the row's scale
 template <int FMT, int N>
-__device__ __forceinline__ Codes<N> kv_quantise(const uint16_t (&x)[N], float& scale) {
+__device__ __forceinline__ Codes<N> kv_quantise(const uint32_t (&x)[N / 2], float& scale) {
   constexpr float LARGEST = FMT == KV_FP8 ? 448.f : 127.f;
-  uint32_t top = 0;
+  // magnitudes of bf16 order as whole numbers do, NaN above infinity
+  u16x2_t pair = {0, 0};
 #pragma unroll
-  for (int i = 0; i < N; ++i) top = max(top, static_cast<uint32_t>(x[i] & 0x7FFF));
-  // (magnitudes of bf16 order as whole numbers do, NaN above infinity; as floats of the same bits they do too)
-  float m = __uint_as_float(top);
+  for (int i = 0; i < N / 2; ++i) pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2_t, x[i] & 0x7FFF7FFFu));
+  uint32_t top = max(pair[0], pair[1]);
   auto join = [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); };
+  float m = __uint_as_float(top);
   m = join(m, row_ror<8>(m));
   m = join(m, row_ror<4>(m));
   m = join(m, row_ror<2>(m));
   m = join(m, row_ror<1>(m));
   top = __float_as_uint(m);
-  const float a = __uint_as_float(top << 16);
-  const bool usable = top < 0x7F80u && top != 0;
-  scale = usable ? a / LARGEST : (top == 0 ? 0.f : __uint_as_float(0x7FC00000u));
-  const float lift = a < 0x1p-90f ? 0x1p60f : 1.f;  // 448 / a has to be a float
-  const float inv = usable ? LARGEST / (a * lift) : 0.f;
+  float a = __uint_as_float(top << 16);
   float y[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float f = usable ? bf2f(x[i]) * lift * inv : 0.f;
-    y[i] = __uint_as_float((__float_as_uint(f) + 8u) & ~15u);
+  for (int i = 0; i < N / 2; ++i) {
+    y[2 * i] = __uint_as_float(x[i] << 16);
+    y[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
   }
+  if (__all(a > 0x1p-90f && a < 0x1p100f)) {
+    // a / LARGEST to its nearest float: the quotient's own error comes back through the multiply-add
+    const float q = a * (1.f / LARGEST);
+    scale = fmaf(fmaf(-LARGEST, q, a), 1.f / LARGEST, q);
+  } else {   // rows of zeros, of numbers whose inverse is no normal float, and those that are not finite
+    const bool usable = top < 0x7F80u && top != 0;
+    scale = usable ? a / LARGEST : (top == 0 ? 0.f : __uint_as_float(0x7FC00000u));
+    const float lift = a >= 0x1p100f ? 0x1p-60f : a > 0x1p-90f ? 1.f : 0x1p60f;
+    a = usable ? a * lift : 1.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = usable ? y[i] * lift : 0.f;
+  }
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float inv = LARGEST * __builtin_amdgcn_rcpf(a);   // off by less than 2^-22.4, the products by less than 2^-22
+#else
+  const float inv = LARGEST / a;
+#endif
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = __uint_as_float((__float_as_uint(y[i] * inv) + 8u) & ~15u);
   Codes<N> c;
 #pragma unroll
   for (int j = 0; j < N / 4; ++j) {
@@ -67,11 +85,11 @@ __device__ __forceinline__ Codes<N> kv_quantise(const uint16_t (&x)[N], float& s
       w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j + 2], y[4 * j + 3], w, true);
       c.w[j] = static_cast<uint32_t>(w);
     } else {
-      uint32_t w = 0;
+      // 1.5 2^23 more: the float's last byte is the whole number, rounded to even, in two's complement
+      uint32_t e[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w |= (static_cast<uint32_t>(static_cast<int>(rintf(y[4 * j + i]))) & 0xFFu) << (8 * i);
-      c.w[j] = w;
+      for (int i = 0; i < 4; ++i) e[i] = __float_as_uint(y[4 * j + i] + 12582912.f);
+      c.w[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0C0C0400u), __builtin_amdgcn_perm(e[1], e[0], 0x0C0C0400u), 0x05040100u);
     }
 #else
     c.w[j] = 0;
@@ -81,27 +99,50 @@ __device__ __forceinline__ Codes<N> kv_quantise(const uint16_t (&x)[N], float& s
 }
 
 template <int N>
-__device__ __forceinline__ void kv_load_row(const uint16_t* p, uint16_t (&x)[N]) {
+__device__ __forceinline__ void kv_load_row(const uint16_t* p, uint32_t (&x)[N / 2]) {
   if constexpr (N == 8) {
     const uint4 v = ld16(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[2 * i] = w[i] & 0xFFFF; x[2 * i + 1] = w[i] >> 16; }
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
   } else {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
-    x[0] = v.x & 0xFFFF; x[1] = v.x >> 16; x[2] = v.y & 0xFFFF; x[3] = v.y >> 16;
+    x[0] = v.x; x[1] = v.y;
   }
+}
+
+// Codes of four tokens, a token a 16-lane group, to words of four tokens' codes of a dim: group i has the dims (N / 4) i + e of its N.
+// Halves of the wave trade places, then neighbouring groups: two register moves where a trip through LDS a word was eight.
+template <int N>
+__device__ __forceinline__ void kv_turn(const Codes<N>& c, uint32_t (&four)[N / 4]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  // lo / hi: the N / 2 codes of the lower and upper dims. Behind the first move the lower groups have tokens' (0 | 1) and (2 | 3) lo
+  const uint32_t lo = N == 8 ? c.w[0] : c.w[0] & 0xFFFFu, hi = N == 8 ? c.w[N / 4 - 1] : c.w[0] >> 16;
+  const auto h = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+  // of these the first and second halves, tokens (0 | 1) below (2 | 3)
+  const uint32_t x = __builtin_amdgcn_perm(h[1], h[0], N == 8 ? 0x05040100u : 0x0C0C0400u);
+  const uint32_t y = __builtin_amdgcn_perm(h[1], h[0], N == 8 ? 0x07060302u : 0x0C0C0501u);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);   // tokens 0, 2 and 1, 3 of the group's own dims
+  if constexpr (N == 8) {
+    four[0] = __builtin_amdgcn_perm(r[1], r[0], 0x06020400u);
+    four[N / 4 - 1] = __builtin_amdgcn_perm(r[1], r[0], 0x07030501u);
+  } else {
+    four[0] = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u);
+  }
+#endif
 }
 
 // rotate_half of a row that 16 lanes hold: lane c's partner is c ^ 8 (D / 2 numbers on)
 template <int N>
-__device__ __forceinline__ void kv_rotate(uint16_t (&x)[N], const float* cs, int c) {
+__device__ __forceinline__ void kv_rotate(uint32_t (&x)[N / 2], const float* cs, int c) {
   const float* cp = cs + (c & 7) * N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float f = bf2f(x[i]), o = row_ror<8>(f);
-    const float co = cp[i], si = cp[8 * N + i];
-    x[i] = f2bf(c < 8 ? f * co - o * si : f * co + o * si);
+  for (int i = 0; i < N / 2; ++i) {
+    float f[2] = {__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xFFFF0000u)};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float o = row_ror<8>(f[j]), co = cp[2 * i + j], si = cp[8 * N + 2 * i + j];
+      f[j] = c < 8 ? f[j] * co - o * si : f[j] * co + o * si;
+    }
+    x[i] = pack2(f[0], f[1]);
   }
 }
 
@@ -116,28 +157,14 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
     const int t = t0 + i;
     if (t < p.T) {
       uint16_t* row = p.q + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head - p.Hkv) * D + c * N;
-      uint16_t x[N];
+      uint32_t x[N / 2];
       kv_load_row<N>(row, x);
       kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j)
-        *reinterpret_cast<uint2*>(row + 4 * j) = make_uint2(x[4 * j] | (static_cast<uint32_t>(x[4 * j + 1]) << 16),
-                                                            x[4 * j + 2] | (static_cast<uint32_t>(x[4 * j + 3]) << 16));
+      if constexpr (N == 8) st16(row, make_uint4(x[0], x[1], x[N / 2 - 2], x[N / 2 - 1]));
+      else *reinterpret_cast<uint2*>(row) = make_uint2(x[0], x[1]);
     }
     return;
   }
-  auto row_of = [&](int t, bool value, uint16_t (&x)[N]) {
-    const uint16_t* src = value ? p.v + static_cast<int64_t>(t) * p.v_stride : p.k + static_cast<int64_t>(t) * p.k_stride;
-    kv_load_row<N>(src + static_cast<int64_t>(head) * D + c * N, x);
-  };
-  auto turned = [&](int t, uint16_t (&x)[N]) {
-    if (ROPE) kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
-  };
-  // the window's own rows are on their way before its slots are known (a quad mostly begins with the window)
-  uint16_t xk[N], xv[N];
-  const int own = min(t0 + i, p.T - 1);
-  row_of(own, false, xk);
-  row_of(own, true, xv);
   // slots of the tokens around the window, -1 where there is none
   int s[10];
 #pragma unroll
@@ -147,80 +174,54 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
     s[j] = t >= 0 && t < p.T && static_cast<int64_t>(v) < p.num_slots ? v : -1;
   }
   // the quad that begins in this window, and this window's tokens that no quad takes
-  int quad = -1;
+  int quad = -1, quad_slot = 0;
   uint32_t taken = 0;
 #pragma unroll
   for (int b = 0; b < 7; ++b)
     if (s[b] >= 0 && (s[b] & 3) == 0 && s[b + 1] == s[b] + 1 && s[b + 2] == s[b] + 2 && s[b + 3] == s[b] + 3) {
-      if (b >= 3) quad = t0 - 3 + b;
+      if (b >= 3) {
+        quad = t0 - 3 + b;
+        quad_slot = s[b];
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (b + j >= 3 && b + j < 7) taken |= 1u << (b + j - 3);
     }
-  auto tile_of = [&](int slot, int64_t& scale_at) {
-    const int64_t page = slot / p.bs;
-    const int off = slot % p.bs;
-    scale_at = (page * p.Hkv + head) * 2 * p.bs + off;
-    return ((page * p.Hkv + head) * p.bs + (off & ~15)) * D;
-  };
-  auto put_k = [&](const Codes<N>& w, int slot, int64_t tile) {
-    uint8_t* dst = p.kc + tile + kv_k_byte(slot % p.bs & 15, c * N);
-    if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w.w[0], w.w[1]);
-    else *reinterpret_cast<uint32_t*>(dst) = w.w[0];
-  };
-  if (quad >= 0) {
-    const int slot = p.slots[quad] + i;
-    int64_t at;
-    const int64_t tile = tile_of(slot, at);
-    uint16_t yk[N], yv[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) { yk[j] = xk[j]; yv[j] = xv[j]; }
-    if (quad != t0) {
-      row_of(quad + i, false, yk);
-      row_of(quad + i, true, yv);
-    }
-    turned(quad + i, yk);
+  // the 16 lanes' token t at offset `off` of a page: its codes of K and V
+  auto write = [&](int t, int64_t page, int off, bool whole) {
+    uint32_t xk[N / 2], xv[N / 2];
+    kv_load_row<N>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head) * D + c * N, xk);
+    kv_load_row<N>(p.v + static_cast<int64_t>(t) * p.v_stride + static_cast<int64_t>(head) * D + c * N, xv);
+    if (ROPE) kv_rotate<N>(xk, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
+    const int64_t ph = page * p.Hkv + head, tile = (ph * p.bs + (off & ~15)) * D, at = ph * 2 * p.bs + off;
     float sk, sv;
-    put_k(kv_quantise<FMT, N>(yk, sk), slot, tile);
-    const Codes<N> w = kv_quantise<FMT, N>(yv, sv);
+    const Codes<N> wk = kv_quantise<FMT, N>(xk, sk), wv = kv_quantise<FMT, N>(xv, sv);
+    uint8_t* dk = p.kc + tile + kv_k_byte(off & 15, c * N);
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(dk) = make_uint2(wk.w[0], wk.w[N / 4 - 1]);
+    else *reinterpret_cast<uint32_t*>(dk) = wk.w[0];
     if (c == 0) {
       p.scales[at] = sk;
       p.scales[at + p.bs] = sv;
     }
-    // lane (i, c) collects its dims' codes of all four tokens: dims N c + (N / 4) i ..
-    uint32_t four[N / 4] = {};
+    if (whole) {
+      uint32_t four[N / 4];
+      kv_turn<N>(wv, four);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      uint32_t got[N / 4];
+      for (int e = 0; e < N / 4; ++e)
+        *reinterpret_cast<uint32_t*>(p.vc + tile + kv_v_byte(off & 12, c * N + (N / 4) * i + e)) = four[e];
+    } else {
+      uint8_t* dv = p.vc + tile + kv_v_byte(off & 15, c * N);
 #pragma unroll
-      for (int j = 0; j < N / 4; ++j) got[j] = __shfl(w.w[j], t * 16 + c, 64);
-#pragma unroll
-      for (int e = 0; e < N / 4; ++e) {
-        const int d = (N / 4) * i + e;   // of the lane's N
-        const uint32_t word = N == 8 && d >= 4 ? got[N / 4 - 1] : got[0];
-        four[e] |= ((word >> (8 * (d & 3))) & 0xFFu) << (8 * t);
-      }
+      for (int e = 0; e < N; ++e) dv[16 * e] = (wv.w[e >> 2] >> (8 * (e & 3))) & 0xFF;
     }
-#pragma unroll
-    for (int e = 0; e < N / 4; ++e)
-      *reinterpret_cast<uint32_t*>(p.vc + tile + kv_v_byte((slot % p.bs & 15) & ~3, c * N + (N / 4) * i + e)) = four[e];
+  };
+  if (quad >= 0) {   // (one division for the wave)
+    const int page = quad_slot / p.bs;
+    write(quad + i, page, quad_slot - page * p.bs + i, true);
   }
-  const int slot = s[3 + 0] * (i == 0) + s[3 + 1] * (i == 1) + s[3 + 2] * (i == 2) + s[3 + 3] * (i == 3);
-  if (!(taken >> i & 1) && slot >= 0) {   // (16 lanes are of one mind: the rotations within them stay whole)
-    int64_t at;
-    const int64_t tile = tile_of(slot, at);
-    turned(own, xk);
-    float sk, sv;
-    put_k(kv_quantise<FMT, N>(xk, sk), slot, tile);
-    const Codes<N> w = kv_quantise<FMT, N>(xv, sv);
-    if (c == 0) {
-      p.scales[at] = sk;
-      p.scales[at + p.bs] = sv;
-    }
-    uint8_t* dst = p.vc + tile + kv_v_byte(slot % p.bs & 15, c * N);
-#pragma unroll
-    for (int e = 0; e < N; ++e) dst[16 * e] = (w.w[e >> 2] >> (8 * (e & 3))) & 0xFF;
-  }
+  const int slot = i == 0 ? s[3] : i == 1 ? s[4] : i == 2 ? s[5] : s[6];
+  if (!(taken >> i & 1) && slot >= 0)   // (16 lanes are of one mind: the rotations within them stay whole)
+    write(t0 + i, slot / p.bs, slot % p.bs, false);
 }
 
 template <int FMT, int D>
