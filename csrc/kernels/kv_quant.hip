@@ -4,7 +4,7 @@
 namespace xgk {
 
 // ---- append ------------------------------------------------------------------------------------------------------------
-// A wave takes a window of four tokens of one head: 16 lanes a row, D / 16 numbers a lane, K and V in turn. A row's largest
+// A wave takes a window of four tokens of one head (or two): 16 lanes a row, D / 16 numbers a lane, K and V in turn. A row's largest
 // magnitude joins over its 16 lanes by register rotations; nothing goes through memory but the row itself (2 D bytes in,
 // D + 4 out: bound by HBM for long steps, by one trip to memory and the launch for single tokens).
 //
@@ -146,11 +146,11 @@ __device__ __forceinline__ void kv_rotate(uint32_t (&x)[N / 2], const float* cs,
   }
 }
 
-template <int FMT, int D, bool ROPE>
+template <int FMT, int D, bool ROPE, int HEADS>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
   constexpr int N = D / 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t0 = (blockIdx.x * 4 + wid) * 4, head = blockIdx.y;
+  const int t0 = (blockIdx.x * 4 + wid) * 4, head = blockIdx.y * HEADS;
   const int i = lane >> 4, c = lane & 15;
   if (t0 >= p.T) return;
   if (ROPE && head >= p.Hkv) {   // a query head, rotated in place
@@ -189,30 +189,36 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
     }
   // the 16 lanes' token t at offset `off` of a page: its codes of K and V
   auto write = [&](int t, int64_t page, int off, bool whole) {
-    uint32_t xk[N / 2], xv[N / 2];
-    kv_load_row<N>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head) * D + c * N, xk);
-    kv_load_row<N>(p.v + static_cast<int64_t>(t) * p.v_stride + static_cast<int64_t>(head) * D + c * N, xv);
-    if (ROPE) kv_rotate<N>(xk, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
-    const int64_t ph = page * p.Hkv + head, tile = (ph * p.bs + (off & ~15)) * D, at = ph * 2 * p.bs + off;
-    float sk, sv;
-    const Codes<N> wk = kv_quantise<FMT, N>(xk, sk), wv = kv_quantise<FMT, N>(xv, sv);
-    uint8_t* dk = p.kc + tile + kv_k_byte(off & 15, c * N);
-    if constexpr (N == 8) *reinterpret_cast<uint2*>(dk) = make_uint2(wk.w[0], wk.w[N / 4 - 1]);
-    else *reinterpret_cast<uint32_t*>(dk) = wk.w[0];
-    if (c == 0) {
-      p.scales[at] = sk;
-      p.scales[at + p.bs] = sv;
+    uint32_t xk[HEADS][N / 2], xv[HEADS][N / 2];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      kv_load_row<N>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head + h) * D + c * N, xk[h]);
+      kv_load_row<N>(p.v + static_cast<int64_t>(t) * p.v_stride + static_cast<int64_t>(head + h) * D + c * N, xv[h]);
     }
-    if (whole) {
-      uint32_t four[N / 4];
-      kv_turn<N>(wv, four);
 #pragma unroll
-      for (int e = 0; e < N / 4; ++e)
-        *reinterpret_cast<uint32_t*>(p.vc + tile + kv_v_byte(off & 12, c * N + (N / 4) * i + e)) = four[e];
-    } else {
-      uint8_t* dv = p.vc + tile + kv_v_byte(off & 15, c * N);
+    for (int h = 0; h < HEADS; ++h) {
+      if (ROPE) kv_rotate<N>(xk[h], p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
+      const int64_t ph = page * p.Hkv + head + h, tile = (ph * p.bs + (off & ~15)) * D, at = ph * 2 * p.bs + off;
+      float sk, sv;
+      const Codes<N> wk = kv_quantise<FMT, N>(xk[h], sk), wv = kv_quantise<FMT, N>(xv[h], sv);
+      uint8_t* dk = p.kc + tile + kv_k_byte(off & 15, c * N);
+      if constexpr (N == 8) *reinterpret_cast<uint2*>(dk) = make_uint2(wk.w[0], wk.w[N / 4 - 1]);
+      else *reinterpret_cast<uint32_t*>(dk) = wk.w[0];
+      if (c == 0) {
+        p.scales[at] = sk;
+        p.scales[at + p.bs] = sv;
+      }
+      if (whole) {
+        uint32_t four[N / 4];
+        kv_turn<N>(wv, four);
 #pragma unroll
-      for (int e = 0; e < N; ++e) dv[16 * e] = (wv.w[e >> 2] >> (8 * (e & 3))) & 0xFF;
+        for (int e = 0; e < N / 4; ++e)
+          *reinterpret_cast<uint32_t*>(p.vc + tile + kv_v_byte(off & 12, c * N + (N / 4) * i + e)) = four[e];
+      } else {
+        uint8_t* dv = p.vc + tile + kv_v_byte(off & 15, c * N);
+#pragma unroll
+        for (int e = 0; e < N; ++e) dv[16 * e] = (wv.w[e >> 2] >> (8 * (e & 3))) & 0xFF;
+      }
     }
   };
   if (quad >= 0) {   // (one division for the wave)
@@ -227,8 +233,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
 template <int FMT, int D>
 static void launch_append(const KvAppend& p, bool rope, hipStream_t st) {
   const dim3 grid((p.T + 15) / 16, p.Hkv + (rope ? p.Hq : 0));
-  if (rope) hipLaunchKernelGGL((kv_append_kernel<FMT, D, true>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((kv_append_kernel<FMT, D, false>), grid, dim3(256), 0, st, p);
+  // two heads a wave from 16 k rows on: half the waves, each with twice the loads on their way, 14.5 -> 11.5 us for 8192 tokens of 8
+  // heads and 46 -> 34 (6 TB/s) for 32768; 4.0 for 3.5 with 64 tokens, where they are too few
+  if (rope) hipLaunchKernelGGL((kv_append_kernel<FMT, D, true, 1>), grid, dim3(256), 0, st, p);
+  else if (p.Hkv % 2 == 0 && static_cast<int64_t>(p.T) * p.Hkv >= 16384)
+    hipLaunchKernelGGL((kv_append_kernel<FMT, D, false, 2>), dim3(grid.x, p.Hkv / 2), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((kv_append_kernel<FMT, D, false, 1>), grid, dim3(256), 0, st, p);
 }
 
 // positions / cos_sin null: k and v as they are; else q (Hq heads, in place) and k are rotated first.

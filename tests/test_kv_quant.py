@@ -229,6 +229,24 @@ def test_append_takes_any_slots_and_leaves_the_rest(dev, fmt, Hkv, D, bs):
         torch.testing.assert_close(cache.scales.cpu(), plain.scales, rtol=2.0 ** -23, atol=0)
 
 
+@pytest.mark.gpu
+@FORMATS
+@pytest.mark.parametrize("Hkv,D", [(8, 128), (8, 64), (12, 64), (5, 128)])
+def test_append_of_many_rows(fmt, Hkv, D):
+    """Two heads a wave (an even number of heads), tokens that begin anywhere in a quad, and some of no slot."""
+    gen = torch.Generator().manual_seed(11)
+    T, bs, nb = 16384 // Hkv + 5, 32, 16384 // Hkv // 32 + 8
+    x = rows(T, 2 * Hkv, D, gen)
+    slots = torch.cat([torch.arange(3, 1003), torch.tensor([-1, -1]), torch.arange(1026, 1026 + T - 1002)]).to(torch.int32)
+    slots[[5, 700]] = -1
+    got, want = (ops.QuantKVCache.alloc(nb, Hkv, bs, D, fmt, d) for d in ("cuda", "cpu"))
+    big = x.to("cuda")
+    ops.kv_quant_append(big[:, :Hkv], big[:, Hkv:], got, slots.to("cuda"))
+    ops.kv_quant_append(x[:, :Hkv], x[:, Hkv:], want, slots)
+    assert torch.equal(got.k.cpu(), want.k) and torch.equal(got.v.cpu(), want.v)
+    torch.testing.assert_close(got.scales.cpu(), want.scales, rtol=2.0 ** -23, atol=0)
+
+
 @DEVICES
 @FORMATS
 @pytest.mark.parametrize("Hkv,D,bs", [(8, 128, 16), (2, 64, 48)])
