@@ -50,6 +50,8 @@ def parse():
     ap.add_argument("--coalesce-max-wait", type=int, default=4, help="admission window bound, in steps")
     ap.add_argument("--moe-comm", default="auto", choices=["auto", "alltoall", "allreduce"])
     ap.add_argument("--no-graphs", action="store_true")
+    ap.add_argument("--kv-cache-dtype", default=None, choices=["fp8", "int8"],
+                    help="KV cache in 8 bits (a scale per token and head); not the bf16 headline")
     ap.add_argument("--weight-dtype", default=None, choices=["fp8", "int8", "int4"],
                     help="weight-only copies for decode batches <= 64: fp8 (E4M3), int8 (per-channel) or int4 "
                          "(per 128-k group) -- not the bf16 headline")
@@ -250,7 +252,7 @@ def main():
                         use_graphs=on_gpu and not a.no_graphs, enable_prefix_cache=not a.no_prefix_cache,
                         moe_comm=a.moe_comm, prompt_coalesce=a.coalesce, block_size=a.block_size,
                         prompt_coalesce_max_wait=a.coalesce_max_wait, decode_prefill_cap=a.prefill_chunk,
-                        weight_dtype=a.weight_dtype, dtype=None if on_gpu else "float32",
+                        weight_dtype=a.weight_dtype, kv_cache_dtype=a.kv_cache_dtype, dtype=None if on_gpu else "float32",
                         graph_batch_sizes=[b for b in [1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128]
                                            if b <= max(64, a.concurrency)], seed=st.dp_rank)
     shard_model = None
@@ -406,7 +408,8 @@ def main():
             "higher_is_better": True,
             "scaling": "weak",
             "vs_baseline": None,
-            "dtype": ("bf16" if on_gpu else "fp32") if a.weight_dtype is None else f"bf16 activations, {a.weight_dtype} decode weights",
+            "dtype": (("bf16" if on_gpu else "fp32") if a.weight_dtype is None else f"bf16 activations, {a.weight_dtype} decode weights")
+                     + ("" if a.kv_cache_dtype is None else f", {a.kv_cache_dtype} KV cache"),
             "data": "synthetic (random-token prompts, random-init weights)",
             "ttft_p50_ms": round(1000 * p50, 2) if p50 == p50 else None,
             "config": {"model": a.model, "global_batch": a.concurrency * dp,

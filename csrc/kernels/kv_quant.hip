@@ -14,14 +14,21 @@ namespace xgk {
 //
 // V's order puts four tokens' codes of a dim into one word: a window whose slots fill such a quad (tokens of a prompt)
 // exchanges its codes within the wave and writes words; other tokens write bytes.
+//
+// Where the rows come from: KV_ROWS k and v as they are; KV_ROPE the rows of the QKV projection, q and k rotated; KV_PARTS the
+// projection's split-K partial sums [S, T, (Hq + 2 Hkv) D] in fp32, added up, q and k rotated (with a table) and rounded to bf16.
+enum : int { KV_ROWS = 0, KV_ROPE = 1, KV_PARTS = 2 };
 struct KvAppend {
-  uint16_t* q;                 // ROPE: query heads, rotated in place (row stride as k)
+  uint16_t* q;                 // query heads: KV_ROPE in place (tokens as k's), KV_PARTS written to
   const uint16_t* k;
   const uint16_t* v;
   int64_t k_stride, v_stride;  // elements between tokens
+  const float* part;           // KV_PARTS
+  int S;
+  int64_t q_stride;
   const int32_t* slots;        // slot of each token; outside [0, num_slots): not written
-  const int32_t* positions;    // ROPE
-  const float* cos_sin;        // ROPE: [max_pos, D]
+  const int32_t* positions;    // of a rotation
+  const float* cos_sin;        // [max_pos, D]
   uint8_t* kc;
   uint8_t* vc;
   float* scales;
@@ -132,36 +139,72 @@ __device__ __forceinline__ void kv_turn(const Codes<N>& c, uint32_t (&four)[N / 
 
 // rotate_half of a row that 16 lanes hold: lane c's partner is c ^ 8 (D / 2 numbers on)
 template <int N>
-__device__ __forceinline__ void kv_rotate(uint32_t (&x)[N / 2], const float* cs, int c) {
+__device__ __forceinline__ void kv_rotate(float (&f)[N], const float* cs, int c) {
   const float* cp = cs + (c & 7) * N;
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    float f[2] = {__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xFFFF0000u)};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float o = row_ror<8>(f[j]), co = cp[2 * i + j], si = cp[8 * N + 2 * i + j];
-      f[j] = c < 8 ? f[j] * co - o * si : f[j] * co + o * si;
-    }
-    x[i] = pack2(f[0], f[1]);
+  for (int i = 0; i < N; ++i) {
+    const float o = row_ror<8>(f[i]), co = cp[i], si = cp[8 * N + i];
+    f[i] = c < 8 ? f[i] * co - o * si : f[i] * co + o * si;
   }
 }
 
-template <int FMT, int D, bool ROPE, int HEADS>
+// N numbers of a token's partial sums, added up: four parts' loads at a time
+template <int N>
+__device__ __forceinline__ void kv_sum_parts(const float* p, int S, int64_t slab, float (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = 0.f;
+  for (int s0 = 0; s0 < S; s0 += 4) {
+    float4 x[4][N / 4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) x[j][i] = *reinterpret_cast<const float4*>(p + min(s0 + j, S - 1) * slab + 4 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float on = s0 + j < S ? 1.f : 0.f;
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        f[4 * i] += on * x[j][i].x; f[4 * i + 1] += on * x[j][i].y; f[4 * i + 2] += on * x[j][i].z; f[4 * i + 3] += on * x[j][i].w;
+      }
+    }
+  }
+}
+
+template <int FMT, int D, int FROM, int HEADS>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
   constexpr int N = D / 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t0 = (blockIdx.x * 4 + wid) * 4, head = blockIdx.y * HEADS;
   const int i = lane >> 4, c = lane & 15;
   if (t0 >= p.T) return;
-  if (ROPE && head >= p.Hkv) {   // a query head, rotated in place
-    const int t = t0 + i;
+  // this lane's numbers of a row, as bf16 pairs: `at` the row's, `column` its place in the partial sums
+  auto row = [&](const uint16_t* at, int64_t column, int t, bool turn, uint32_t (&x)[N / 2]) {
+    if constexpr (FROM != KV_PARTS) kv_load_row<N>(at + c * N, x);
+    if constexpr (FROM != KV_ROWS) {
+      float f[N];
+      if constexpr (FROM == KV_PARTS) {
+        const int64_t width = static_cast<int64_t>(p.Hq + 2 * p.Hkv) * D;
+        kv_sum_parts<N>(p.part + t * width + column + c * N, p.S, p.T * width, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+          f[2 * j] = __uint_as_float(x[j] << 16);
+          f[2 * j + 1] = __uint_as_float(x[j] & 0xFFFF0000u);
+        }
+      }
+      if (turn && p.cos_sin) kv_rotate<N>(f, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) x[j] = pack2(f[2 * j], f[2 * j + 1]);
+    }
+  };
+  if (FROM != KV_ROWS && head >= p.Hkv) {   // a query head
+    const int t = t0 + i, h = head - p.Hkv;
     if (t < p.T) {
-      uint16_t* row = p.q + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head - p.Hkv) * D + c * N;
+      uint16_t* dst = p.q + static_cast<int64_t>(t) * p.q_stride + static_cast<int64_t>(h) * D;
       uint32_t x[N / 2];
-      kv_load_row<N>(row, x);
-      kv_rotate<N>(x, p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
-      if constexpr (N == 8) st16(row, make_uint4(x[0], x[1], x[N / 2 - 2], x[N / 2 - 1]));
-      else *reinterpret_cast<uint2*>(row) = make_uint2(x[0], x[1]);
+      row(dst, static_cast<int64_t>(h) * D, t, true, x);
+      if constexpr (N == 8) st16(dst + c * N, make_uint4(x[0], x[1], x[N / 2 - 2], x[N / 2 - 1]));
+      else *reinterpret_cast<uint2*>(dst + c * N) = make_uint2(x[0], x[1]);
     }
     return;
   }
@@ -192,12 +235,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
     uint32_t xk[HEADS][N / 2], xv[HEADS][N / 2];
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-      kv_load_row<N>(p.k + static_cast<int64_t>(t) * p.k_stride + static_cast<int64_t>(head + h) * D + c * N, xk[h]);
-      kv_load_row<N>(p.v + static_cast<int64_t>(t) * p.v_stride + static_cast<int64_t>(head + h) * D + c * N, xv[h]);
+      const int64_t dim = static_cast<int64_t>(head + h) * D;
+      row(p.k + static_cast<int64_t>(t) * p.k_stride + dim, static_cast<int64_t>(p.Hq) * D + dim, t, true, xk[h]);
+      row(p.v + static_cast<int64_t>(t) * p.v_stride + dim, static_cast<int64_t>(p.Hq + p.Hkv) * D + dim, t, false, xv[h]);
     }
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-      if (ROPE) kv_rotate<N>(xk[h], p.cos_sin + static_cast<int64_t>(p.positions[t]) * D, c);
       const int64_t ph = page * p.Hkv + head + h, tile = (ph * p.bs + (off & ~15)) * D, at = ph * 2 * p.bs + off;
       float sk, sv;
       const Codes<N> wk = kv_quantise<FMT, N>(xk[h], sk), wv = kv_quantise<FMT, N>(xv[h], sv);
@@ -231,31 +274,47 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvAppend p) {
 }
 
 template <int FMT, int D>
-static void launch_append(const KvAppend& p, bool rope, hipStream_t st) {
-  const dim3 grid((p.T + 15) / 16, p.Hkv + (rope ? p.Hq : 0));
+static void launch_append(const KvAppend& p, int from, hipStream_t st) {
+  const dim3 grid((p.T + 15) / 16, p.Hkv + (from != KV_ROWS ? p.Hq : 0));
   // two heads a wave from 16 k rows on: half the waves, each with twice the loads on their way, 14.5 -> 11.5 us for 8192 tokens of 8
   // heads and 46 -> 34 (6 TB/s) for 32768; 4.0 for 3.5 with 64 tokens, where they are too few
-  if (rope) hipLaunchKernelGGL((kv_append_kernel<FMT, D, true, 1>), grid, dim3(256), 0, st, p);
+  if (from == KV_PARTS) hipLaunchKernelGGL((kv_append_kernel<FMT, D, KV_PARTS, 1>), grid, dim3(256), 0, st, p);
+  else if (from == KV_ROPE) hipLaunchKernelGGL((kv_append_kernel<FMT, D, KV_ROPE, 1>), grid, dim3(256), 0, st, p);
   else if (p.Hkv % 2 == 0 && static_cast<int64_t>(p.T) * p.Hkv >= 16384)
-    hipLaunchKernelGGL((kv_append_kernel<FMT, D, false, 2>), dim3(grid.x, p.Hkv / 2), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((kv_append_kernel<FMT, D, false, 1>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((kv_append_kernel<FMT, D, KV_ROWS, 2>), dim3(grid.x, p.Hkv / 2), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((kv_append_kernel<FMT, D, KV_ROWS, 1>), grid, dim3(256), 0, st, p);
 }
 
-// positions / cos_sin null: k and v as they are; else q (Hq heads, in place) and k are rotated first.
+static int append(int fmt, const KvAppend& p, int from, int D, hipStream_t st) {
+  if (p.T <= 0) return 0;
+  if (p.bs <= 0 || p.bs % KV_TILE || p.Hkv < 1 || (D != 64 && D != 128)) return -1;
+  if (fmt == KV_FP8 && D == 128) launch_append<KV_FP8, 128>(p, from, st);
+  else if (fmt == KV_FP8) launch_append<KV_FP8, 64>(p, from, st);
+  else if (fmt == KV_INT8 && D == 128) launch_append<KV_INT8, 128>(p, from, st);
+  else if (fmt == KV_INT8) launch_append<KV_INT8, 64>(p, from, st);
+  else return -1;
+  return 0;
+}
+
+// cos_sin null: k and v as they are; else q (Hq heads, in place) and k are rotated first.
 int kv_append(int fmt, uint16_t* q, const uint16_t* k, int64_t k_stride, const uint16_t* v, int64_t v_stride,
               const int32_t* slots, const int32_t* positions, const float* cos_sin, uint8_t* kc, uint8_t* vc, float* scales,
               int64_t num_blocks, int T, int Hq, int Hkv, int D, int bs, hipStream_t st) {
-  if (T <= 0) return 0;
-  if (bs <= 0 || bs % KV_TILE || Hkv < 1 || (D != 64 && D != 128) || k_stride % (D / 16) || v_stride % (D / 16)) return -1;
-  const bool rope = cos_sin != nullptr;
-  if (rope && (q == nullptr || positions == nullptr)) return -1;
-  const KvAppend p{q, k, v, k_stride, v_stride, slots, positions, cos_sin, kc, vc, scales, num_blocks * bs, T, Hq, Hkv, bs};
-  if (fmt == KV_FP8 && D == 128) launch_append<KV_FP8, 128>(p, rope, st);
-  else if (fmt == KV_FP8) launch_append<KV_FP8, 64>(p, rope, st);
-  else if (fmt == KV_INT8 && D == 128) launch_append<KV_INT8, 128>(p, rope, st);
-  else if (fmt == KV_INT8) launch_append<KV_INT8, 64>(p, rope, st);
-  else return -1;
-  return 0;
+  if (k_stride % (D >= 16 ? D / 16 : 1) || v_stride % (D >= 16 ? D / 16 : 1)) return -1;
+  if (cos_sin != nullptr && (q == nullptr || positions == nullptr)) return -1;
+  const KvAppend p{q, k, v, k_stride, v_stride, nullptr, 0, k_stride, slots, positions, cos_sin, kc, vc, scales, num_blocks * bs,
+                   T, Hq, Hkv, bs};
+  return append(fmt, p, cos_sin ? KV_ROPE : KV_ROWS, D, st);
+}
+
+// The same of partial sums; q goes to q_out. cos_sin null: no rotation.
+int kv_append_partials(int fmt, const float* part, int S, uint16_t* q_out, int64_t q_stride, const int32_t* slots,
+                       const int32_t* positions, const float* cos_sin, uint8_t* kc, uint8_t* vc, float* scales,
+                       int64_t num_blocks, int T, int Hq, int Hkv, int D, int bs, hipStream_t st) {
+  if (S < 1 || part == nullptr || q_out == nullptr || q_stride % 8 || (cos_sin != nullptr && positions == nullptr)) return -1;
+  const KvAppend p{q_out, nullptr, nullptr, 0, 0, part, S, q_stride, slots, positions, cos_sin, kc, vc, scales, num_blocks * bs,
+                   T, Hq, Hkv, bs};
+  return append(fmt, p, KV_PARTS, D, st);
 }
 
 // ---- read back ---------------------------------------------------------------------------------------------------------

@@ -64,6 +64,8 @@ int prefill_attention(const uint16_t*, int64_t, const uint16_t*, const uint16_t*
                       const int32_t*, uint16_t*, int64_t, int, int, int, int, int, int, float, hipStream_t, int);
 int kv_append(int, uint16_t*, const uint16_t*, int64_t, const uint16_t*, int64_t, const int32_t*, const int32_t*, const float*,
               uint8_t*, uint8_t*, float*, int64_t, int, int, int, int, int, hipStream_t);
+int kv_append_partials(int, const float*, int, uint16_t*, int64_t, const int32_t*, const int32_t*, const float*, uint8_t*, uint8_t*,
+                       float*, int64_t, int, int, int, int, int, hipStream_t);
 int kv_read(int, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t, int, const int32_t*, const int32_t*, int,
             int, int, int, int, int, uint16_t*, uint16_t*, hipStream_t);
 int quant_decode_attention(int, const uint16_t*, int64_t, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t,
@@ -225,6 +227,14 @@ PYBIND11_MODULE(_kernels, m) {
                          P<const int32_t>(pos), P<const float>(cs), P<uint8_t>(kc), P<uint8_t>(vc), P<float>(scales), blocks, T,
                          Hq, Hkv, D, bs, S(st)),
           "kv_append");
+  });
+  m.def("kv_append_partials", [](int fmt, uintptr_t part, int S_, uintptr_t q, int64_t qs, uintptr_t slots, uintptr_t pos,
+                                 uintptr_t cs, uintptr_t kc, uintptr_t vc, uintptr_t scales, int64_t blocks, int T, int Hq, int Hkv,
+                                 int D, int bs, uintptr_t st) {
+    check(xgk::kv_append_partials(fmt, P<const float>(part), S_, P<uint16_t>(q), qs, P<const int32_t>(slots), P<const int32_t>(pos),
+                                  P<const float>(cs), P<uint8_t>(kc), P<uint8_t>(vc), P<float>(scales), blocks, T, Hq, Hkv, D, bs,
+                                  S(st)),
+          "kv_append_partials");
   });
   m.def("kv_read", [](int fmt, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt, int64_t bts, int W, uintptr_t starts,
                       uintptr_t cu, int S_, int n, int blocks, int Hkv, int D, int bs, uintptr_t k, uintptr_t v, uintptr_t st) {

@@ -99,6 +99,9 @@ class EngineConfig:
     early_release: bool = True
     # "fp8": weight-only E4M3 copies for batch <= 16 decode (bf16 activations)
     weight_dtype: Optional[str] = None
+    # "fp8" / "int8": the KV cache in 8 bits with a scale per token and head (ops.QuantKVCache): twice the tokens
+    # in the same memory, half the bytes a decode step reads. None: the model's dtype
+    kv_cache_dtype: Optional[str] = None
     # custom xGMI all-reduce peer-wait limit while serving: a TP peer this late fails
     # the step (CustomAllReduceTimeout -> replica restart); warmup runs under 20 s
     collective_timeout_s: float = 2.0
@@ -190,7 +193,7 @@ class LLMEngine:
                                   max_num_seqs=cfg.max_num_seqs, max_num_batched_tokens=cfg.max_num_batched_tokens,
                                   max_model_len=self.max_model_len, use_graphs=use_graphs,
                                   graph_batch_sizes=graph_bs, is_driver=self.is_driver,
-                                  mixed_chunk=cfg.decode_prefill_cap)
+                                  mixed_chunk=cfg.decode_prefill_cap, kv_cache_dtype=cfg.kv_cache_dtype)
         self.runner.collective_timeout_s = cfg.collective_timeout_s
         self._dp_seqs = cfg.decode_prefill_seqs if cfg.decode_prefill_seqs is not None else \
             (1 if self.runner.mixed_chunk > 0 else 0)
@@ -245,6 +248,8 @@ class LLMEngine:
         m = self.mcfg
         if hasattr(self.model, "cache_bytes_per_block"):
             return max(1, self.model.cache_bytes_per_block(self.cfg.block_size))
+        if self.cfg.kv_cache_dtype is not None:
+            return 2 * m.num_layers * self.model.num_kv_heads_local * self.cfg.block_size * (m.head_dim + 4)
         esz = torch.tensor([], dtype=self.model.dtype).element_size()
         return 2 * m.num_layers * self.model.num_kv_heads_local * self.cfg.block_size * m.head_dim * esz
 
@@ -840,25 +845,29 @@ class LLMEngine:
     def export_prefix(self, tokens: Sequence[int]):
         """CacheEntry for the longest cached page-aligned prefix of `tokens` (this rank's KV shard)."""
         from .kv_io import CacheEntry
-        if self.stateful or self.runner.kv is None:
+        if self.stateful or (self.runner.kv is None and self.runner.kv_quant is None):
             raise ValueError("prefix export needs the engine's own page layout")
         with self._lock:
             blocks = self.sched.cached_prefix([int(t) for t in tokens])
             idx = torch.tensor(blocks, dtype=torch.long, device=self.device)
-            kv = self.runner.kv.index_select(2, idx).cpu()
+            kv = self.runner.read_pages(idx)
         n = len(blocks) * self.cfg.block_size
-        return CacheEntry([int(t) for t in tokens[:n]], kv, n, self.mcfg.name, self.cfg.block_size, self.tp_rank)
+        meta = {} if self.cfg.kv_cache_dtype is None else {"kv_cache_dtype": self.cfg.kv_cache_dtype}
+        return CacheEntry([int(t) for t in tokens[:n]], kv, n, self.mcfg.name, self.cfg.block_size, self.tp_rank, meta)
 
     def import_prefix(self, entry) -> int:
         """Install a CacheEntry into the prefix cache; returns #pages newly written."""
-        if self.stateful or self.runner.kv is None:
+        if self.stateful or (self.runner.kv is None and self.runner.kv_quant is None):
             raise ValueError("prefix import needs the engine's own page layout")
         if entry.block_size != self.cfg.block_size:
             raise ValueError(f"entry block_size {entry.block_size} != engine {self.cfg.block_size}")
-        want = tuple(self.runner.kv.shape[:2]) + (entry.kv.shape[2],) + tuple(self.runner.kv.shape[3:])
+        if entry.meta.get("kv_cache_dtype") != self.cfg.kv_cache_dtype:
+            raise ValueError(f"entry KV dtype {entry.meta.get('kv_cache_dtype')} != engine {self.cfg.kv_cache_dtype}")
+        page_dim = 2 if self.runner.kv_quant is None else 1
+        n_pages = entry.kv.shape[page_dim] if entry.kv.dim() > page_dim else 0
+        want = self.runner.page_shape(n_pages)
         if tuple(entry.kv.shape) != want:
             raise ValueError(f"entry KV shape {tuple(entry.kv.shape)} does not match this engine {want}")
-        n_pages = entry.kv.shape[2]
         with self._lock:
             res = self.sched.install_prefix([int(t) for t in entry.key], n_pages)
             if not res:
@@ -866,8 +875,7 @@ class LLMEngine:
             before, blocks = res[0], res[1:]
             if len(blocks) > before:
                 idx = torch.tensor(blocks[before:], dtype=torch.long, device=self.device)
-                src = entry.kv[:, :, before:len(blocks)].to(self.device, self.runner.kv.dtype)
-                self.runner.kv.index_copy_(2, idx, src)
+                self.runner.write_pages(idx, entry.kv.narrow(page_dim, before, len(blocks) - before))
         return len(blocks) - before
 
     def set_decode_prefill_cap(self, cap: Optional[int] = None) -> None:

@@ -2,13 +2,14 @@
 Property 12 "deserialize(serialize(entry)) == entry").
 
 A CacheEntry is a page-aligned token prefix plus its KV tensors in the
-engine's paged layout, gathered into [L, 2, n_pages, Hkv, block_size, D].
+engine's paged layout, gathered into [L, 2, n_pages, Hkv, block_size, D] (an
+8-bit cache: its pages' bytes, [L, n_pages, Hkv, bytes]).
 Wire format (little endian):
 
     b"XGKV" | u32 version | u64 header_len | header JSON | raw tensor bytes
 
 header = {key, token_count, dtype, shape, model, block_size, tp_rank}. The
-payload is the tensor's raw memory (bf16/fp16/fp32), so a round trip is
+payload is the tensor's raw memory (bf16/fp16/fp32/uint8), so a round trip is
 bit-exact. `LLMEngine.export_prefix` / `import_prefix` move entries in and
 out of the radix prefix cache (warm restarts, cross-replica prefix sharing).
 """
@@ -25,13 +26,14 @@ from ..core.errors import CacheDeserialization, CacheSerialization
 
 MAGIC = b"XGKV"
 VERSION = 1
-_DTYPES = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32}
+_DTYPES = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32,
+           "uint8": torch.uint8}
 
 
 @dataclass
 class CacheEntry:
     key: List[int]                 # the cached token prefix (page aligned)
-    kv: torch.Tensor               # [L, 2, n_pages, Hkv, block_size, D]
+    kv: torch.Tensor               # [L, 2, n_pages, Hkv, block_size, D], or an 8-bit cache's bytes
     token_count: int
     model: str = ""
     block_size: int = 16

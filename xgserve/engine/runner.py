@@ -2,7 +2,8 @@
 
 * The paged KV cache is one zero-initialised HBM tensor [L, 2, NB, Hkv, bs, D]
   (zero-init: stale pages can never inject NaN into masked lanes), sized from
-  the free HBM left after the weights (gpu_memory_utilization of 288 GB).
+  the free HBM left after the weights (gpu_memory_utilization of 288 GB), or
+  with kv_cache_dtype an 8-bit cache a layer (ops.QuantKVCache: twice the tokens).
 * All per-step int32 metadata of an eager step is packed into ONE pinned host
   buffer and moved with ONE async H2D copy.
 * Pure-decode steps replay a HIP graph captured per padded batch size; the
@@ -104,7 +105,7 @@ class ModelRunner:
     def __init__(self, model, *, block_size: int, num_blocks: int, max_num_seqs: int,
                  max_num_batched_tokens: int, max_model_len: int, use_graphs: bool = True,
                  graph_batch_sizes: Optional[List[int]] = None, is_driver: bool = True,
-                 mixed_chunk: int = 0):
+                 mixed_chunk: int = 0, kv_cache_dtype: Optional[str] = None):
         self.model = model
         self.cfg = model.cfg
         self.device = model.device
@@ -124,9 +125,16 @@ class ModelRunner:
         # layout of their own allocate it themselves: pages + one state row per sequence slot.
         # needs_seq_meta: no such state, but operators that take the step's per-sequence view
         self.seq_state = bool(getattr(model, "has_sequence_state", False) or getattr(model, "needs_seq_meta", False))
+        self.kv_quant: Optional[List[ops.QuantKVCache]] = None
+        if kv_cache_dtype is not None and (hasattr(model, "alloc_cache") or self.dtype != torch.bfloat16):
+            raise ValueError(f"{cfg.name}: an 8-bit KV cache needs the engine's own page layout and bfloat16 activations")
         if hasattr(model, "alloc_cache"):
             self.kv = None
             self.kv_caches = model.alloc_cache(num_blocks, block_size, max_num_seqs)
+        elif kv_cache_dtype is not None:
+            self.kv = None
+            self.kv_caches = self.kv_quant = [ops.QuantKVCache.alloc(num_blocks, self.Hkv, block_size, cfg.head_dim, kv_cache_dtype,
+                                                                     self.device) for _ in range(cfg.num_layers)]
         else:
             self.kv = torch.zeros(cfg.num_layers, 2, num_blocks, self.Hkv, block_size, cfg.head_dim,
                                   dtype=self.dtype, device=self.device)
@@ -137,7 +145,7 @@ class ModelRunner:
         Hq_local = cfg.num_heads // model.tp
         self.max_splits = tune.get_int("decode_max_splits", 16)
         self.workspace = DecodeWorkspace(max(max_num_seqs, 1), Hq_local, cfg.head_dim, self.max_splits,
-                                         self.device) if (self.is_cuda and self.kv is not None) else None
+                                         self.device) if (self.is_cuda and not hasattr(model, "alloc_cache")) else None
         # pinned staging for eager steps
         cap = 9 * max_num_batched_tokens + 4 * max_num_seqs * (self.max_blocks_per_seq + 6) + 64
         # two pinned host staging buffers + device twins: a step may return
@@ -194,9 +202,36 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ utils
     def kv_bytes(self) -> int:
+        if self.kv_quant is not None:
+            return sum(c.nbytes() for c in self.kv_quant)
         if self.kv is None:
             return self.kv_caches.nbytes()
         return self.kv.numel() * self.kv.element_size()
+
+    def read_pages(self, idx: torch.Tensor) -> torch.Tensor:
+        """Whole pages on the host: [L, 2, n, Hkv, bs, D], or an 8-bit cache's bytes (keys' codes, values' codes, scales)
+        [L, n, Hkv, bytes]."""
+        if self.kv_quant is None:
+            return self.kv.index_select(2, idx).cpu()
+        return torch.stack([torch.cat([t.index_select(0, idx).flatten(2).view(torch.uint8) for t in (c.k, c.v, c.scales)], 2)
+                            for c in self.kv_quant]).cpu()
+
+    def page_shape(self, n: int) -> Tuple[int, ...]:
+        """The shape of read_pages of n pages."""
+        if self.kv_quant is None:
+            return tuple(self.kv.shape[:2]) + (n,) + tuple(self.kv.shape[3:])
+        c = self.kv_quant[0]
+        return (len(self.kv_quant), n, c.num_kv_heads, 2 * c.block_size * c.head_dim + 8 * c.block_size)
+
+    def write_pages(self, idx: torch.Tensor, pages: torch.Tensor) -> None:
+        """read_pages' pages into pages idx."""
+        if self.kv_quant is None:
+            self.kv.index_copy_(2, idx, pages.to(self.device, self.kv.dtype))
+            return
+        for c, rows in zip(self.kv_quant, pages.to(self.device)):
+            codes = c.block_size * c.head_dim
+            for t, part in ((c.k, rows[..., :codes]), (c.v, rows[..., codes:2 * codes]), (c.scales, rows[..., 2 * codes:])):
+                t.index_copy_(0, idx, part.contiguous().view(t.dtype).view(len(idx), *t.shape[1:]))
 
     DECODE_SPLIT_WGS = 512
 

@@ -10,6 +10,7 @@ import torch
 
 from .. import ops
 from ..ops.attention import DecodeWorkspace
+from ..ops.kv_quant import QuantKVCache
 from ..parallel.state import get_state
 
 @dataclass
@@ -57,7 +58,8 @@ def init_weight(shape, std: float, device, dtype, gen: Optional[torch.Generator]
 
 
 class PagedAttention:
-    """q/k/v from a fused QKV row -> rope + paged KV append -> ragged attention."""
+    """q/k/v from a fused QKV row -> rope + paged KV append -> ragged attention. kv: a layer's bf16 pages (k, v), or its
+    `QuantKVCache`."""
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, use_rope: bool = True):
         self.Hq = num_heads
@@ -69,6 +71,9 @@ class PagedAttention:
     def __call__(self, qkv: torch.Tensor, meta: AttnMeta, kv: Tuple[torch.Tensor, torch.Tensor],
                  cos_sin: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         T = qkv.shape[0]
+        if isinstance(kv, QuantKVCache):
+            ops.rope_kv_quant(qkv, meta.positions, cos_sin, kv, meta.slot_mapping, self.Hq, self.use_rope)
+            return self.attend(qkv[:, :self.Hq * self.D].view(T, self.Hq, self.D), meta, kv, out)
         kc, vc = kv
         ops.rope_cache(qkv, meta.positions, cos_sin, kc, vc, meta.slot_mapping, self.Hq, self.Hkv, self.D,
                        self.use_rope)
@@ -79,6 +84,9 @@ class PagedAttention:
                       cos_sin: torch.Tensor) -> torch.Tensor:
         """QKV as split-K partial sums (decode skinny GEMM): reduce + rope + KV append in one kernel."""
         T = meta.num_tokens
+        if isinstance(kv, QuantKVCache):
+            q = ops.rope_kv_quant_partials(pend, meta.positions, cos_sin, kv, meta.slot_mapping, self.Hq, self.use_rope)
+            return self.attend(q.view(T, self.Hq, self.D), meta, kv)
         q = torch.empty(T, self.Hq * self.D, dtype=torch.bfloat16, device=pend.part.device)
         ops.rope_cache_partials(pend, q, meta.positions, cos_sin, kv[0], kv[1], meta.slot_mapping, self.Hq,
                                 self.Hkv, self.D, self.use_rope)
@@ -87,7 +95,10 @@ class PagedAttention:
     def fused_decode(self, pend, meta: AttnMeta, kv: Tuple[torch.Tensor, torch.Tensor],
                      cos_sin: torch.Tensor) -> torch.Tensor:
         """Pure-decode step on QKV split-K partials: the attention kernel's prologue
-        reduces them, applies RoPE and appends K/V (ops.decode_attention_fused)."""
+        reduces them, applies RoPE and appends K/V (ops.decode_attention_fused; an 8-bit
+        cache: a launch of its own)."""
+        if isinstance(kv, QuantKVCache):
+            return self.from_partials(pend, meta, kv, cos_sin)
         return ops.decode_attention_fused(pend, meta.positions, meta.slot_mapping, cos_sin, kv[0], kv[1],
                                           meta.dec_block_tables, meta.dec_seq_lens, self.Hq, self.scale,
                                           meta.num_splits, meta.workspace, self.use_rope)
@@ -95,10 +106,18 @@ class PagedAttention:
     def attend(self, q: torch.Tensor, meta: AttnMeta, kv: Tuple[torch.Tensor, torch.Tensor],
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         T = q.shape[0]
-        kc, vc = kv
         if out is None:
             out = torch.empty(T, self.Hq, self.D, dtype=q.dtype, device=q.device)
         nd = meta.num_decodes
+        if isinstance(kv, QuantKVCache):
+            if nd > 0:
+                ops.quant_decode_attention(q[:nd], kv, meta.dec_block_tables, meta.dec_seq_lens, self.scale, meta.num_splits,
+                                           meta.workspace, out=out[:nd])
+            if T > nd:
+                ops.quant_prefill_attention(q[nd:], kv, meta.pre_block_tables, meta.pre_qsl, meta.pre_seq_lens, meta.pre_max_q,
+                                            self.scale, out=out[nd:])
+            return out.view(T, self.Hq * self.D)
+        kc, vc = kv
         # (decode rows' attention on a side stream under the prefill chunk's attention
         # measured within noise, profiles/r2_mixed_attn_overlap.md)
         if nd > 0:

@@ -244,6 +244,13 @@ def _append(cache, q, k, v, slots, positions, cos_sin, Hq) -> None:
                         bs, stream_ptr())
 
 
+def _check_cos_sin(cos_sin: torch.Tensor, cache: QuantKVCache) -> None:
+    if cos_sin.dtype is not torch.float32:
+        raise TypeError("cos_sin must be float32")
+    if not (cos_sin.dim() == 2 and cos_sin.shape[1] == cache.head_dim and cos_sin.is_contiguous() and cos_sin.get_device() == cache.index):
+        raise ValueError(f"cos_sin must be a contiguous [max_pos, {cache.head_dim}] table beside the cache")
+
+
 def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, cache: QuantKVCache,
                   slot_mapping: torch.Tensor, num_heads: int, apply_rope: bool = True) -> None:
     """`rope_cache` for an 8-bit cache: rows qkv [T, (Hq + 2 Hkv) D] bf16, q rotated in place, k rotated (to bf16, as the bf16
@@ -259,10 +266,7 @@ def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
     _int32(slot_mapping, "slot_mapping", 1, cache.device)
     _int32(positions, "positions", 1, cache.device)
     _need(slot_mapping.shape[0] == T and positions.shape[0] == T, f"slot_mapping and positions must have {T} entries")
-    if cos_sin.dtype != torch.float32:
-        raise TypeError("cos_sin must be float32")
-    _need(cos_sin.dim() == 2 and cos_sin.shape[1] == D and cos_sin.is_contiguous() and cos_sin.device == cache.device,
-          f"cos_sin must be a contiguous [max_pos, {D}] table beside the cache")
+    _check_cos_sin(cos_sin, cache)
     if T == 0:
         return
     if not _native(cache.k):
@@ -272,6 +276,40 @@ def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
         q.copy_(_rotate(q.float(), cos, sin).to(qkv.dtype))
         return kv_quant_append_ref(_rotate(k.float(), cos, sin).to(torch.bfloat16), v, cache, slot_mapping)
     _append(cache, qkv, k, v, slot_mapping, positions, cos_sin, num_heads)
+
+
+def rope_kv_quant_partials(pend, positions: torch.Tensor, cos_sin: torch.Tensor, cache: QuantKVCache, slot_mapping: torch.Tensor,
+                           num_heads: int, apply_rope: bool = True) -> torch.Tensor:
+    """`rope_cache_partials` for an 8-bit cache: QKV as split-K partial sums (PendingSum [S, T, (Hq + 2 Hkv) D]); k and v to the
+    cache, q -> [T, Hq D] bf16."""
+    H, D = cache.num_kv_heads, cache.head_dim
+    S, T, W = pend.part.shape
+    index = cache.index
+    if not (W == (num_heads + 2 * H) * D and pend.part.dtype is torch.float32 and pend.part.is_contiguous()
+            and pend.part.get_device() == index and pend.part.data_ptr() % 16 == 0):
+        raise ValueError(f"partial sums must be contiguous float32 [S, T, {(num_heads + 2 * H) * D}] beside the cache")
+    if not (_plain_lists(index, T, slot_mapping, positions)):
+        _int32(slot_mapping, "slot_mapping", 1, cache.device)
+        _int32(positions, "positions", 1, cache.device)
+        _need(slot_mapping.shape[0] == T and positions.shape[0] == T, f"slot_mapping and positions must have {T} entries")
+    _check_cos_sin(cos_sin, cache)
+    q = torch.empty(T, num_heads * D, dtype=torch.bfloat16, device=cache.device)
+    if T == 0:
+        return q
+    if not _native(cache.k):
+        qkv = pend.part.sum(0)
+        k, v = (qkv[:, (num_heads + i * H) * D:(num_heads + (i + 1) * H) * D].unflatten(1, (H, D)) for i in (0, 1))
+        x = qkv[:, :num_heads * D].unflatten(1, (num_heads, D))
+        if apply_rope:
+            cs = cos_sin[positions.long()]
+            x, k = (_rotate(y, cs[:, None, :D // 2], cs[:, None, D // 2:]) for y in (x, k))
+        kv_quant_append_ref(k.to(torch.bfloat16), v.to(torch.bfloat16), cache, slot_mapping)
+        return q.copy_(x.flatten(1))
+    nb, _, bs, _ = cache.dims
+    kernels().kv_append_partials(cache.code, pend.part.data_ptr(), S, q.data_ptr(), q.stride(0), slot_mapping.data_ptr(),
+                                 positions.data_ptr(), cos_sin.data_ptr() if apply_rope else 0, cache.k.data_ptr(),
+                                 cache.v.data_ptr(), cache.scales.data_ptr(), nb, T, num_heads, H, D, bs, stream_ptr())
+    return q
 
 
 def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch.Tensor, cu_tokens: torch.Tensor, num_tokens: int,

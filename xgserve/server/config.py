@@ -102,6 +102,8 @@ class WorkerSection:
     # and int4 (per 128-k group scales) are weight-only copies for decode batches <= 64,
     # bf16 activations (Req 10.3; the reference's Q8_0 / Q4_0 levels)
     quantization: str = "bf16"
+    # fp8 | int8: the KV cache in 8 bits, a scale per token and head; None: the activations' type
+    kv_cache_dtype: Optional[str] = None
     block_size: int = 16
     max_num_seqs: int = 256
     max_num_batched_tokens: int = 8192
@@ -201,6 +203,10 @@ class ServerConfig:
             e.append("worker.replicas and worker.tp must be > 0")
         if w.quantization not in ("bf16", "fp16", "fp32", "fp8", "int8", "int4"):
             e.append(f"worker.quantization {w.quantization!r} not supported (bf16|fp16|fp32|fp8|int8|int4)")
+        if w.kv_cache_dtype not in (None, "fp8", "int8"):
+            e.append(f"worker.kv_cache_dtype {w.kv_cache_dtype!r} not supported (fp8|int8)")
+        elif w.kv_cache_dtype is not None and w.quantization in ("fp16", "fp32"):
+            e.append("worker.kv_cache_dtype needs bf16 activations")
         if not (0.0 < w.gpu_memory_utilization <= 1.0):
             e.append("worker.gpu_memory_utilization must be in (0, 1]")
         if w.block_size % 16:
