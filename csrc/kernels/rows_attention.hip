@@ -11,7 +11,7 @@
 //   O^T[D][16 rows] += V^T P^T      the same instruction over 32 keys. The S^T accumulators are the P^T fragment where
 //     the 8 keys of lane group g are 4 g + {0..3} of both 16-key halves; the cache holds V in that order (bf16: V is
 //     turned through LDS). V's scale joins the weight before its rounding to bf16 (2^-9, as everywhere here)
-// The waves' states join through LDS, splits of a long range through decode_join_kernel: (O / l, log2-sum-exp) in fp32.
+// The waves' states join through LDS, parts of a row's keys through rows_join_kernel: (O / l, log2-sum-exp) in fp32.
 //
 // Waves share no tile, so the key loop has no barrier, and K / V go from HBM to registers: one tile's loads are on their
 // way while another is worked on. Rows without keys give zeros. Keys outside a row's range are never read into its result,
@@ -35,13 +35,12 @@ struct RowsArgs {
   int64_t table_stride;
   int width, num_blocks;
   const int32_t* seq_lens;
-  float* part_out;        // [tokens, Hq, slots, D], slots > 1
-  float* part_lse;        // [tokens, Hq, slots]
+  float* part_out;        // [parts, D]; null: whole rows, written to `out`
+  float* part_lse;        // [parts]
   uint16_t* out;
   int64_t out_stride;
   int Hq, Hkv, G, bs;
   float scale;            // softmax's, in base 2
-  int slots;              // parts of a row (1: `out` is written here)
   uint32_t page_magic;    // page_of
 };
 
@@ -69,7 +68,9 @@ struct RowsBlock {
   int block;              // which 16 RT of the list's ntok G rows
   int table;              // row of `tables`
   int kbeg, kend;         // keys
-  int slot;               // of the rows' parts
+  bool whole;             // its rows have no other parts: they go to `out`
+  int64_t part0;          // else row (token, head) writes part part0 + (token Hq + head) part_step
+  int part_step;
   int causal0;            // >= 0: token i sees keys < causal0 + i + 1; OWN: those below its seq_lens; ALL: all (below kend, each)
 };
 enum : int { OWN = -1, ALL = -2 };
@@ -445,11 +446,11 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
       const float inv = sum == 0.f ? 0.f : 1.f / sum;   // (a row that sees no key)
       const int tok = r / p.G, head = kvh * p.G + r - tok * p.G;
       const int64_t at = static_cast<int64_t>(w.tok0 + tok);
-      if (p.slots == 1) {
+      if (w.whole) {
         *reinterpret_cast<uint2*>(p.out + at * p.out_stride + static_cast<int64_t>(head) * D + d) =
             make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
       } else {
-        const int64_t part = (at * p.Hq + head) * p.slots + w.slot;
+        const int64_t part = w.part0 + (at * p.Hq + head) * w.part_step;
         *reinterpret_cast<float4*>(p.part_out + part * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         if (d == 0) p.part_lse[part] = sum == 0.f ? -INFINITY : M + __log2f(sum);
       }
@@ -669,14 +670,14 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int tok = r / p.G, head = kvh * p.G + r - tok * p.G;
     const int64_t at = static_cast<int64_t>(w.tok0 + tok);
-    if (p.slots == 1) {
+    if (w.whole) {
       uint16_t* dst = p.out + at * p.out_stride + static_cast<int64_t>(head) * D + 4 * g;
 #pragma unroll
       for (int mt = 0; mt < C::MT; ++mt)
         *reinterpret_cast<uint2*>(dst + 16 * mt) = make_uint2(pack2(acc[rt][mt][0] * inv, acc[rt][mt][1] * inv),
                                                               pack2(acc[rt][mt][2] * inv, acc[rt][mt][3] * inv));
     } else {
-      const int64_t part = (at * p.Hq + head) * p.slots + w.slot;
+      const int64_t part = w.part0 + (at * p.Hq + head) * w.part_step;
 #pragma unroll
       for (int mt = 0; mt < C::MT; ++mt)
         *reinterpret_cast<float4*>(p.part_out + part * D + 16 * mt + 4 * g) =
@@ -698,29 +699,142 @@ __device__ __forceinline__ void share(int& kbeg, int& kend, int split, int split
   kend = min(kend, 32 * (first + min(tiles, (split + 1) * each)));
 }
 
-// One new token of sequence b, its heads' block `block` of 16: share `split` of `splits` of its keys, from `start` on.
+// ---- decode: shares of the batch's keys -------------------------------------------------------------------------------------
+// A batch's sequences are of any lengths, which the host does not know, so the keys are shared out here: of `shares` workgroups a kv
+// head (and block of 16 query heads) each takes up to `run` units of 128 keys (a 32-key tile a wave) of one sequence, with run the
+// batch's units over shares - B. So a sequence has ceil(units / run) parts, at least one, and all have shares at most. (With as many
+// parts for each sequence the longest one bounds the step: 1 sequence of 60 k keys beside 63 of 500, fp8, took 423 us, and takes 42.)
+constexpr int MAX_PARTS = 128;
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+#else
+  return v;
+#endif
+}
+// sums of the lanes up to each
+__device__ __forceinline__ int wave_scan(int v) {
+  v = scan_step<0x111, 0xF>(v);
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);
+  return scan_step<0x143, 0xC>(v);
+}
+
+struct Share {
+  int b, part;            // sequence (-1: none) and which of its parts
+  int parts, first;       // its parts, and the share that is its first
+  int kbeg, kend;
+};
+
+__device__ __forceinline__ void own_keys(const RowsArgs& p, const int32_t* starts, int b, int& kbeg, int& kend) {
+  kend = min(max(p.seq_lens[b], 0), p.width * p.bs);
+  kbeg = starts ? min(max(starts[b], 0), kend) : 0;
+}
+
+// Share i, or (of >= 0) the first share of sequence `of`, of a batch whose keys are cut; AT_ONCE lengths a lane at a time.
+template <int AT_ONCE>
+__device__ __forceinline__ void cut_share(const RowsArgs& p, const int32_t* starts, int B, int shares, int i, int of, Share& s, int& run) {
+  const int lane = threadIdx.x & 63;
+  int u[AT_ONCE];
+  auto units = [&](int b0) {
+    int kbeg[AT_ONCE], kend[AT_ONCE];
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a) own_keys(p, starts, min(b0 + 64 * a + lane, B - 1), kbeg[a], kend[a]);
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a)
+      u[a] = b0 + 64 * a + lane < B && kend[a] > kbeg[a] ? (((kend[a] + 31) >> 5) - (kbeg[a] >> 5) + 3) >> 2 : 0;
+  };
+  int all = 0, most = 0;
+  for (int b0 = 0; b0 < B; b0 += 64 * AT_ONCE) {
+    units(b0);
+    int sum = 0;
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a) {
+      sum += u[a];
+      most = max(most, u[a]);
+    }
+    all += __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  }
+  most = __float_as_int(wave_join(__int_as_float(most), [](float x, float y) { return __int_as_float(max(__float_as_int(x), __float_as_int(y))); }));
+  run = __builtin_amdgcn_readfirstlane(max(max(1, (all + shares - B - 1) / (shares - B)), (most + MAX_PARTS - 1) / MAX_PARTS));
+  int before = 0;
+  for (int b0 = 0; b0 < B && s.b < 0; b0 += 64 * AT_ONCE) {
+    if (B > 64 * AT_ONCE) units(b0);
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a) {
+      const int b = b0 + 64 * a + lane, parts = b < B ? max(1, (u[a] + run - 1) / run) : 0;
+      const int upto = before + wave_scan(parts);
+      const uint64_t who = __ballot(of >= 0 ? b == of : i >= upto - parts && i < upto);
+      if (who) {
+        const int l = __builtin_ctzll(who);
+        s.b = b0 + 64 * a + l;
+        s.parts = __builtin_amdgcn_readlane(parts, l);
+        s.first = __builtin_amdgcn_readlane(upto, l) - s.parts;
+      }
+      before = __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+}
+
+// All lanes of the wave take part.
+__device__ __forceinline__ Share find_share(const RowsArgs& p, const int32_t* starts, int B, int shares, int i, int of) {
+  Share s{-1, 0, 1, 0, 0, 0};
+  int run = 0;
+  if (shares <= B) {
+    s.b = s.first = of >= 0 ? of : i;
+    if (s.b >= B) s.b = -1;
+  } else if (B <= 64) {
+    cut_share<1>(p, starts, B, shares, i, of, s, run);
+  } else {
+    cut_share<4>(p, starts, B, shares, i, of, s, run);
+  }
+  s.b = __builtin_amdgcn_readfirstlane(s.b);
+  s.first = __builtin_amdgcn_readfirstlane(s.first);
+  s.parts = __builtin_amdgcn_readfirstlane(s.parts);
+  s.part = of >= 0 ? 0 : i - s.first;
+  if (s.b >= 0) {
+    own_keys(p, starts, s.b, s.kbeg, s.kend);
+    s.kbeg = __builtin_amdgcn_readfirstlane(s.kbeg);
+    s.kend = __builtin_amdgcn_readfirstlane(s.kend);
+    if (s.parts > 1) {
+      const int first = s.kbeg >> 5;
+      s.kend = min(s.kend, 32 * (first + (s.part + 1) * 4 * run));
+      s.kbeg = max(s.kbeg, 32 * (first + s.part * 4 * run));
+    }
+  }
+  return s;
+}
+
+// Share i of the sequences' new tokens, block `block` of their heads. counts: each sequence's parts besides.
 template <int FMT, int D>
-__device__ __forceinline__ void decode_block(const RowsArgs& p, int kvh, int b, int block, int start, int split, int splits, int slot,
-                                             uint8_t* space, float (*m_lds)[16], float (*l_lds)[16]) {
+__device__ __forceinline__ void decode_share(const RowsArgs& p, int kvh, const int32_t* starts, const int32_t* counts, int B, int shares,
+                                             int i, int block, int64_t part0, uint8_t* space, float (*m_lds)[16], float (*l_lds)[16]) {
+  const Share s = find_share(p, starts, B, shares, i, -1);
+  if (s.b < 0) return;
   RowsBlock w;
-  w.tok0 = w.table = b;
+  w.tok0 = w.table = s.b;
   w.ntok = 1;
   w.block = block;
-  w.kend = min(max(p.seq_lens[b], 0), p.width * p.bs);
-  w.kbeg = min(max(start, 0), w.kend);
-  share(w.kbeg, w.kend, split, splits);
+  w.kbeg = s.kbeg;
+  w.kend = s.kend;
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
-  w.slot = slot;
+  w.whole = s.parts == 1 && !(counts && counts[s.b] > 0);
+  w.part0 = part0 + static_cast<int64_t>(i - s.b) * p.Hq;   // (share i's rows: i Hq + head)
+  w.part_step = 1;
   w.causal0 = ALL;
   attend_rows<FMT, D, 1, true>(p, w, kvh, space, m_lds, l_lds);
 }
 
-// One new token of each sequence. Grid (Hkv, B heads' blocks of 16, splits).
+// One new token of each sequence. Grid (Hkv, shares heads' blocks of 16).
 template <int FMT, int D>
-__global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, int blocks, int splits) {
+__global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, int B, int blocks, int shares) {
   XGK_ROWS_LDS(FMT, D, 1);
-  const int b = blockIdx.y / blocks;
-  decode_block<FMT, D>(p, blockIdx.x, b, blockIdx.y - b * blocks, 0, blockIdx.z, splits, blockIdx.z, space, m_lds, l_lds);
+  const int i = blockIdx.y / blocks;
+  decode_share<FMT, D>(p, blockIdx.x, nullptr, nullptr, B, shares, i, blockIdx.y - i * blocks, 0, space, m_lds, l_lds);
 }
 
 // Prompt portions, causal. Grid (Hkv, blocks of rows of the longest, sequences splits). Late blocks see the most keys: first.
@@ -740,7 +854,9 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsA
   w.kend = max(0, min(len, w.causal0 + last_tok + 1));
   share(w.kbeg, w.kend, blockIdx.z - s * splits, splits);
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
-  w.slot = blockIdx.z - s * splits;
+  w.whole = splits == 1;
+  w.part0 = blockIdx.z - s * splits;
+  w.part_step = splits;
   if constexpr (RT == 8) {
     __shared__ __attribute__((aligned(16))) uint8_t space[BlockCfg<FMT, D>::SPACE];
     attend_block<FMT, D>(p, w, blockIdx.x, space);
@@ -751,15 +867,16 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsA
 }
 
 // Groups of decode rows with common keys, in one launch: first the common parts (items [n][8]: first sequence, sequences, block of
-// rows, first key, end key, slot), then each sequence's own keys. The first are bound by the vector and matrix work, the others by
-// HBM, and run beside each other. Grid (Hkv, n_items + B heads' blocks of 16, splits of the own keys).
+// rows, first key, end key, slot), then the shares of the sequences' own keys. The first are bound by the vector and matrix work, the
+// others by HBM, and run beside each other. Grid (Hkv, n_items + shares heads' blocks of 16). Parts: slots a row of the common
+// ones, then the shares'.
 template <int FMT, int D, int RT>
 __global__ void __launch_bounds__(256, 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
-                                                             int prefix_slots, int blocks, int splits) {
+                                                             const int32_t* counts, int slots, int B, int blocks, int shares) {
   XGK_ROWS_LDS(FMT, D, RT);
   if (blockIdx.y >= n_items) {
-    const int i = blockIdx.y - n_items, split = i % splits, row = i / splits, b = row / blocks;
-    decode_block<FMT, D>(p, blockIdx.x, b, row - b * blocks, prefix[b], split, splits, prefix_slots + split, space,
+    const int at = blockIdx.y - n_items, i = at / blocks;
+    decode_share<FMT, D>(p, blockIdx.x, prefix, counts, B, shares, i, at - i * blocks, static_cast<int64_t>(B) * p.Hq * slots, space,
                          reinterpret_cast<float(*)[16]>(m_lds), reinterpret_cast<float(*)[16]>(l_lds));
     return;
   }
@@ -771,115 +888,146 @@ __global__ void __launch_bounds__(256, 2) rows_shared_kernel(RowsArgs p, const i
   w.kend = min(it[4], p.width * p.bs);
   w.kbeg = min(it[3], w.kend);
   if (w.kbeg >= w.kend) w.kbeg = w.kend = 0;
-  w.slot = it[5];
+  w.whole = false;
+  w.part0 = it[5];
+  w.part_step = slots;
   w.causal0 = OWN;
   attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, m_lds, l_lds);
 }
 
-// Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). counts (with first_free): the first counts[token]
-// slots and those from first_free on hold parts; else all. qsl: tokens outside [qsl[0], qsl[S]) have none. A workgroup has a row,
-// four dims a thread, and 1024 / D parts at once: 57 parts of 72 rows take 2.6 us, and took 8.3 with a row's parts one behind the
-// other in D / 4 threads.
-template <int D>
-__global__ void __launch_bounds__(256) rows_join_kernel(const float* __restrict__ part_out, const float* __restrict__ part_lse,
-                                                        uint16_t* __restrict__ out, int64_t out_stride, int Hq, int slots,
-                                                        const int32_t* __restrict__ counts, int first_free,
-                                                        const int32_t* __restrict__ qsl, int S) {
-  constexpr int TPR = D / 4, AT_ONCE = 256 / TPR;
-  __shared__ float sums[AT_ONCE], tops[AT_ONCE];
-  __shared__ __attribute__((aligned(16))) float outs[AT_ONCE][D];
-  const int64_t row = blockIdx.x;
-  const int tok = row / Hq, head = row - static_cast<int64_t>(tok) * Hq;
-  if (qsl && (tok < qsl[0] || tok >= qsl[S])) return;
-  const int d = threadIdx.x % TPR * 4, mine = threadIdx.x / TPR;
-  const int front = counts ? min(max(counts[tok], 0), first_free) : slots;
-  const int n = counts ? front + slots - first_free : slots;
-  const float* lse = part_lse + row * slots;
-  const float* po = part_out + row * slots * D + d;
+// Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). They are the first counts[token] (null: all) of the
+// row's `slots`, and, of `shares`, its sequence's; rows of one part are in `out` already. qsl: tokens outside [qsl[0], qsl[S]) have
+// none. A workgroup has ROWS rows of a token, four dims a thread, and 4 x 1024 / (D ROWS) parts of a row on their way at once: one row
+// where there are few (72 rows of 57 parts took 8.3 us with D / 4 threads a row), four where workgroups would only queue.
+struct JoinArgs {
+  const int32_t* counts;
+  int slots;
+  const int32_t* starts;
+  int B, shares;
+  const int32_t* qsl;
+  int S;
+};
+template <int D, int ROWS>
+__global__ void __launch_bounds__(256) rows_join_kernel(RowsArgs p, JoinArgs j) {
+  constexpr int TPR = D / 4, GROUPS = 256 / TPR, OF_ROW = GROUPS / ROWS, AHEAD = 4;
+  __shared__ float sums[GROUPS], tops[GROUPS];
+  __shared__ __attribute__((aligned(16))) float outs[GROUPS][D];
+  const int tok = blockIdx.x;
+  if (j.qsl && (tok < j.qsl[0] || tok >= j.qsl[j.S])) return;
+  const int d = threadIdx.x % TPR * 4, group = threadIdx.x / TPR, mine = group % OF_ROW;
+  const int head = blockIdx.y * ROWS + group / OF_ROW;
+  const int front = j.counts ? min(max(j.counts[tok], 0), j.slots) : j.slots;
+  int n = front, first = 0;
+  if (j.shares) {
+    const Share s = find_share(p, j.starts, j.B, j.shares, 0, tok);
+    n += s.parts;
+    first = s.first;
+    if (n == 1) return;
+  }
+  const int64_t row = static_cast<int64_t>(tok) * p.Hq + min(head, p.Hq - 1);
+  const int64_t back = (static_cast<int64_t>(j.B) * j.slots + first) * p.Hq + min(head, p.Hq - 1);
   float M = LOWEST, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = mine; i < n; i += AT_ONCE) {
-    const int s = i < front ? i : i - front + first_free;
-    const float e = lse[s];
-    const float4 x = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * D);
-    const float top = fmaxf(M, e), old = exp2_fast(M - top), f = exp2_fast(e - top);
+  for (int i0 = mine; i0 < n; i0 += AHEAD * OF_ROW) {
+    float e[AHEAD], top = M;
+    float4 x[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = min(i0 + a * OF_ROW, n - 1);
+      const int64_t part = i < front ? row * j.slots + i : back + static_cast<int64_t>(i - front) * p.Hq;
+      e[a] = p.part_lse[part];
+      x[a] = *reinterpret_cast<const float4*>(p.part_out + part * D + d);
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (i0 + a * OF_ROW >= n) e[a] = -INFINITY;
+      top = fmaxf(top, e[a]);
+    }
+    const float old = exp2_fast(M - top);
     M = top;
-    sum = sum * old + f;
-    o = make_float4(o.x * old + f * x.x, o.y * old + f * x.y, o.z * old + f * x.z, o.w * old + f * x.w);
+    sum *= old;
+    o = make_float4(o.x * old, o.y * old, o.z * old, o.w * old);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const float f = exp2_fast(e[a] - M);
+      sum += f;
+      o = make_float4(o.x + f * x[a].x, o.y + f * x[a].y, o.z + f * x[a].z, o.w + f * x[a].w);
+    }
   }
   if (d == 0) {
-    sums[mine] = sum;
-    tops[mine] = M;
+    sums[group] = sum;
+    tops[group] = M;
   }
-  *reinterpret_cast<float4*>(&outs[mine][d]) = o;
+  *reinterpret_cast<float4*>(&outs[group][d]) = o;
   __syncthreads();
-  if (mine != 0) return;
-  for (int i = 1; i < AT_ONCE; ++i) M = fmaxf(M, tops[i]);
+  if (mine != 0 || head >= p.Hq) return;
+#pragma unroll
+  for (int i = 1; i < OF_ROW; ++i) M = fmaxf(M, tops[group + i]);
   sum = 0.f;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < AT_ONCE; ++i) {
-    const float f = exp2_fast(tops[i] - M);
-    const float4 x = *reinterpret_cast<const float4*>(&outs[i][d]);
-    sum += sums[i] * f;
+  for (int i = 0; i < OF_ROW; ++i) {
+    const float f = exp2_fast(tops[group + i] - M);
+    const float4 x = *reinterpret_cast<const float4*>(&outs[group + i][d]);
+    sum += sums[group + i] * f;
     o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint2*>(out + tok * out_stride + static_cast<int64_t>(head) * D + d) =
+  *reinterpret_cast<uint2*>(p.out + tok * p.out_stride + static_cast<int64_t>(head) * D + d) =
       make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
 }
 
 static bool rows_ok(const RowsArgs& p, int D) {
   return p.bs > 0 && p.bs % KV_TILE == 0 && p.Hkv >= 1 && p.Hq % p.Hkv == 0 && (D == 64 || D == 128) && p.width >= 1 &&
-         p.num_blocks >= 1 && p.slots >= 1 && (p.slots == 1 || (p.part_out && p.part_lse)) && p.q_stride % 8 == 0 &&
+         p.num_blocks >= 1 && !p.part_out == !p.part_lse && p.q_stride % 8 == 0 &&
          p.out_stride % 4 == 0 && static_cast<int64_t>(p.width) * (p.bs / KV_TILE) * (p.bs / KV_TILE) < 1 << 30;
 }
 static uint32_t page_magic(int bs) { return bs >= KV_TILE ? (1u << 31) / (bs / KV_TILE) + 1 : 1; }
 
-static void join(const RowsArgs& p, int D, int tokens, const int32_t* counts, int first_free, const int32_t* qsl, int S,
-                 hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(tokens) * p.Hq);
-  if (D == 128)
-    hipLaunchKernelGGL(rows_join_kernel<128>, grid, dim3(256), 0, st, p.part_out, p.part_lse, p.out, p.out_stride, p.Hq, p.slots,
-                       counts, first_free, qsl, S);
-  else
-    hipLaunchKernelGGL(rows_join_kernel<64>, grid, dim3(256), 0, st, p.part_out, p.part_lse, p.out, p.out_stride, p.Hq, p.slots,
-                       counts, first_free, qsl, S);
+static void join(const RowsArgs& p, int D, int tokens, const JoinArgs& j, hipStream_t st) {
+  const bool few = static_cast<int64_t>(tokens) * p.Hq <= 512;
+  const dim3 grid(tokens, few ? p.Hq : (p.Hq + 3) / 4);
+  if (D == 128 && few) hipLaunchKernelGGL((rows_join_kernel<128, 1>), grid, dim3(256), 0, st, p, j);
+  else if (D == 128) hipLaunchKernelGGL((rows_join_kernel<128, 4>), grid, dim3(256), 0, st, p, j);
+  else if (few) hipLaunchKernelGGL((rows_join_kernel<64, 1>), grid, dim3(256), 0, st, p, j);
+  else hipLaunchKernelGGL((rows_join_kernel<64, 4>), grid, dim3(256), 0, st, p, j);
 }
 
 #define XGK_FMT_DIM(DO)                                                                                              \
   if (fmt == KV_FP8 && D == 128) DO(KV_FP8, 128) else if (fmt == KV_FP8) DO(KV_FP8, 64)                               \
   else if (fmt == KV_INT8 && D == 128) DO(KV_INT8, 128) else if (fmt == KV_INT8) DO(KV_INT8, 64)
 
-// Decode over an 8-bit cache. Returns 0, or -1 for what it does not take.
+// Decode over an 8-bit cache. shares: B (whole rows), or more (part_out / part_lse: shares Hq parts). Returns 0, or -1 for what it
+// does not take.
 int quant_decode_attention(int fmt, const uint16_t* q, int64_t q_stride, const uint8_t* k, const uint8_t* v, const float* scales,
                            const int32_t* tables, int64_t table_stride, int width, const int32_t* seq_lens, float* part_out,
                            float* part_lse, uint16_t* out, int64_t out_stride, int B, int Hq, int Hkv, int D, int bs,
-                           int num_blocks, float scale, int splits, hipStream_t st) {
+                           int num_blocks, float scale, int shares, hipStream_t st) {
   if (B <= 0) return 0;
   const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
-                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits, page_magic(bs)};
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, page_magic(bs)};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || static_cast<int64_t>(B) * blocks > 65535 || splits > 65535) return -1;
-#define XGK_GO(F, DD)                                                                                                   \
-  {                                                                                                                     \
-    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, B * blocks, splits), dim3(256), 0, st, p, blocks, splits); \
+  if (!rows_ok(p, D) || shares < B || static_cast<int64_t>(shares) * blocks > 65535 || (shares > B) != (part_out != nullptr)) return -1;
+#define XGK_GO(F, DD)                                                                                                        \
+  {                                                                                                                          \
+    hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, shares * blocks), dim3(256), 0, st, p, B, blocks, shares);     \
   }
   XGK_FMT_DIM(XGK_GO) else return -1;
 #undef XGK_GO
-  if (splits > 1) join(p, D, B, nullptr, 0, nullptr, 0, st);
+  if (part_out) join(p, D, B, JoinArgs{nullptr, 0, nullptr, B, shares, nullptr, 0}, st);
   return 0;
 }
 
-// Causal attention of packed prompt portions over an 8-bit cache; 16 RT rows a workgroup.
+// Causal attention of packed prompt portions over an 8-bit cache; 16 RT rows a workgroup, `splits` parts of their keys (parts:
+// tokens Hq splits).
 int quant_prefill_attention(int fmt, const uint16_t* q, int64_t q_stride, const uint8_t* k, const uint8_t* v, const float* scales,
                             const int32_t* tables, int64_t table_stride, int width, const int32_t* qsl, const int32_t* seq_lens,
                             float* part_out, float* part_lse, uint16_t* out, int64_t out_stride, int tokens, int S, int max_q,
                             int Hq, int Hkv, int D, int bs, int num_blocks, float scale, int RT, int splits, hipStream_t st) {
   if (tokens <= 0 || S <= 0 || max_q <= 0) return 0;
   const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
-                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, splits, page_magic(bs)};
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8)) return -1;
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, page_magic(bs)};
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8) || splits < 1 || (splits > 1) != (part_out != nullptr)) return -1;
   const int64_t blocks = (static_cast<int64_t>(max_q) * p.G + 16 * RT - 1) / (16 * RT);
   if (blocks > 65535 || static_cast<int64_t>(S) * splits > 65535) return -1;
   const dim3 grid(Hkv, static_cast<unsigned>(blocks), S * splits);
@@ -891,39 +1039,40 @@ int quant_prefill_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
   }
   XGK_FMT_DIM(XGK_GO) else return -1;
 #undef XGK_GO
-  if (splits > 1) join(p, D, tokens, nullptr, 0, qsl, S, st);
+  if (part_out) join(p, D, tokens, JoinArgs{nullptr, splits, nullptr, 0, 0, qsl, S}, st);
   return 0;
 }
 
-// Decode rows in groups with a common prefix. items: rows_prefix_kernel's, prefix: keys of each row that the items cover,
-// counts: its parts of them (at most prefix_slots), splits: parts of the rest.
+// Decode rows in groups with a common prefix. items: rows_shared_kernel's, prefix: keys of each row that the items cover, counts: its
+// parts of them (at most `slots`), shares: of the keys behind. Whole rows where slots is 0 and shares B; else B Hq slots + shares Hq
+// parts.
 int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const void* k, const void* v, const float* scales,
                             const int32_t* tables, int64_t table_stride, int width, const int32_t* seq_lens, float* part_out,
                             float* part_lse, uint16_t* out, int64_t out_stride, int B, int Hq, int Hkv, int D, int bs,
                             int num_blocks, float scale, const int32_t* items, int n_items, const int32_t* prefix,
-                            const int32_t* counts, int prefix_slots, int RT, int splits, hipStream_t st) {
+                            const int32_t* counts, int slots, int RT, int shares, hipStream_t st) {
   if (B <= 0) return 0;
   const RowsArgs p{q, q_stride, static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), scales, tables, table_stride,
                    width, num_blocks, seq_lens, part_out, part_lse, out, out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs,
-                   scale * 1.44269504088896341f, prefix_slots + splits, page_magic(bs)};
+                   scale * 1.44269504088896341f, page_magic(bs)};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2) || splits < 1 || prefix_slots < 0 || n_items < 0 ||
-      n_items + static_cast<int64_t>(B) * blocks * splits > 65535)
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2) || shares < B || slots < 0 || n_items < 0 ||
+      n_items + static_cast<int64_t>(shares) * blocks > 65535 || (slots > 0 || shares > B) != (part_out != nullptr))
     return -1;
-  const dim3 grid(Hkv, n_items + B * blocks * splits);
-#define XGK_GO(F, DD)                                                                                                     \
-  {                                                                                                                       \
-    if (RT == 1)                                                                                                          \
-      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 1>), grid, dim3(256), 0, st, p, items, n_items, prefix, prefix_slots, \
-                         blocks, splits);                                                                                 \
-    else                                                                                                                  \
-      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 2>), grid, dim3(256), 0, st, p, items, n_items, prefix, prefix_slots, \
-                         blocks, splits);                                                                                 \
+  const dim3 grid(Hkv, n_items + shares * blocks);
+#define XGK_GO(F, DD)                                                                                                          \
+  {                                                                                                                            \
+    if (RT == 1)                                                                                                               \
+      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 1>), grid, dim3(256), 0, st, p, items, n_items, prefix, counts, slots, B,  \
+                         blocks, shares);                                                                                      \
+    else                                                                                                                       \
+      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 2>), grid, dim3(256), 0, st, p, items, n_items, prefix, counts, slots, B,  \
+                         blocks, shares);                                                                                      \
   }
   XGK_FMT_DIM(XGK_GO)
   else if (fmt == KV_BF16 && D == 128) XGK_GO(KV_BF16, 128) else if (fmt == KV_BF16) XGK_GO(KV_BF16, 64) else return -1;
 #undef XGK_GO
-  if (p.slots > 1) join(p, D, B, counts, prefix_slots, nullptr, 0, st);
+  if (part_out) join(p, D, B, JoinArgs{counts, slots, prefix, B, shares, nullptr, 0}, st);
   return 0;
 }
 

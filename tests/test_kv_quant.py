@@ -342,6 +342,24 @@ def test_decode(dev, fmt, Hq, Hkv, D, bs, splits):
 
 
 @DEVICES
+@FORMATS
+@pytest.mark.parametrize("B,splits", [(3, 7), (64, 2), (65, 3), (130, 1), (300, 2), (300, None)])
+def test_decode_of_batches_of_any_lengths(dev, fmt, B, splits):
+    """Shares of the batch's keys: one long sequence among short and empty ones, more sequences than lanes of a wave, and of four."""
+    gen = torch.Generator().manual_seed(B)
+    lens = [(i * 37) % 90 for i in range(B)]
+    lens[B // 3], lens[-1] = 1500, 700
+    cache, table, truth = make(lens, 1, 64, 16, fmt, dev, gen)
+    q = rows(B, 4, 64, gen).to(dev)
+    out = ops.quant_decode_attention(q, cache, table, i32(lens, dev), 0.125, num_splits=splits)
+    some = range(B) if B < 100 else [0, 1, B // 3, 63, 64, 65, 127, 128, B - 2, B - 1]
+    for s in some:
+        check(out[s:s + 1], *attention(q[s:s + 1].double().cpu(), *truth[s], [lens[s]], 0.125))
+    same = ops.quant_decode_attention(q, cache, table, i32(lens, dev), 0.125, num_splits=splits)
+    assert torch.equal(out, same)
+
+
+@DEVICES
 def test_decode_into_a_strided_output_with_a_workspace(dev):
     gen = torch.Generator().manual_seed(2)
     lens = [200, 0, 77]

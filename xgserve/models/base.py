@@ -111,8 +111,7 @@ class PagedAttention:
         nd = meta.num_decodes
         if isinstance(kv, QuantKVCache):
             if nd > 0:
-                ops.quant_decode_attention(q[:nd], kv, meta.dec_block_tables, meta.dec_seq_lens, self.scale, meta.num_splits,
-                                           meta.workspace, out=out[:nd])
+                ops.quant_decode_attention(q[:nd], kv, meta.dec_block_tables, meta.dec_seq_lens, self.scale, out=out[:nd])
             if T > nd:
                 ops.quant_prefill_attention(q[nd:], kv, meta.pre_block_tables, meta.pre_qsl, meta.pre_seq_lens, meta.pre_max_q,
                                             self.scale, out=out[nd:])

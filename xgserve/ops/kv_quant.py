@@ -398,17 +398,28 @@ def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
     return int(num_splits)
 
 
-def _parts(workspace: Optional[DecodeWorkspace], rows: int, D: int, slots: int, device):
-    """The parts' buffer and the addresses of outputs and log-sums in it; rows: tokens times query heads."""
-    if slots <= 1:
-        return None, 0, 0
+def _shares(num_splits: Optional[int], B: int, wgs: int, max_keys: int) -> int:
+    """Shares of a batch's keys, which the kernel gives out by the sequences' lengths: B for one part each. wgs: workgroups a share.
+    Where the sequences alone fill most of the chip, only those longer than the mean are cut, and none where none can be long: us
+    whole and with that, 200 of 1500 keys on 8 kv heads 109 / 115, 128 of 64 - 2000 54 / 58, 64 of 5000 102 / 105, 1 of 60 k beside
+    63 of 500 424 / 40."""
+    if num_splits is None:
+        full = 8 * B * wgs >= 3 * SPLIT_WGS
+        if max_keys < SPLIT_FROM * (4 if full else 1):
+            return B
+        more = min(-(-SPLIT_WGS // wgs), B * -(-max_keys // SPLIT_KEYS))
+        return B + (min(more, B) if full else more)
+    return B * _splits(num_splits, 1, 0)
+
+
+def _parts(workspace: Optional[DecodeWorkspace], parts: int, D: int, device):
+    """The parts' buffer and the addresses of outputs [parts, D] and log-sums [parts] in it."""
     if workspace is None:
-        buf = torch.empty(rows * slots * (D + 1), dtype=torch.float32, device=device)
+        buf = torch.empty(parts * (D + 1), dtype=torch.float32, device=device)
         at = buf.data_ptr()
-        return buf, at, at + 4 * rows * slots * D
-    if (workspace.part_lse.device != device or workspace.part_lse.numel() < rows * slots
-            or workspace.part_out.numel() < rows * slots * D):
-        raise ValueError(f"the workspace is too small for {slots} parts of {rows} rows of {D}, or on another device")
+        return buf, at, at + 4 * parts * D
+    if workspace.part_lse.device != device or workspace.part_lse.numel() < parts or workspace.part_out.numel() < parts * D:
+        raise ValueError(f"the workspace is too small for {parts} parts of {D}, or on another device")
     return workspace, workspace.part_out.data_ptr(), workspace.part_lse.data_ptr()
 
 
@@ -417,15 +428,19 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`decode_attention` over an 8-bit cache: q [B, Hq, D] bf16 (tokens may be strided), one new token of each sequence, whose own
     key is in the cache already -> [B, Hq, D]. block_tables [B, W], seq_lens [B] int32; a length of 0 gives zeros, one behind the
-    table means the whole table. num_splits: parts of the key range (None: by the batch and the table's width)."""
+    table means the whole table. num_splits: parts that a sequence's keys are cut into on average, more the longer it is (None: by the
+    batch and the table's width); a workspace needs B num_splits of them."""
     (nb, Hkv, bs, D), dev = cache.dims, cache.device
     _check_decode(q, Hkv, D, cache.index, dev, block_tables, seq_lens)
     B, Hq, _ = q.shape
     out = _check_out(out, q)
     W = block_tables.shape[1]
-    splits = _splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs)
+    blocks = -(-Hq // Hkv // 16)
+    shares = _shares(num_splits, B, Hkv * blocks, W * bs)
     if B == 0:
         return out
+    if shares * blocks > 65535:
+        raise ValueError("at most 65535 parts (for each 16 query heads of a kv head)")
     if not _native(cache.k):
         for b in range(B):
             L = min(int(seq_lens[b]), W * bs)
@@ -434,11 +449,11 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
                 k, v = _any_rows_ref(cache, block_tables[b], 0, L)
                 out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
         return out
-    keep, po, pl = _parts(workspace, B * Hq, D, splits, dev)
+    keep, po, pl = _parts(workspace, shares * Hq, D, dev) if shares > B else (None, 0, 0)
     kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
                                      seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale,
-                                     splits, stream_ptr())
+                                     shares, stream_ptr())
     return out
 
 
@@ -490,7 +505,7 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
                 k, v = _any_rows_ref(cache, block_tables[s], 0, min(L, W * bs))
                 out[a:a + n] = _attend_causal(q[a:a + n], k, v, max(L - (b - a), 0), scale).to(q.dtype)
         return out
-    keep, po, pl = _parts(workspace, T * Hq, D, splits, dev)
+    keep, po, pl = _parts(workspace, T * Hq * splits, D, dev) if splits > 1 else (None, 0, 0)
     kernels().quant_prefill_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
                                       cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
                                       query_start_loc.data_ptr(), seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), T, S,
@@ -557,7 +572,7 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
     """Decode attention q [B, Hq, D] bf16 of sequences in groups with a common prefix, whose keys are read once for the group: of a
     group, the first prefix_lens[g] keys of every sequence are those of its first sequence's table, the rest its own table's; a
     sequence shorter than the prefix sees as much of it as it is long. kv: a `QuantKVCache`, or the bf16 pages (k, v) [NB, Hkv, bs,
-    D]. num_splits: parts of the keys behind the prefix. A workspace needs plan.slots + num_splits parts."""
+    D]. num_splits: parts of the keys behind the prefix, on average. A workspace needs B (plan.slots + num_splits) of them."""
     quant = isinstance(kv, QuantKVCache)
     if quant:
         kc, vc, (nb, Hkv, bs, D), fmt = kv.k, kv.v, kv.dims, kv.code
@@ -581,7 +596,10 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
         raise ValueError(f"the plan is on {plan.prefix.device}, the cache on {dev}" if plan.prefix.device != dev
                          else "a prefix is longer than the tables")
     out = _check_out(out, q)
-    splits = _splits(num_splits, B * Hkv * -(-Hq // Hkv // 16), W * bs - plan.shortest)
+    blocks = -(-Hq // Hkv // 16)
+    shares = _shares(num_splits, B, Hkv * blocks, W * bs - plan.shortest)
+    if plan.items.shape[0] + shares * blocks > 65535:
+        raise ValueError("at most 65535 parts (for each 16 query heads of a kv head)")
     if B == 0:
         return out
     if not _native(kc):
@@ -596,10 +614,10 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
                     out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
             at += n
         return out
-    keep, po, pl = _parts(workspace, B * Hq, D, plan.slots + splits, dev)
+    keep, po, pl = _parts(workspace, (B * plan.slots + shares) * Hq, D, dev) if plan.slots or shares > B else (None, 0, 0)
     kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride(0), kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
                                       block_tables.data_ptr(), block_tables.stride(0), W, seq_lens.data_ptr(), po, pl,
                                       out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale, plan.items.data_ptr(),
                                       plan.items.shape[0], plan.prefix.data_ptr(), plan.counts.data_ptr(), plan.slots,
-                                      plan.row_tiles, splits, stream_ptr())
+                                      plan.row_tiles, shares, stream_ptr())
     return out
