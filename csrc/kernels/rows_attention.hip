@@ -108,9 +108,9 @@ struct RowsCfg {
 };
 
 // Products q k of 32 keys -> scores less their rows' running maxima, which rise (and sums and outputs shrink) where a score is more
-// than RAISE above its row's. kf, vs: the keys' and values' factors. EDGE: some row does not see some key of the 32 from key0 on:
+// than RAISE above its row's. ks, vs: the keys' and values' factors (SCALED: the keys' times softmax's scale). EDGE: some row does not see some key of the 32 from key0 on:
 // its score becomes -inf. A value that is not finite then reaches the rows that see it by their scores, and no other by its factor.
-template <bool EDGE, bool WIDE, int NA, int RT, int MT>
+template <bool EDGE, bool WIDE, bool SCALED, int NA, int RT, int MT>
 __device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[NA], float4 (&vs)[NA], float scale, int key0, int kbeg,
                                        int kend, const int (&limit)[RT], float (&m)[RT], float (&l)[RT], float (&high)[RT],
                                        f32x4_t (&acc)[RT][MT]) {
@@ -121,7 +121,7 @@ __device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[
     const float f[4] = {ks[a].x, ks[a].y, ks[a].z, ks[a].w};
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float k = WIDE ? scale : f[r] * scale;
+      const float k = WIDE ? scale : SCALED ? f[r] : f[r] * scale;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[a][rt][r] = fmaf(s[a][rt][r], k, -m[rt]);
     }
@@ -147,10 +147,13 @@ __device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    top[rt] = fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3]));
+    top[rt] = fmaxf(s[0][rt][0], s[0][rt][1]);
+    top[rt] = fmaxf(fmaxf(top[rt], s[0][rt][2]), s[0][rt][3]);
 #pragma unroll
-    for (int a = 1; a < NA; ++a)
-      top[rt] = fmaxf(top[rt], fmaxf(fmaxf(s[a][rt][0], s[a][rt][1]), fmaxf(s[a][rt][2], s[a][rt][3])));
+    for (int a = 1; a < NA; ++a) {
+      top[rt] = fmaxf(fmaxf(top[rt], s[a][rt][0]), s[a][rt][1]);
+      top[rt] = fmaxf(fmaxf(top[rt], s[a][rt][2]), s[a][rt][3]);
+    }
     raise = raise || top[rt] > high[rt];
   }
   if (__any(raise)) {
@@ -343,7 +346,7 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   };
   // scores of tile t, whose V is in registers
   auto judge = [&](int t, f32x4_t (&s)[2][RT], const float4 (&factors)[2], auto edge) {
-    scores<decltype(edge)::value, C::WIDE, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, w.kend, limit, m, l, high, acc);
+    scores<decltype(edge)::value, C::WIDE, false, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, w.kend, limit, m, l, high, acc);
     if constexpr (decltype(edge)::value) {   // V of keys outside the range: anything (E4M3's NaN too), so zeros
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
@@ -594,7 +597,7 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint2*>(vd + (((wid >> 1) * C::MT + i) * 64 + lane) * 16 + (wid & 1) * 8) = kv_widen4<FMT>(x[i]);
       }
-      if (lane < 32) reinterpret_cast<float*>(kd + 2 * C::SIDE)[g * C::KEYS + wid * 16 + li] = factor;
+      if (lane < 32) reinterpret_cast<float*>(kd + 2 * C::SIDE)[g * C::KEYS + wid * 16 + li] = g ? factor : factor * p.scale;
     }
   };
   if (stages > 0) {
@@ -632,7 +635,7 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
           vs[a] = *reinterpret_cast<const float4*>(sd + C::KEYS + 16 * a);
         }
       }
-      scores<decltype(edge)::value, C::WIDE, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, w.kend, limit, m, l, high, acc);
+      scores<decltype(edge)::value, C::WIDE, true, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, w.kend, limit, m, l, high, acc);
       bf16x8_t pf[2][C::RT];
       weights<C::WIDE, 4, C::RT>(s, vs, l, pf);
 #pragma unroll
@@ -873,7 +876,10 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsA
 template <int FMT, int D, int RT>
 __global__ void __launch_bounds__(256, 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
                                                              const int32_t* counts, int slots, int B, int blocks, int shares) {
-  XGK_ROWS_LDS(FMT, D, RT);
+  constexpr int SPACE = RT == 8 && BlockCfg<FMT, D>::SPACE > RowsCfg<FMT, D, 2>::SPACE ? BlockCfg<FMT, D>::SPACE : RowsCfg<FMT, D, 2>::SPACE;
+  constexpr int LISTS = RT == 8 ? 1 : RT;
+  __shared__ __attribute__((aligned(16))) uint8_t space[SPACE];
+  __shared__ float m_lds[4][16 * LISTS], l_lds[4][16 * LISTS];
   if (blockIdx.y >= n_items) {
     const int at = blockIdx.y - n_items, i = at / blocks;
     decode_share<FMT, D>(p, blockIdx.x, prefix, counts, B, shares, i, at - i * blocks, static_cast<int64_t>(B) * p.Hq * slots, space,
@@ -892,7 +898,8 @@ __global__ void __launch_bounds__(256, 2) rows_shared_kernel(RowsArgs p, const i
   w.part0 = it[5];
   w.part_step = slots;
   w.causal0 = OWN;
-  attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, m_lds, l_lds);
+  if constexpr (RT == 8) attend_block<FMT, D>(p, w, blockIdx.x, space);
+  else attend_rows<FMT, D, RT, false>(p, w, blockIdx.x, space, m_lds, l_lds);
 }
 
 // Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). They are the first counts[token] (null: all) of the
@@ -1056,22 +1063,26 @@ int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
                    width, num_blocks, seq_lens, part_out, part_lse, out, out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs,
                    scale * 1.44269504088896341f, page_magic(bs)};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2) || shares < B || slots < 0 || n_items < 0 ||
+  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8) || shares < B || slots < 0 || n_items < 0 ||
       n_items + static_cast<int64_t>(shares) * blocks > 65535 || (slots > 0 || shares > B) != (part_out != nullptr))
     return -1;
   const dim3 grid(Hkv, n_items + shares * blocks);
-#define XGK_GO(F, DD)                                                                                                          \
-  {                                                                                                                            \
-    if (RT == 1)                                                                                                               \
-      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 1>), grid, dim3(256), 0, st, p, items, n_items, prefix, counts, slots, B,  \
-                         blocks, shares);                                                                                      \
-    else                                                                                                                       \
-      hipLaunchKernelGGL((rows_shared_kernel<F, DD, 2>), grid, dim3(256), 0, st, p, items, n_items, prefix, counts, slots, B,  \
-                         blocks, shares);                                                                                      \
+#define XGK_SHARED(F, DD, R)                                                                                                   \
+  hipLaunchKernelGGL((rows_shared_kernel<F, DD, R>), grid, dim3(256), 0, st, p, items, n_items, prefix, counts, slots, B, blocks, shares)
+#define XGK_GO(F, DD)                           \
+  {                                             \
+    if (RT == 1) XGK_SHARED(F, DD, 1);          \
+    else if (RT == 2) XGK_SHARED(F, DD, 2);     \
+    else return -1;                             \
   }
   XGK_FMT_DIM(XGK_GO)
+  else if (fmt == KV_BF16 && RT == 8) {
+    if (D == 128) XGK_SHARED(KV_BF16, 128, 8);
+    else XGK_SHARED(KV_BF16, 64, 8);
+  }
   else if (fmt == KV_BF16 && D == 128) XGK_GO(KV_BF16, 128) else if (fmt == KV_BF16) XGK_GO(KV_BF16, 64) else return -1;
 #undef XGK_GO
+#undef XGK_SHARED
   if (part_out) join(p, D, B, JoinArgs{counts, slots, prefix, B, shares, nullptr, 0}, st);
   return 0;
 }

@@ -485,14 +485,18 @@ def groups_of(sizes, prefixes, tails, Hkv, D, bs, fmt, dev, gen):
 @DEVICES
 @pytest.mark.parametrize("fmt", ["bf16", "fp8", "int8"])
 @pytest.mark.parametrize("Hq,Hkv,D,bs", [(32, 8, 128, 16), (8, 1, 128, 32), (12, 12, 64, 16), (6, 2, 64, 48), (20, 1, 128, 16)])
-@pytest.mark.parametrize("splits", [None, 1, 5])
-def test_shared_prefix(dev, fmt, Hq, Hkv, D, bs, splits):
+@pytest.mark.parametrize("splits,wide", [(None, False), (1, False), (5, False), (None, True), (3, True)])
+def test_shared_prefix(dev, fmt, Hq, Hkv, D, bs, splits, wide, monkeypatch):
+    if wide:
+        monkeypatch.setattr(kv_quant, "WIDE_ROWS", 0)
+        monkeypatch.setattr(kv_quant, "WIDE_TILES", 0)
     gen = torch.Generator().manual_seed(Hq * 5 + D)
     sizes, prefixes = [3, 1, 5, 17, 2], [100, 0, 33, 64, 400]
     tails = [[5, 1, 40], [70], [1, 2, 3, 4, 100], list(range(1, 18)), [0, 9]]
     cache, table, lens, seqs = groups_of(sizes, prefixes, tails, Hkv, D, bs, fmt, dev, gen)
     q = rows(len(lens), Hq, D, gen, 1.5).to(dev)
     plan = ops.shared_prefix_plan(sizes, prefixes, Hq, Hkv, dev)
+    assert (plan.wide is not None) == wide
     scale = 1 / math.sqrt(D)
     out = ops.shared_prefix_attention(q, cache, table, i32(lens, dev), plan, scale, num_splits=splits)
     for s, L in enumerate(lens):
@@ -513,6 +517,27 @@ def test_shared_prefix_of_sequences_shorter_than_it(dev, fmt):
         check(out[s:s + 1], *attention(q[s:s + 1].double().cpu(), *seqs[s], [L], 0.2))
 
 
+def test_work_of_a_plan():
+    """Every (block of rows, 32 keys) of every group is in one item, in blocks of either size."""
+    sizes, prefixes, G, Hkv = [40, 1, 9, 3], [30000, 0, 9001, 31], 4, 8
+    plan = ops.shared_prefix_plan(sizes, prefixes, G * Hkv, Hkv, "cpu")
+    assert plan.wide is not None and plan.slots == max(plan.work.slots, plan.wide.slots)
+    assert ops.shared_prefix_plan([40], [200], G * Hkv, Hkv, "cpu").wide is None
+    assert ops.shared_prefix_plan([9], [30000], G * Hkv, Hkv, "cpu").wide is None
+    for work in (plan.work, plan.wide):
+        at = 0
+        for n, p in zip(sizes, prefixes):
+            items = [it for it in work.items.tolist() if it[0] == at]
+            blocks = -(-n * G // (16 * work.row_tiles))
+            assert all(it[1] == n for it in items) and {it[2] for it in items} == (set(range(blocks)) if p else set())
+            for b in range(blocks if p else 0):
+                mine = sorted((it[3], it[4], it[5]) for it in items if it[2] == b)
+                assert mine[0][0] == 0 and mine[-1][1] == p and all(x[1] == y[0] and x[1] % 32 == 0 for x, y in zip(mine, mine[1:]))
+                assert [x[2] for x in mine] == list(range(len(mine)))
+                assert work.counts[at:at + n].tolist() == [len(mine)] * n and len(mine) <= work.slots
+            at += n
+
+
 @DEVICES
 def test_nothing_shared_is_decode(dev):
     gen = torch.Generator().manual_seed(22)
@@ -520,7 +545,7 @@ def test_nothing_shared_is_decode(dev):
     cache, table, truth = make(lens, 2, 128, 16, "int8", dev, gen)
     q = rows(4, 8, 128, gen).to(dev)
     plan = ops.shared_prefix_plan([1, 3], [0, 0], 8, 2, dev)
-    assert plan.slots == 0 and plan.items.shape[0] == 0
+    assert plan.slots == 0 and plan.work.items.shape[0] == 0
     a = ops.shared_prefix_attention(q, cache, table, i32(lens, dev), plan, 0.1, num_splits=2)
     b = ops.quant_decode_attention(q, cache, table, i32(lens, dev), 0.1, num_splits=2)
     assert torch.equal(a, b)

@@ -515,20 +515,52 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
 
 # ----------------------------------------------------------------------------------------------------------- shared prefixes
 @dataclass
+class PrefixWork:
+    """What the workgroups of the groups' common keys do."""
+    row_tiles: int               # 16-row tiles of a workgroup
+    slots: int                   # most parts that a prefix is cut into
+    items: torch.Tensor          # [n, 8] int32: first sequence, sequences, block of rows, first key, end key, slot
+    counts: torch.Tensor         # [num_seqs] int32: parts of each sequence's prefix
+
+
+@dataclass
 class SharedPrefixPlan:
     """Which sequences of a decode batch share which prefix, and the launch's work (`shared_prefix_plan`)."""
     num_seqs: int
     num_heads: int
     num_kv_heads: int
-    row_tiles: int               # 16-row tiles of a workgroup of the common part
-    slots: int                   # most parts that a prefix is cut into
-    items: torch.Tensor          # [n, 8] int32: first sequence, sequences, block of rows, first key, end key, slot
+    work: PrefixWork
+    wide: Optional[PrefixWork]   # of bf16 pages, where blocks of 128 rows pay
+    slots: int                   # most parts of either
     prefix: torch.Tensor         # [num_seqs] int32: keys that the common part covers
-    counts: torch.Tensor         # [num_seqs] int32: its parts
     group_sizes: Tuple[int, ...]
     prefix_lens: Tuple[int, ...]
     shortest: int                # prefix
     longest: int
+
+
+# bf16 pages, whose V each wave turns through LDS: blocks of 128 rows share that, from rows that nearly fill one and a share of the
+# work on which their longer start is lost. us with blocks of 32 / 128 rows: 5 groups of 108 rows behind 5 - 30 k keys 156 / 123, 512
+# rows behind 8000 keys 76 / 62, 256 behind 4096 (32 tiles a workgroup) 35 / 38. (8-bit pages, fp8: 81 / 104, 52 / 55.)
+WIDE_ROWS = 96
+WIDE_TILES = 48
+
+
+def _prefix_work(sizes, lens, G: int, Hkv: int, rt: int, each: int, put) -> PrefixWork:
+    """each: 32-key tiles of a workgroup."""
+    items: List[List[int]] = []
+    counts, at = [], 0
+    for n, p in zip(sizes, lens):
+        blocks, tiles = -(-n * G // (16 * rt)), -(-p // 32)
+        parts = min(MAX_SPLITS, -(-tiles // each))
+        share = -(-tiles // parts) * 32 if parts else 0
+        parts = -(-p // share) if parts else 0
+        # (the blocks of one range of keys side by side: they read the same bytes)
+        items += [[at, n, i, j * share, min(p, (j + 1) * share), j, 0, 0] for j in range(parts) for i in range(blocks)]
+        counts += [parts] * n
+        at += n
+    _need(len(items) <= 65535, "too many groups")
+    return PrefixWork(rt, max(counts, default=0), put(items, (8,)), put(counts, ()))
 
 
 def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], num_heads: int, num_kv_heads: int,
@@ -541,29 +573,21 @@ def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], n
     _need(all(n >= 1 for n in sizes) and all(0 <= n < 1 << 30 for n in lens), "groups of at least one sequence, lengths of at least 0")
     _need(num_kv_heads >= 1 and num_heads >= 1 and num_heads % num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
     G = num_heads // num_kv_heads
-    rt = 2 if max([n * G for n, p in zip(sizes, lens) if p > 0], default=0) > 16 else 1
-    blocks = [-(-n * G // (16 * rt)) for n in sizes]
-    tiles = [-(-p // 32) for p in lens]
-    total = sum(b * t for b, t in zip(blocks, tiles)) * num_kv_heads
-    each = max(4, -(-total // PREFIX_WGS))      # 32-key tiles of a workgroup
-    items: List[List[int]] = []
-    prefix, counts, at = [], [], 0
-    for n, p, b, t in zip(sizes, lens, blocks, tiles):
-        parts = min(MAX_SPLITS, -(-t // each))
-        share = -(-t // parts) * 32 if parts else 0
-        parts = -(-p // share) if parts else 0
-        # (the blocks of one range of keys side by side: they read the same bytes)
-        items += [[at, n, i, j * share, min(p, (j + 1) * share), j, 0, 0] for j in range(parts) for i in range(b)]
-        prefix += [p] * n
-        counts += [parts] * n
-        at += n
-    _need(len(items) <= 65535, "too many groups")
 
     def put(rows, width):
         return torch.tensor(rows, dtype=torch.int32).reshape(-1, *width).to(device)
 
-    return SharedPrefixPlan(at, num_heads, num_kv_heads, rt, max(counts, default=0), put(items, (8,)), put(prefix, ()), put(counts, ()),
-                            tuple(sizes), tuple(lens), min(lens, default=0), max(lens, default=0))
+    def tiles(rt):   # of a workgroup, where PREFIX_WGS have them all
+        total = sum(-(-n * G // (16 * rt)) * -(-p // 32) for n, p in zip(sizes, lens)) * num_kv_heads
+        return max(4, -(-total // PREFIX_WGS))
+
+    most = max([n * G for n, p in zip(sizes, lens) if p > 0], default=0)
+    rt = 1 if most <= 16 else 2
+    work = _prefix_work(sizes, lens, G, num_kv_heads, rt, tiles(rt), put)
+    wide = _prefix_work(sizes, lens, G, num_kv_heads, 8, tiles(8), put) if most >= WIDE_ROWS and tiles(rt) >= WIDE_TILES else None
+    prefix = [p for n, p in zip(sizes, lens) for _ in range(n)]
+    return SharedPrefixPlan(len(prefix), num_heads, num_kv_heads, work, wide, max(work.slots, wide.slots if wide else 0),
+                            put(prefix, ()), tuple(sizes), tuple(lens), min(lens, default=0), max(lens, default=0))
 
 
 def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch.Tensor, torch.Tensor]], block_tables: torch.Tensor,
@@ -598,7 +622,8 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
     out = _check_out(out, q)
     blocks = -(-Hq // Hkv // 16)
     shares = _shares(num_splits, B, Hkv * blocks, W * bs - plan.shortest)
-    if plan.items.shape[0] + shares * blocks > 65535:
+    work = plan.work if quant or plan.wide is None else plan.wide
+    if work.items.shape[0] + shares * blocks > 65535:
         raise ValueError("at most 65535 parts (for each 16 query heads of a kv head)")
     if B == 0:
         return out
@@ -614,10 +639,10 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
                     out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
             at += n
         return out
-    keep, po, pl = _parts(workspace, (B * plan.slots + shares) * Hq, D, dev) if plan.slots or shares > B else (None, 0, 0)
+    keep, po, pl = _parts(workspace, (B * work.slots + shares) * Hq, D, dev) if work.slots or shares > B else (None, 0, 0)
     kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride(0), kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
                                       block_tables.data_ptr(), block_tables.stride(0), W, seq_lens.data_ptr(), po, pl,
-                                      out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale, plan.items.data_ptr(),
-                                      plan.items.shape[0], plan.prefix.data_ptr(), plan.counts.data_ptr(), plan.slots,
-                                      plan.row_tiles, shares, stream_ptr())
+                                      out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale, work.items.data_ptr(),
+                                      work.items.shape[0], plan.prefix.data_ptr(), work.counts.data_ptr(), work.slots,
+                                      work.row_tiles, shares, stream_ptr())
     return out
