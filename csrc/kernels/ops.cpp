@@ -70,13 +70,13 @@ int kv_read(int, const uint8_t*, const uint8_t*, const float*, const int32_t*, i
             int, int, int, int, int, uint16_t*, uint16_t*, hipStream_t);
 int quant_decode_attention(int, const uint16_t*, int64_t, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t,
                            int, const int32_t*, float*, float*, uint16_t*, int64_t, int, int, int, int, int, int, float, int,
-                           hipStream_t);
+                           int, hipStream_t);
 int quant_prefill_attention(int, const uint16_t*, int64_t, const uint8_t*, const uint8_t*, const float*, const int32_t*, int64_t,
                             int, const int32_t*, const int32_t*, float*, float*, uint16_t*, int64_t, int, int, int, int, int,
                             int, int, int, float, int, int, hipStream_t);
 int shared_prefix_attention(int, const uint16_t*, int64_t, const void*, const void*, const float*, const int32_t*, int64_t, int,
                             const int32_t*, float*, float*, uint16_t*, int64_t, int, int, int, int, int, int, float,
-                            const int32_t*, int, const int32_t*, const int32_t*, int, int, int, hipStream_t);
+                            const int32_t*, int, const int32_t*, const int32_t*, int, int, int, int, hipStream_t);
 void argmax_logprob(const void*, int, int64_t, int, int, int32_t*, float*, hipStream_t, float* ws = nullptr,
                     int* cnt = nullptr);
 int argmax_ws_floats_per_row();
@@ -245,10 +245,11 @@ PYBIND11_MODULE(_kernels, m) {
   });
   m.def("quant_decode_attention", [](int fmt, uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt,
                                      int64_t bts, int W, uintptr_t sl, uintptr_t po, uintptr_t pl, uintptr_t out, int64_t os, int B,
-                                     int Hq, int Hkv, int D, int bs, int blocks, float scale, int splits, uintptr_t st) {
+                                     int Hq, int Hkv, int D, int bs, int blocks, float scale, int shares, int least,
+                                     uintptr_t st) {
     check(xgk::quant_decode_attention(fmt, P<const uint16_t>(q), qs, P<const uint8_t>(kc), P<const uint8_t>(vc),
                                       P<const float>(scales), P<const int32_t>(bt), bts, W, P<const int32_t>(sl), P<float>(po),
-                                      P<float>(pl), P<uint16_t>(out), os, B, Hq, Hkv, D, bs, blocks, scale, splits, S(st)),
+                                      P<float>(pl), P<uint16_t>(out), os, B, Hq, Hkv, D, bs, blocks, scale, shares, least, S(st)),
           "quant_decode_attention");
   });
   m.def("quant_prefill_attention", [](int fmt, uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt,
@@ -264,11 +265,11 @@ PYBIND11_MODULE(_kernels, m) {
   m.def("shared_prefix_attention", [](int fmt, uintptr_t q, int64_t qs, uintptr_t kc, uintptr_t vc, uintptr_t scales, uintptr_t bt,
                                       int64_t bts, int W, uintptr_t sl, uintptr_t po, uintptr_t pl, uintptr_t out, int64_t os,
                                       int B, int Hq, int Hkv, int D, int bs, int blocks, float scale, uintptr_t items, int n_items,
-                                      uintptr_t prefix, uintptr_t counts, int slots, int rt, int splits, uintptr_t st) {
+                                      uintptr_t prefix, uintptr_t counts, int slots, int rt, int shares, int least, uintptr_t st) {
     check(xgk::shared_prefix_attention(fmt, P<const uint16_t>(q), qs, P<const void>(kc), P<const void>(vc), P<const float>(scales),
                                        P<const int32_t>(bt), bts, W, P<const int32_t>(sl), P<float>(po), P<float>(pl),
                                        P<uint16_t>(out), os, B, Hq, Hkv, D, bs, blocks, scale, P<const int32_t>(items), n_items,
-                                       P<const int32_t>(prefix), P<const int32_t>(counts), slots, rt, splits, S(st)),
+                                       P<const int32_t>(prefix), P<const int32_t>(counts), slots, rt, shares, least, S(st)),
           "shared_prefix_attention");
   });
   m.def("argmax_logprob", [](uintptr_t logits, int is_f32, int64_t stride, int B, int V, uintptr_t tok, uintptr_t lp,

@@ -42,6 +42,7 @@ struct RowsArgs {
   int Hq, Hkv, G, bs;
   float scale;            // softmax's, in base 2
   uint32_t page_magic;    // page_of
+  int least;              // decode: units of 128 keys that a share has where there are that many
 };
 
 // tables are not written while a kernel reads them: scalar loads
@@ -751,9 +752,21 @@ __device__ __forceinline__ void cut_share(const RowsArgs& p, const int32_t* star
     for (int a = 0; a < AT_ONCE; ++a)
       u[a] = b0 + 64 * a + lane < B && kend[a] > kbeg[a] ? (((kend[a] + 31) >> 5) - (kbeg[a] >> 5) + 3) >> 2 : 0;
   };
-  int all = 0, most = 0;
+  bool cut = false;
   for (int b0 = 0; b0 < B; b0 += 64 * AT_ONCE) {
     units(b0);
+#pragma unroll
+    for (int a = 0; a < AT_ONCE; ++a) cut = cut || __any(u[a] > p.least);
+  }
+  if (!cut) {   // one part each
+    const int b = of >= 0 ? of : i;
+    s.b = b < B ? b : -1;
+    s.first = b;
+    return;
+  }
+  int all = 0, most = 0;
+  for (int b0 = 0; b0 < B; b0 += 64 * AT_ONCE) {
+    if (B > 64 * AT_ONCE) units(b0);
     int sum = 0;
 #pragma unroll
     for (int a = 0; a < AT_ONCE; ++a) {
@@ -763,7 +776,7 @@ __device__ __forceinline__ void cut_share(const RowsArgs& p, const int32_t* star
     all += __builtin_amdgcn_readlane(wave_scan(sum), 63);
   }
   most = __float_as_int(wave_join(__int_as_float(most), [](float x, float y) { return __int_as_float(max(__float_as_int(x), __float_as_int(y))); }));
-  run = __builtin_amdgcn_readfirstlane(max(max(1, (all + shares - B - 1) / (shares - B)), (most + MAX_PARTS - 1) / MAX_PARTS));
+  run = __builtin_amdgcn_readfirstlane(max(max(p.least, (all + shares - B - 1) / (shares - B)), (most + MAX_PARTS - 1) / MAX_PARTS));
   int before = 0;
   for (int b0 = 0; b0 < B && s.b < 0; b0 += 64 * AT_ONCE) {
     if (B > 64 * AT_ONCE) units(b0);
@@ -1009,12 +1022,12 @@ static void join(const RowsArgs& p, int D, int tokens, const JoinArgs& j, hipStr
 int quant_decode_attention(int fmt, const uint16_t* q, int64_t q_stride, const uint8_t* k, const uint8_t* v, const float* scales,
                            const int32_t* tables, int64_t table_stride, int width, const int32_t* seq_lens, float* part_out,
                            float* part_lse, uint16_t* out, int64_t out_stride, int B, int Hq, int Hkv, int D, int bs,
-                           int num_blocks, float scale, int shares, hipStream_t st) {
+                           int num_blocks, float scale, int shares, int least, hipStream_t st) {
   if (B <= 0) return 0;
   const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
-                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, page_magic(bs)};
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, page_magic(bs), least};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || shares < B || static_cast<int64_t>(shares) * blocks > 65535 || (shares > B) != (part_out != nullptr)) return -1;
+  if (!rows_ok(p, D) || least < 1 || shares < B || static_cast<int64_t>(shares) * blocks > 65535 || (shares > B) != (part_out != nullptr)) return -1;
 #define XGK_GO(F, DD)                                                                                                        \
   {                                                                                                                          \
     hipLaunchKernelGGL((rows_decode_kernel<F, DD>), dim3(Hkv, shares * blocks), dim3(256), 0, st, p, B, blocks, shares);     \
@@ -1033,7 +1046,7 @@ int quant_prefill_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
                             int Hq, int Hkv, int D, int bs, int num_blocks, float scale, int RT, int splits, hipStream_t st) {
   if (tokens <= 0 || S <= 0 || max_q <= 0) return 0;
   const RowsArgs p{q, q_stride, k, v, scales, tables, table_stride, width, num_blocks, seq_lens, part_out, part_lse, out,
-                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, page_magic(bs)};
+                   out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs, scale * 1.44269504088896341f, page_magic(bs), 1};
   if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8) || splits < 1 || (splits > 1) != (part_out != nullptr)) return -1;
   const int64_t blocks = (static_cast<int64_t>(max_q) * p.G + 16 * RT - 1) / (16 * RT);
   if (blocks > 65535 || static_cast<int64_t>(S) * splits > 65535) return -1;
@@ -1057,13 +1070,13 @@ int shared_prefix_attention(int fmt, const uint16_t* q, int64_t q_stride, const 
                             const int32_t* tables, int64_t table_stride, int width, const int32_t* seq_lens, float* part_out,
                             float* part_lse, uint16_t* out, int64_t out_stride, int B, int Hq, int Hkv, int D, int bs,
                             int num_blocks, float scale, const int32_t* items, int n_items, const int32_t* prefix,
-                            const int32_t* counts, int slots, int RT, int shares, hipStream_t st) {
+                            const int32_t* counts, int slots, int RT, int shares, int least, hipStream_t st) {
   if (B <= 0) return 0;
   const RowsArgs p{q, q_stride, static_cast<const uint8_t*>(k), static_cast<const uint8_t*>(v), scales, tables, table_stride,
                    width, num_blocks, seq_lens, part_out, part_lse, out, out_stride, Hq, Hkv, Hkv > 0 ? Hq / Hkv : 0, bs,
-                   scale * 1.44269504088896341f, page_magic(bs)};
+                   scale * 1.44269504088896341f, page_magic(bs), least};
   const int blocks = (p.G + 15) / 16;
-  if (!rows_ok(p, D) || (RT != 1 && RT != 2 && RT != 8) || shares < B || slots < 0 || n_items < 0 ||
+  if (!rows_ok(p, D) || least < 1 || (RT != 1 && RT != 2 && RT != 8) || shares < B || slots < 0 || n_items < 0 ||
       n_items + static_cast<int64_t>(shares) * blocks > 65535 || (slots > 0 || shares > B) != (part_out != nullptr))
     return -1;
   const dim3 grid(Hkv, n_items + shares * blocks);

@@ -33,7 +33,8 @@ MAX_SPLITS = 64
 # us of decode, one part / the parts that this makes: 1 sequence of 640 keys 6.0 / 6.5, 1280 8.5 / 6.9, 5120 35.7 / 8.9; 16 of 640
 # 8.5 / 9.4, 5120 48.8 / 30.5; 48 of 1280 25.2 / 25.4 (8 kv heads of 128). Below SPLIT_FROM keys a second launch costs more
 SPLIT_WGS = 512     # workgroups that fill the chip: two a CU
-SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
+SPLIT_KEYS = 128
+WHOLE_UNITS = 16   # a workgroup's four waves have a 32-key tile each
 SPLIT_FROM = 1024
 # the common parts of shared prefixes: one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences behind
 # 4096 keys: 256 workgroups 26.9 us, 512 32.6, 1024 40.6)
@@ -398,7 +399,7 @@ def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
     return int(num_splits)
 
 
-def _shares(num_splits: Optional[int], B: int, wgs: int, max_keys: int) -> int:
+def _shares(num_splits: Optional[int], B: int, wgs: int, max_keys: int) -> Tuple[int, int]:
     """Shares of a batch's keys, which the kernel gives out by the sequences' lengths: B for one part each. wgs: workgroups a share.
     Where the sequences alone fill most of the chip, only those longer than the mean are cut, and none where none can be long: us
     whole and with that, 200 of 1500 keys on 8 kv heads 109 / 115, 128 of 64 - 2000 54 / 58, 64 of 5000 102 / 105, 1 of 60 k beside
@@ -406,10 +407,10 @@ def _shares(num_splits: Optional[int], B: int, wgs: int, max_keys: int) -> int:
     if num_splits is None:
         full = 8 * B * wgs >= 3 * SPLIT_WGS
         if max_keys < SPLIT_FROM * (4 if full else 1):
-            return B
+            return B, 1
         more = min(-(-SPLIT_WGS // wgs), B * -(-max_keys // SPLIT_KEYS))
-        return B + (min(more, B) if full else more)
-    return B * _splits(num_splits, 1, 0)
+        return (B + min(more, B), WHOLE_UNITS) if full else (B + more, 1)
+    return B * _splits(num_splits, 1, 0), 1
 
 
 def _parts(workspace: Optional[DecodeWorkspace], parts: int, D: int, device):
@@ -436,7 +437,7 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     out = _check_out(out, q)
     W = block_tables.shape[1]
     blocks = -(-Hq // Hkv // 16)
-    shares = _shares(num_splits, B, Hkv * blocks, W * bs)
+    shares, least = _shares(num_splits, B, Hkv * blocks, W * bs)
     if B == 0:
         return out
     if shares * blocks > 65535:
@@ -453,7 +454,7 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
                                      seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale,
-                                     shares, stream_ptr())
+                                     shares, least, stream_ptr())
     return out
 
 
@@ -621,7 +622,7 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
                          else "a prefix is longer than the tables")
     out = _check_out(out, q)
     blocks = -(-Hq // Hkv // 16)
-    shares = _shares(num_splits, B, Hkv * blocks, W * bs - plan.shortest)
+    shares, least = _shares(num_splits, B, Hkv * blocks, W * bs - plan.shortest)
     work = plan.work if quant or plan.wide is None else plan.wide
     if work.items.shape[0] + shares * blocks > 65535:
         raise ValueError("at most 65535 parts (for each 16 query heads of a kv head)")
@@ -644,5 +645,5 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
                                       block_tables.data_ptr(), block_tables.stride(0), W, seq_lens.data_ptr(), po, pl,
                                       out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale, work.items.data_ptr(),
                                       work.items.shape[0], plan.prefix.data_ptr(), work.counts.data_ptr(), work.slots,
-                                      work.row_tiles, shares, stream_ptr())
+                                      work.row_tiles, shares, least, stream_ptr())
     return out
