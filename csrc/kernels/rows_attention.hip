@@ -706,7 +706,8 @@ __device__ __forceinline__ void share(int& kbeg, int& kend, int split, int split
 // ---- decode: shares of the batch's keys -------------------------------------------------------------------------------------
 // A batch's sequences are of any lengths, which the host does not know, so the keys are shared out here: of `shares` workgroups a kv
 // head (and block of 16 query heads) each takes up to `run` units of 128 keys (a 32-key tile a wave) of one sequence, with run the
-// batch's units over shares - B. So a sequence has ceil(units / run) parts, at least one, and all have shares at most. (With as many
+// batch's units over shares - B, and `least` where none has more: a short search, for share i is sequence i then (256 sequences of
+// 300 - 900 keys 71 -> 68 us). So a sequence has ceil(units / run) parts, at least one, and all have shares at most. (With as many
 // parts for each sequence the longest one bounds the step: 1 sequence of 60 k keys beside 63 of 500, fp8, took 423 us, and takes 42.)
 constexpr int MAX_PARTS = 128;
 

@@ -33,8 +33,8 @@ MAX_SPLITS = 64
 # us of decode, one part / the parts that this makes: 1 sequence of 640 keys 6.0 / 6.5, 1280 8.5 / 6.9, 5120 35.7 / 8.9; 16 of 640
 # 8.5 / 9.4, 5120 48.8 / 30.5; 48 of 1280 25.2 / 25.4 (8 kv heads of 128). Below SPLIT_FROM keys a second launch costs more
 SPLIT_WGS = 512     # workgroups that fill the chip: two a CU
-SPLIT_KEYS = 128
-WHOLE_UNITS = 16   # a workgroup's four waves have a 32-key tile each
+SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
+WHOLE_UNITS = 16    # units of SPLIT_KEYS that stay whole where the sequences alone fill most of the chip
 SPLIT_FROM = 1024
 # the common parts of shared prefixes: one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences behind
 # 4096 keys: 256 workgroups 26.9 us, 512 32.6, 1024 40.6)
@@ -401,9 +401,9 @@ def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
 
 def _shares(num_splits: Optional[int], B: int, wgs: int, max_keys: int) -> Tuple[int, int]:
     """Shares of a batch's keys, which the kernel gives out by the sequences' lengths: B for one part each. wgs: workgroups a share.
-    Where the sequences alone fill most of the chip, only those longer than the mean are cut, and none where none can be long: us
-    whole and with that, 200 of 1500 keys on 8 kv heads 109 / 115, 128 of 64 - 2000 54 / 58, 64 of 5000 102 / 105, 1 of 60 k beside
-    63 of 500 424 / 40."""
+    And the units that a share has at least. Where the sequences alone fill most of the chip, only those longer than the mean and
+    than WHOLE_UNITS are cut, and none where none can be long: us whole and with that, 200 of 1500 keys on 8 kv heads 116 / 117, 128
+    of 64 - 2000 54 / 57, 64 of 500 - 8000 115 / 111, 1 of 60 k beside 63 of 500 424 / 27."""
     if num_splits is None:
         full = 8 * B * wgs >= 3 * SPLIT_WGS
         if max_keys < SPLIT_FROM * (4 if full else 1):
