@@ -109,8 +109,9 @@ struct RowsCfg {
 };
 
 // Products q k of 32 keys -> scores less their rows' running maxima, which rise (and sums and outputs shrink) where a score is more
-// than RAISE above its row's. ks, vs: the keys' and values' factors (SCALED: the keys' times softmax's scale). EDGE: some row does not see some key of the 32 from key0 on:
-// its score becomes -inf. A value that is not finite then reaches the rows that see it by their scores, and no other by its factor.
+// than RAISE above its row's. ks, vs: the keys' and values' factors (SCALED: the keys' times softmax's scale). EDGE: some row does not
+// see some key of the 32 from key0 on: its score becomes -inf. A value that is not finite then reaches the rows that see it by their
+// scores, and no other by its factor (bf16: add_odd).
 template <bool EDGE, bool WIDE, bool SCALED, int NA, int RT, int MT>
 __device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[NA], float4 (&vs)[NA], float scale, int key0, int kbeg,
                                        int kend, const int (&limit)[RT], float (&m)[RT], float (&l)[RT], float (&high)[RT],
@@ -202,6 +203,54 @@ __device__ __forceinline__ void weights(f32x4_t (&s)[NA][RT], const float4 (&vs)
         o[2 * x + 1] = pack2(e[2], e[3]);
       }
       pf[pair][rt] = as_frag(make_uint4(o[0], o[1], o[2], o[3]));
+    }
+  }
+}
+
+// bf16 pages, tiles at the edges: a value that is infinite or NaN would reach rows that do not see it, as 0 times it. Its row of V is
+// zeros in the products, and is added to the rows that see it by itself.
+
+// One load of rows of V, D / 8 lanes each, of which the caller's lanes `in` count: bits of its rows that are odd in this way, now zeros
+template <int D>
+__device__ __forceinline__ uint32_t odd_rows(uint4& x, bool in) {
+  constexpr int LANES = D / 8;
+  auto odd = [](uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; };
+  const uint64_t who = __ballot(in && (odd(x.x) || odd(x.y) || odd(x.z) || odd(x.w)));
+  uint32_t rows = 0;
+  if (who) {
+#pragma unroll
+    for (int i = 0; i < 64 / LANES; ++i) rows |= (who >> (i * LANES) & ((1ull << LANES) - 1)) ? 1u << i : 0u;
+    if (rows >> ((threadIdx.x & 63) / LANES) & 1) x = make_uint4(0, 0, 0, 0);
+  }
+  return rows;
+}
+
+// odd: such keys of the 16 NA from key0 on, s: scores, row_of: a key's row of V
+template <int NA, int RT, int MT, typename F>
+__device__ __forceinline__ void add_odd(uint64_t odd, const f32x4_t (&s)[NA][RT], int key0, const int (&limit)[RT], F row_of,
+                                        f32x4_t (&acc)[RT][MT]) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+#pragma unroll 1
+  for (; odd; odd &= odd - 1) {
+    const int x = __builtin_ctzll(odd);
+    const uint16_t* v = row_of(key0 + x);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float score = 0.f;
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) score = x >> 4 == a && (x & 3) == r ? s[a][rt][r] : score;
+      const float w = exp2_fast(__shfl(score, (x & 12) * 4 + li, 64));
+      const bool seen = key0 + x < limit[rt];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const uint2 y = *reinterpret_cast<const uint2*>(v + 16 * mt + 4 * g);
+        const float f[4] = {bf2f(y.x & 0xFFFF), bf2f(y.x >> 16), bf2f(y.y & 0xFFFF), bf2f(y.y >> 16)};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[rt][mt][r] += seen ? w * f[r] : 0.f;
+        __builtin_amdgcn_sched_barrier(0);   // (a load in flight, not all: registers)
+      }
     }
   }
 }
@@ -324,6 +373,15 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   if (w.causal0 != ALL)
     for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
   least = __builtin_amdgcn_readfirstlane(least);
+  // no row sees the keys from here on, which may never have been written
+  int end = w.kend;
+  if (w.causal0 == OWN) {
+    int most = limit[0];
+#pragma unroll
+    for (int rt = 1; rt < RT; ++rt) most = max(most, limit[rt]);
+    for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o, 64));
+    end = __builtin_amdgcn_readfirstlane(most);
+  }
   const int whole = max(0, min(n, ((least >> 5) - t0 + 3) >> 2) - ahead);      // tiles that every row sees
   // S^T of the tile whose K is in registers
   auto product = [&](f32x4_t (&s)[2][RT]) {
@@ -345,9 +403,15 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
       }
     }
   };
-  // scores of tile t, whose V is in registers
+  auto row_of = [&](int key) {   // of V
+    const int pg = page_of(key >> 4, p.page_magic);
+    return reinterpret_cast<const uint16_t*>(v_head + static_cast<uint64_t>(min(max(table[pg], 0), p.num_blocks - 1)) * page_bytes) +
+           (key - pg * p.bs) * D;
+  };
+  // scores of tile t, whose V is in registers; bf16: its odd rows
   auto judge = [&](int t, f32x4_t (&s)[2][RT], const float4 (&factors)[2], auto edge) {
-    scores<decltype(edge)::value, C::WIDE, false, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, w.kend, limit, m, l, high, acc);
+    uint32_t odd = 0;
+    scores<decltype(edge)::value, C::WIDE, false, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, end, limit, m, l, high, acc);
     if constexpr (decltype(edge)::value) {   // V of keys outside the range: anything (E4M3's NaN too), so zeros
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
@@ -355,20 +419,23 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
 #pragma unroll
           for (int i = 0; i < C::LOADS; ++i) {
             const int key = 32 * t + 16 * a + (lane + 64 * i) / (D / 8);
-            if (key < w.kbeg || key >= w.kend) vr[a][i] = make_uint4(0, 0, 0, 0);
+            const bool in = key >= w.kbeg && key < end;
+            if (!in) vr[a][i] = make_uint4(0, 0, 0, 0);
+            if constexpr (!ONCE) odd |= odd_rows<D>(vr[a][i], in) << (16 * a + 64 / (D / 8) * i);   // (once: all rows see the same keys)
           }
         } else {
           uint32_t keep = 0;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int key = 32 * t + 16 * a + 4 * g + r;
-            keep |= key >= w.kbeg && key < w.kend ? 0xFFu << (8 * r) : 0u;
+            keep |= key >= w.kbeg && key < end ? 0xFFu << (8 * r) : 0u;
           }
 #pragma unroll
           for (int i = 0; i < C::LOADS; ++i) vr[a][i] = make_uint4(vr[a][i].x & keep, vr[a][i].y & keep, vr[a][i].z & keep, vr[a][i].w & keep);
         }
       }
     }
+    return odd;
   };
   auto step = [&](int j, auto edge) {
     f32x4_t s[2][RT];
@@ -376,9 +443,12 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
     const float4 factors[2] = {ks[0], ks[1]};
     settle();
     load_k();
-    judge(nth(j), s, factors, edge);
+    const uint32_t odd = judge(nth(j), s, factors, edge);
     bf16x8_t pf[1][RT];
     weights<C::WIDE, 2, RT>(s, vs, l, pf);
+    if constexpr (C::WIDE && !ONCE && decltype(edge)::value) {
+      if (odd) add_odd(odd, s, 32 * nth(j), limit, row_of, acc);
+    }
     uint16_t* turn = reinterpret_cast<uint16_t*>(space) + wid * 32 * D;
     if constexpr (C::WIDE) {
 #pragma unroll
@@ -494,9 +564,13 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
   }
   most = __builtin_amdgcn_readfirstlane(most);   // no row of the wave sees the keys from here on
   int* of_waves = reinterpret_cast<int*>(space);
-  if (lane == 0) of_waves[wid] = least;
+  if (lane == 0) {
+    of_waves[wid] = least;
+    of_waves[4 + wid] = most;
+  }
   __syncthreads();
   least = __builtin_amdgcn_readfirstlane(min(min(of_waves[0], of_waves[1]), min(of_waves[2], of_waves[3])));
+  const int kend = __builtin_amdgcn_readfirstlane(max(max(of_waves[4], of_waves[5]), max(of_waves[6], of_waves[7])));   // and none of these
   __syncthreads();
 
   float m[C::RT], l[C::RT], high[C::RT];
@@ -509,8 +583,8 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
     for (int mt = 0; mt < C::MT; ++mt) acc[rt][mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int tpp = p.bs >> 4, last = max((w.kend + 15) / 16 - 1, 0);
-  const int stages = w.kend > w.kbeg ? (w.kend - w.kbeg + C::KEYS - 1) / C::KEYS : 0;
+  const int tpp = p.bs >> 4, last = max((kend + 15) / 16 - 1, 0);
+  const int stages = kend > w.kbeg ? (kend - w.kbeg + C::KEYS - 1) / C::KEYS : 0;
   const Constant<int32_t> table = constant(p.tables + w.table * p.table_stride);
   const uint32_t elem = C::WIDE ? 2 : 1;
   const uint32_t page_bytes = static_cast<uint32_t>(p.Hkv) * p.bs * D * elem, page_scales = static_cast<uint32_t>(p.Hkv) * 2 * p.bs;
@@ -557,20 +631,31 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
       factor = sc[static_cast<uint32_t>((g & 1) * p.bs + li)];
     }
   };
-  auto kept = [&](int key) { return key >= w.kbeg && key < w.kend; };
+  auto row_of = [&](int key) {   // of V
+    const int pg = page_of(key >> 4, p.page_magic);
+    return reinterpret_cast<const uint16_t*>(v_head + static_cast<uint64_t>(min(max(table[pg], 0), p.num_blocks - 1)) * page_bytes) +
+           (key - pg * p.bs) * D;
+  };
+  auto kept = [&](int key) { return key >= w.kbeg && key < kend; };
   auto lay = [&](int stage, auto edge) {
     uint8_t* kd = space + (stage & 1) * C::STAGE;
     uint8_t* vd = kd + C::SIDE;
     const int key0 = w.kbeg + stage * C::KEYS;
     if constexpr (C::WIDE) {
+      uint32_t odd = 0;
 #pragma unroll
       for (int i = 0; i < C::RAW; ++i) {
         st16(kd + ((wid * C::KK + i) * 64 + lane) * 16, kraw[i]);
         const int row = 16 * wid + (lane + 64 * i) / (D / 8), ch = (lane + 64 * i) % (D / 8);
         uint4 x = vraw[i];
-        if (decltype(edge)::value && !kept(key0 + row)) x = make_uint4(0, 0, 0, 0);
+        if constexpr (decltype(edge)::value) {
+          const bool in = kept(key0 + row);
+          if (!in) x = make_uint4(0, 0, 0, 0);
+          odd |= odd_rows<D>(x, in) << (64 / (D / 8) * i);
+        }
         st16(vd + (row * (D / 8) + (ch ^ (((row & 7) << 1) & (D / 8 - 1)))) * 16, x);
       }
+      if (lane == 0) reinterpret_cast<uint16_t*>(kd + 2 * C::SIDE)[wid] = odd;
     } else {
 #pragma unroll
       for (int i = 0; i < C::RAW; ++i) {
@@ -636,9 +721,14 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
           vs[a] = *reinterpret_cast<const float4*>(sd + C::KEYS + 16 * a);
         }
       }
-      scores<decltype(edge)::value, C::WIDE, true, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, w.kend, limit, m, l, high, acc);
+      scores<decltype(edge)::value, C::WIDE, true, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, kend, limit, m, l, high, acc);
       bf16x8_t pf[2][C::RT];
       weights<C::WIDE, 4, C::RT>(s, vs, l, pf);
+      if constexpr (C::WIDE && decltype(edge)::value) {
+        const uint2 o = *reinterpret_cast<const uint2*>(kd + 2 * C::SIDE);
+        const uint64_t odd = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(o.y)) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(o.x));
+        if (odd) add_odd(odd, s, key0, limit, row_of, acc);
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -659,8 +749,9 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
     }
     __syncthreads();
   };
-  // stages that every row sees (and whose next one ends within the range), then the others: two loops, as above
-  const int whole = max(0, min(min((least - w.kbeg) / C::KEYS, stages), (w.kend - w.kbeg) / C::KEYS - 1));
+  // stages that every row sees (and whose next one, laid down meanwhile, ends within the range, and of bf16 is seen by every row too),
+  // then the others: two loops, as above
+  const int whole = max(0, min(min((least - w.kbeg) / C::KEYS - (C::WIDE ? 1 : 0), stages), (kend - w.kbeg) / C::KEYS - 1));
 #pragma unroll 1
   for (int stage = 0; stage < whole; ++stage) step(stage, std::false_type{});
 #pragma unroll 1
@@ -888,7 +979,7 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsA
 // others by HBM, and run beside each other. Grid (Hkv, n_items + shares heads' blocks of 16). Parts: slots a row of the common
 // ones, then the shares'.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256, 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
+__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
                                                              const int32_t* counts, int slots, int B, int blocks, int shares) {
   constexpr int SPACE = RT == 8 && BlockCfg<FMT, D>::SPACE > RowsCfg<FMT, D, 2>::SPACE ? BlockCfg<FMT, D>::SPACE : RowsCfg<FMT, D, 2>::SPACE;
   constexpr int LISTS = RT == 8 ? 1 : RT;
@@ -1001,7 +1092,8 @@ __global__ void __launch_bounds__(256) rows_join_kernel(RowsArgs p, JoinArgs j) 
 static bool rows_ok(const RowsArgs& p, int D) {
   return p.bs > 0 && p.bs % KV_TILE == 0 && p.Hkv >= 1 && p.Hq % p.Hkv == 0 && (D == 64 || D == 128) && p.width >= 1 &&
          p.num_blocks >= 1 && !p.part_out == !p.part_lse && p.q_stride % 8 == 0 &&
-         p.out_stride % 4 == 0 && static_cast<int64_t>(p.width) * (p.bs / KV_TILE) * (p.bs / KV_TILE) < 1 << 30;
+         p.out_stride % 4 == 0 && static_cast<int64_t>(p.width) * (p.bs / KV_TILE) * (p.bs / KV_TILE) < 1 << 30 &&
+         static_cast<int64_t>(p.width) * p.bs < 1ll << 31 && static_cast<int64_t>(p.Hkv) * p.bs * D < 1ll << 31;
 }
 static uint32_t page_magic(int bs) { return bs >= KV_TILE ? (1u << 31) / (bs / KV_TILE) + 1 : 1; }
 
