@@ -106,6 +106,9 @@ def test_generation_and_prefix_pages(fmt):
         other.import_prefix(back)
     with pytest.raises(ValueError, match="KV dtype"):
         _engine(None).import_prefix(back)
+    back.kv = back.kv.float()
+    with pytest.raises(ValueError, match="uint8"):
+        b.import_prefix(back)
     with pytest.raises(CacheDeserialization):
         deserialize(serialize(entry)[:-1])
 

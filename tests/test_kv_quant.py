@@ -467,11 +467,11 @@ def test_prompts(dev, fmt, Hq, Hkv, D, bs, splits, rt):
             check(out[a:b], *attention(q[a:b].double().cpu(), *truth[s], [ctx[s] + i + 1 for i in range(n)], scale))
 
 
-def groups_of(sizes, prefixes, tails, Hkv, D, bs, fmt, dev, gen):
+def groups_of(sizes, prefixes, tails, Hkv, D, bs, fmt, dev, gen, fill=None):
     """Sequences in groups; a group's whole pages of the prefix are common, and only its first sequence's table is right below the
     prefix: the others' first pages are somebody else's."""
     lens = [p + t for m, p, tt in zip(sizes, prefixes, tails) for t in tt]
-    cache, table, truth = make(lens, Hkv, D, bs, fmt, dev, gen)
+    cache, table, truth = make(lens, Hkv, D, bs, fmt, dev, gen, fill)
     seqs, at = [], 0
     for m, p in zip(sizes, prefixes):
         for i in range(m):
@@ -515,6 +515,40 @@ def test_shared_prefix_of_sequences_shorter_than_it(dev, fmt):
     out = ops.shared_prefix_attention(q, cache, table, i32(short, dev), plan, 0.2)
     for s, L in enumerate(short):
         check(out[s:s + 1], *attention(q[s:s + 1].double().cpu(), *seqs[s], [L], 0.2))
+
+
+@DEVICES
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("D,Hq", [(128, 8), (64, 24), (64, 2)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_a_value_that_is_not_finite_reaches_only_those_who_see_it(dev, fmt, D, Hq, wide, monkeypatch):
+    """Sequences shorter than their prefix beside longer ones; behind the second group's, pages that were never written."""
+    if wide:
+        monkeypatch.setattr(kv_quant, "WIDE_ROWS", 0)
+        monkeypatch.setattr(kv_quant, "WIDE_TILES", 0)
+    gen = torch.Generator().manual_seed(23)
+
+    def fill(k, v):
+        v[40, 0, 3] = math.inf
+        v[95, 1, D - 1] = -math.inf
+        v[200, 1, 7] = math.nan
+        v[201, 1, 6] = math.nan
+        v[299, 0, 17] = math.inf
+
+    sizes, prefixes = [12, 3], [300, 64]
+    tails = [[10, 1] + [0] * 10, [1, 1, 1]]
+    cache, table, lens, seqs = groups_of(sizes, prefixes, tails, 2, D, 16, fmt, dev, gen, fill)
+    short = [310, 301, 300, 299, 41, 40, 39, 200, 201, 0, 96, 64] + [65, 30, 1]
+    q = rows(len(short), Hq, D, gen).to(dev)
+    plan = ops.shared_prefix_plan(sizes, [300, 200], Hq, 2, dev)
+    assert (plan.wide is not None) == wide
+    out = ops.shared_prefix_attention(q, cache, table, i32(short, dev), plan, 0.1)
+    for s, L in enumerate(short):
+        ref, bound = attention(q[s:s + 1].double().cpu(), *seqs[s], [L], 0.1)
+        got = out[s:s + 1].double().cpu()
+        assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got[ref.isinf()], ref[ref.isinf()])
+        good = ref.isfinite()
+        check(got[good], ref[good], bound[good])
 
 
 def test_work_of_a_plan():
@@ -610,6 +644,8 @@ def test_refusals():
         ops.QuantKVCache(c.k.transpose(0, 2), c.v.transpose(0, 2), c.scales, "fp8")
     with pytest.raises(TypeError):
         ops.QuantKVCache(c.k.view(torch.int8), c.v, c.scales, "fp8")
+    with pytest.raises(ValueError):
+        ops.QuantKVCache(c.k, torch.zeros(c.v.numel() + 8, dtype=torch.uint8)[8:].view(c.v.shape), c.scales, "fp8")
 
     rows3, slots = z(3, 2, 64), z(3, dtype=i)
     for k, v, s, e in ((rows3.float(), rows3, slots, TypeError), (rows3, rows3.half(), slots, TypeError),
@@ -620,7 +656,8 @@ def test_refusals():
         with pytest.raises(e):
             ops.kv_quant_append(k, v, c, s)
     cs = z(8, 64, dtype=f32)
-    for qkv, pos, table, e in ((z(3, 6 * 64 - 1), slots, cs, ValueError), (z(3, 6 * 64), slots.long(), cs, TypeError),
+    for qkv, pos, table, e in ((z(3, 6 * 64 - 1), slots, cs, ValueError), (z(1, 6 * 64).expand(3, -1), slots, cs, ValueError),
+                               (z(3, 6 * 64), slots.long(), cs, TypeError),
                                (z(3, 6 * 64), slots[:2], cs, ValueError), (z(3, 6 * 64), slots, cs.double(), TypeError),
                                (z(3, 6 * 64), slots, z(8, 32, dtype=f32), ValueError)):
         with pytest.raises(e):
@@ -641,6 +678,8 @@ def test_refusals():
                         ((q, c, bt[:1], ln), {}, ValueError), ((q, c, bt, ln.long()), {}, TypeError),
                         ((q, c, bt[:, :0], ln), {}, ValueError), ((q, c, bt, ln), dict(num_splits=0), ValueError),
                         ((q, c, bt, ln), dict(num_splits=65), ValueError), ((q, c, bt, ln), dict(out=z(2, 4, 32)), ValueError),
+                        ((q, c, bt, ln), dict(out=z(1, 4, 64).expand(2, -1, -1)), ValueError),
+                        ((z(2, 0, 64), c, bt, ln), {}, ValueError),
                         ((q, c, bt, ln), dict(out=z(2, 4, 64, dtype=f32)), TypeError)):
         with pytest.raises(e):
             ops.quant_decode_attention(*args, 0.1, **kw)

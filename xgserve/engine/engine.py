@@ -863,6 +863,8 @@ class LLMEngine:
             raise ValueError(f"entry block_size {entry.block_size} != engine {self.cfg.block_size}")
         if entry.meta.get("kv_cache_dtype") != self.cfg.kv_cache_dtype:
             raise ValueError(f"entry KV dtype {entry.meta.get('kv_cache_dtype')} != engine {self.cfg.kv_cache_dtype}")
+        if self.runner.kv_quant is not None and entry.kv.dtype != torch.uint8:
+            raise ValueError(f"entry pages are {entry.kv.dtype}, an 8-bit cache's bytes are uint8")
         page_dim = 2 if self.runner.kv_quant is None else 1
         n_pages = entry.kv.shape[page_dim] if entry.kv.dim() > page_dim else 0
         want = self.runner.page_shape(n_pages)

@@ -86,6 +86,7 @@ class QuantKVCache:
         _need(tuple(self.scales.shape) == (nb, hkv, 2, bs), "scales must be [num_blocks, Hkv, 2, block_size]")
         _need(all(t.is_contiguous() for t in (self.k, self.v, self.scales)), "a cache is contiguous")
         _need(self.k.device == self.v.device == self.scales.device, "a cache is on one device")
+        _need(all(t.data_ptr() % 16 == 0 for t in (self.k, self.v, self.scales)), "a cache's parts begin at multiples of 16 bytes")
         self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = self.dims = nb, hkv, bs, d
         self.device, self.code = self.k.device, KV_FORMATS[self.fmt]
         self.index = self.k.get_device()   # -1: host
@@ -259,6 +260,7 @@ def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
     H, D, T = cache.num_kv_heads, cache.head_dim, qkv.shape[0]
     _need(qkv.dim() == 2 and qkv.shape[1] >= (num_heads + 2 * H) * D and (T == 0 or qkv.stride(1) == 1),
           "qkv must be [T, (Hq + 2 Hkv) D], contiguous in the last dimension")
+    _need(T < 2 or qkv.stride(0) >= qkv.shape[1], "qkv's tokens must not overlap")
     k = qkv[:, num_heads * D:(num_heads + H) * D].unflatten(1, (H, D))
     v = qkv[:, (num_heads + H) * D:(num_heads + 2 * H) * D].unflatten(1, (H, D))
     if not apply_rope:
@@ -342,7 +344,7 @@ def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch
         for s in range(S):
             lo, a, b = int(starts[s]), int(cu_tokens[s]), min(int(cu_tokens[s + 1]), num_tokens)
             n = min(b - a, W * cache.block_size - lo)
-            if n > 0:
+            if n > 0 and lo >= 0:
                 k[a:a + n], v[a:a + n] = _rows_ref(cache, _slots_ref(block_tables[s], cache.block_size, lo, lo + n, cache.num_blocks))
         return k, v
     kernels().kv_read(cache.code, cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), block_tables.data_ptr(),
@@ -369,6 +371,7 @@ def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out.dtype != q.dtype:
         raise TypeError(f"out must be {q.dtype}, got {out.dtype}")
     _need(out.shape == q.shape and out.device == q.device, f"out must be {list(q.shape)} beside q")
+    _need(q.shape[0] < 2 or out.stride(0) >= q.shape[1] * q.shape[2], "out's tokens must not overlap")
     if q.shape[0]:
         _need(out.stride(2) == 1 and (q.shape[1] == 1 or out.stride(1) == q.shape[2]) and out.stride(0) % 4 == 0
               and out.data_ptr() % 8 == 0, "out's heads must be contiguous within a token, and tokens begin at multiples of 8 bytes")
@@ -384,7 +387,7 @@ def _check_tables(block_tables, seq_lens, device, S: int) -> None:
 
 def _check_decode(q, Hkv: int, D: int, index: int, device, block_tables, seq_lens) -> None:
     """q, tables and lengths of a step with one new token of each sequence."""
-    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 and _plain_table(block_tables, index, q.shape[0])
+    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 < q.shape[1] and _plain_table(block_tables, index, q.shape[0])
             and _plain_lists(index, q.shape[0], seq_lens)):
         _check_q(q, Hkv, D, device)
         _check_tables(block_tables, seq_lens, device, q.shape[0])
@@ -429,8 +432,8 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`decode_attention` over an 8-bit cache: q [B, Hq, D] bf16 (tokens may be strided), one new token of each sequence, whose own
     key is in the cache already -> [B, Hq, D]. block_tables [B, W], seq_lens [B] int32; a length of 0 gives zeros, one behind the
-    table means the whole table. num_splits: parts that a sequence's keys are cut into on average, more the longer it is (None: by the
-    batch and the table's width); a workspace needs B num_splits of them."""
+    table means the whole table. num_splits: parts that a sequence's keys are cut into on average, more the longer it is; a workspace
+    needs B num_splits of them (None: by the batch and the table's width, at most B + 512)."""
     (nb, Hkv, bs, D), dev = cache.dims, cache.device
     _check_decode(q, Hkv, D, cache.index, dev, block_tables, seq_lens)
     B, Hq, _ = q.shape
@@ -478,7 +481,7 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
     sweeps; None = `_row_tiles`): 1, 2 or 8."""
     (nb, Hkv, bs, D), dev, index = cache.dims, cache.device, cache.index
     S = seq_lens.shape[0]
-    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 and _plain_table(block_tables, index, S)
+    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 < q.shape[1] and _plain_table(block_tables, index, S)
             and _plain_lists(index, S, seq_lens) and _plain_lists(index, S + 1, query_start_loc) and max_q_len >= 0):
         _check_q(q, Hkv, D, dev)
         _check_tables(block_tables, seq_lens, dev, S)
@@ -597,7 +600,7 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
     """Decode attention q [B, Hq, D] bf16 of sequences in groups with a common prefix, whose keys are read once for the group: of a
     group, the first prefix_lens[g] keys of every sequence are those of its first sequence's table, the rest its own table's; a
     sequence shorter than the prefix sees as much of it as it is long. kv: a `QuantKVCache`, or the bf16 pages (k, v) [NB, Hkv, bs,
-    D]. num_splits: parts of the keys behind the prefix, on average. A workspace needs B (plan.slots + num_splits) of them."""
+    D]. num_splits: parts of the keys behind the prefix, as in `quant_decode_attention`. A workspace needs these and B plan.slots."""
     quant = isinstance(kv, QuantKVCache)
     if quant:
         kc, vc, (nb, Hkv, bs, D), fmt = kv.k, kv.v, kv.dims, kv.code
