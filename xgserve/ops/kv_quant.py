@@ -36,9 +36,11 @@ SPLIT_WGS = 512     # workgroups that fill the chip: two a CU
 SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
 WHOLE_UNITS = 16    # units of SPLIT_KEYS that stay whole where the sequences alone fill most of the chip
 SPLIT_FROM = 1024
-# the common parts of shared prefixes: one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences behind
-# 4096 keys: 256 workgroups 26.9 us, 512 32.6, 1024 40.6)
+# the common parts of shared prefixes: at most one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences
+# behind 4096 keys: 256 workgroups 27 us, 384 30, 512 31, 1024 40; 128 behind 8000: 48, 54, 57, 61), or half as many again where one
+# would have PREFIX_LONG 32-key tiles and more (5 groups of 27 behind 5 - 30 k: 248 workgroups 88 us, 360 71, 504 74)
 PREFIX_WGS = 256
+PREFIX_LONG = 192
 
 
 def _need(ok: bool, what: str) -> None:
@@ -451,7 +453,7 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
             out[b] = 0
             if L > 0:
                 k, v = _any_rows_ref(cache, block_tables[b], 0, L)
-                out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
+                out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1], device=q.device), scale)[0].to(q.dtype)
         return out
     keep, po, pl = _parts(workspace, shares * Hq, D, dev) if shares > B else (None, 0, 0)
     kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
@@ -551,7 +553,7 @@ WIDE_TILES = 48
 
 
 def _prefix_work(sizes, lens, G: int, Hkv: int, rt: int, each: int, put) -> PrefixWork:
-    """each: 32-key tiles of a workgroup."""
+    """each: 32-key tiles of a workgroup, at most."""
     items: List[List[int]] = []
     counts, at = [], 0
     for n, p in zip(sizes, lens):
@@ -581,14 +583,24 @@ def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], n
     def put(rows, width):
         return torch.tensor(rows, dtype=torch.int32).reshape(-1, *width).to(device)
 
-    def tiles(rt):   # of a workgroup, where PREFIX_WGS have them all
-        total = sum(-(-n * G // (16 * rt)) * -(-p // 32) for n, p in zip(sizes, lens)) * num_kv_heads
-        return max(4, -(-total // PREFIX_WGS))
+    def tiles(rt, wgs):   # of a workgroup, where so many have them all (or nearly: no more than twice the mean)
+        work = [(num_kv_heads * -(-n * G // (16 * rt)), -(-p // 32)) for n, p in zip(sizes, lens)]
+        lo = max(4, -(-sum(b * t for b, t in work) // wgs))
+        hi = 2 * lo
+        while lo < hi:
+            mid = (lo + hi) // 2
+            lo, hi = (lo, mid) if sum(b * -(-t // mid) for b, t in work) <= wgs else (mid + 1, hi)
+        return lo
 
     most = max([n * G for n, p in zip(sizes, lens) if p > 0], default=0)
     rt = 1 if most <= 16 else 2
-    work = _prefix_work(sizes, lens, G, num_kv_heads, rt, tiles(rt), put)
-    wide = _prefix_work(sizes, lens, G, num_kv_heads, 8, tiles(8), put) if most >= WIDE_ROWS and tiles(rt) >= WIDE_TILES else None
+    each = tiles(rt, PREFIX_WGS)
+    wide = None
+    if most >= WIDE_ROWS and each >= WIDE_TILES:
+        wide = _prefix_work(sizes, lens, G, num_kv_heads, 8, tiles(8, PREFIX_WGS), put)
+    if each >= PREFIX_LONG:
+        each = tiles(rt, PREFIX_WGS * 3 // 2)
+    work = _prefix_work(sizes, lens, G, num_kv_heads, rt, each, put)
     prefix = [p for n, p in zip(sizes, lens) for _ in range(n)]
     return SharedPrefixPlan(len(prefix), num_heads, num_kv_heads, work, wide, max(work.slots, wide.slots if wide else 0),
                             put(prefix, ()), tuple(sizes), tuple(lens), min(lens, default=0), max(lens, default=0))
@@ -640,7 +652,7 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
                 if L > 0:
                     front, back = _any_rows_ref(kv, block_tables[at], 0, min(p, L)), _any_rows_ref(kv, block_tables[b], min(p, L), L)
                     k, v = (torch.cat(x) for x in zip(front, back))
-                    out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1]), scale)[0].to(q.dtype)
+                    out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1], device=q.device), scale)[0].to(q.dtype)
             at += n
         return out
     keep, po, pl = _parts(workspace, (B * work.slots + shares) * Hq, D, dev) if work.slots or shares > B else (None, 0, 0)
