@@ -81,6 +81,11 @@ def available() -> bool:
         return False
 
 
+def loaded() -> bool:
+    """Whether `kernels()` has the library already."""
+    return _K is not None
+
+
 def use_native(t: torch.Tensor) -> bool:
     """True when `t` lives on the GPU (native path mandatory)."""
     if t.device.type != "cuda":

@@ -21,7 +21,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ._native import kernels, on_current_device, ptr, stream_ptr, use_native
+from ._native import kernels, loaded, ptr, stream_ptr, use_native
 from .attention import DecodeWorkspace, _attend
 from .rope import _rotate
 
@@ -98,11 +98,12 @@ class QuantKVCache:
 
 
 def _native(cache_tensor: torch.Tensor) -> bool:
-    if not cache_tensor.is_cuda or not use_native(cache_tensor):
+    index = cache_tensor.get_device()
+    if index < 0:
         return False
-    if not on_current_device(cache_tensor):
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"the cache is on {cache_tensor.device}, which is not the current device")
-    return True
+    return loaded() or use_native(cache_tensor)
 
 
 # Arguments are looked over twice: `_plain_*` ask once whether all is as it nearly always is (a call of a decode step is
@@ -311,7 +312,7 @@ def rope_kv_quant_partials(pend, positions: torch.Tensor, cos_sin: torch.Tensor,
         kv_quant_append_ref(k.to(torch.bfloat16), v.to(torch.bfloat16), cache, slot_mapping)
         return q.copy_(x.flatten(1))
     nb, _, bs, _ = cache.dims
-    kernels().kv_append_partials(cache.code, pend.part.data_ptr(), S, q.data_ptr(), q.stride(0), slot_mapping.data_ptr(),
+    kernels().kv_append_partials(cache.code, pend.part.data_ptr(), S, q.data_ptr(), num_heads * D, slot_mapping.data_ptr(),
                                  positions.data_ptr(), cos_sin.data_ptr() if apply_rope else 0, cache.k.data_ptr(),
                                  cache.v.data_ptr(), cache.scales.data_ptr(), nb, T, num_heads, H, D, bs, stream_ptr())
     return q
@@ -350,7 +351,7 @@ def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch
                 k[a:a + n], v[a:a + n] = _rows_ref(cache, _slots_ref(block_tables[s], cache.block_size, lo, lo + n, cache.num_blocks))
         return k, v
     kernels().kv_read(cache.code, cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), block_tables.data_ptr(),
-                      block_tables.stride(0), W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens, nb, Hkv, D, bs,
+                      block_tables.stride()[0], W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens, nb, Hkv, D, bs,
                       k.data_ptr(), v.data_ptr(), stream_ptr())
     return k, v
 
@@ -367,9 +368,11 @@ def _check_q(q: torch.Tensor, Hkv: int, D: int, device) -> None:
         _need(q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0, "q's tokens must begin at multiples of 16 bytes")
 
 
-def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """The output, and the stride of its tokens."""
     if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        return out, out.stride()[0]
     if out.dtype != q.dtype:
         raise TypeError(f"out must be {q.dtype}, got {out.dtype}")
     _need(out.shape == q.shape and out.device == q.device, f"out must be {list(q.shape)} beside q")
@@ -377,7 +380,7 @@ def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if q.shape[0]:
         _need(out.stride(2) == 1 and (q.shape[1] == 1 or out.stride(1) == q.shape[2]) and out.stride(0) % 4 == 0
               and out.data_ptr() % 8 == 0, "out's heads must be contiguous within a token, and tokens begin at multiples of 8 bytes")
-    return out
+    return out, out.stride()[0]
 
 
 def _check_tables(block_tables, seq_lens, device, S: int) -> None:
@@ -387,12 +390,14 @@ def _check_tables(block_tables, seq_lens, device, S: int) -> None:
     _need(block_tables.shape[1] >= 1 or S == 0, "block_tables must have a column")
 
 
-def _check_decode(q, Hkv: int, D: int, index: int, device, block_tables, seq_lens) -> None:
-    """q, tables and lengths of a step with one new token of each sequence."""
-    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 < q.shape[1] and _plain_table(block_tables, index, q.shape[0])
-            and _plain_lists(index, q.shape[0], seq_lens)):
+def _check_decode(q, Hkv: int, D: int, index: int, device, block_tables, seq_lens) -> Tuple[int, int, int]:
+    """q, tables and lengths of a step with one new token of each sequence -> sequences, query heads, columns."""
+    (B, Hq, _), W = q.shape if q.dim() == 3 else (0, 0, 0), block_tables.shape[-1]
+    if not (_plain_heads(q, index, D, 8, 16) and Hq % Hkv == 0 < Hq and _plain_table(block_tables, index, B)
+            and _plain_lists(index, B, seq_lens)):
         _check_q(q, Hkv, D, device)
-        _check_tables(block_tables, seq_lens, device, q.shape[0])
+        _check_tables(block_tables, seq_lens, device, B)
+    return B, Hq, W
 
 
 def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
@@ -437,10 +442,8 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     table means the whole table. num_splits: parts that a sequence's keys are cut into on average, more the longer it is; a workspace
     needs B num_splits of them (None: by the batch and the table's width, at most B + 512)."""
     (nb, Hkv, bs, D), dev = cache.dims, cache.device
-    _check_decode(q, Hkv, D, cache.index, dev, block_tables, seq_lens)
-    B, Hq, _ = q.shape
-    out = _check_out(out, q)
-    W = block_tables.shape[1]
+    B, Hq, W = _check_decode(q, Hkv, D, cache.index, dev, block_tables, seq_lens)
+    out, out_stride = _check_out(out, q)
     blocks = -(-Hq // Hkv // 16)
     shares, least = _shares(num_splits, B, Hkv * blocks, W * bs)
     if B == 0:
@@ -456,9 +459,9 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
                 out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1], device=q.device), scale)[0].to(q.dtype)
         return out
     keep, po, pl = _parts(workspace, shares * Hq, D, dev) if shares > B else (None, 0, 0)
-    kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
-                                     cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
-                                     seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale,
+    kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride()[0], cache.k.data_ptr(), cache.v.data_ptr(),
+                                     cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride()[0], W,
+                                     seq_lens.data_ptr(), po, pl, out.data_ptr(), out_stride, B, Hq, Hkv, D, bs, nb, scale,
                                      shares, least, stream_ptr())
     return out
 
@@ -491,7 +494,7 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
         _need(query_start_loc.shape[0] == S + 1, "query_start_loc must have one entry more than seq_lens")
         _need(0 <= max_q_len, "max_q_len must not be negative")
     T, Hq, _ = q.shape
-    out = _check_out(out, q)
+    out, out_stride = _check_out(out, q)
     if T == 0 or S == 0 or max_q_len == 0:
         return out
     W, G = block_tables.shape[1], Hq // Hkv
@@ -512,9 +515,9 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
                 out[a:a + n] = _attend_causal(q[a:a + n], k, v, max(L - (b - a), 0), scale).to(q.dtype)
         return out
     keep, po, pl = _parts(workspace, T * Hq * splits, D, dev) if splits > 1 else (None, 0, 0)
-    kernels().quant_prefill_attention(cache.code, q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(),
-                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), W,
-                                      query_start_loc.data_ptr(), seq_lens.data_ptr(), po, pl, out.data_ptr(), out.stride(0), T, S,
+    kernels().quant_prefill_attention(cache.code, q.data_ptr(), q.stride()[0], cache.k.data_ptr(), cache.v.data_ptr(),
+                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride()[0], W,
+                                      query_start_loc.data_ptr(), seq_lens.data_ptr(), po, pl, out.data_ptr(), out_stride, T, S,
                                       max_q_len, Hq, Hkv, D, bs, nb, scale, rt, splits, stream_ptr())
     return out
 
@@ -627,15 +630,13 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
         if D not in (64, 128) or bs < TILE or bs % TILE or nb < 1 or Hkv < 1:
             raise ValueError(f"heads of 64 or 128 numbers in pages of a multiple of {TILE} tokens")
     dev = kc.device
-    _check_decode(q, Hkv, D, kc.get_device(), dev, block_tables, seq_lens)
-    B, Hq, _ = q.shape
-    W = block_tables.shape[1]
+    B, Hq, W = _check_decode(q, Hkv, D, kc.get_device(), dev, block_tables, seq_lens)
     if plan.num_seqs != B or plan.num_heads != Hq or plan.num_kv_heads != Hkv:
         raise ValueError(f"the plan is for {plan.num_seqs} sequences of {plan.num_heads} / {plan.num_kv_heads} heads, not {B} of {Hq} / {Hkv}")
     if plan.prefix.device != dev or plan.longest > W * bs:
         raise ValueError(f"the plan is on {plan.prefix.device}, the cache on {dev}" if plan.prefix.device != dev
                          else "a prefix is longer than the tables")
-    out = _check_out(out, q)
+    out, out_stride = _check_out(out, q)
     blocks = -(-Hq // Hkv // 16)
     shares, least = _shares(num_splits, B, Hkv * blocks, W * bs - plan.shortest)
     work = plan.work if quant or plan.wide is None else plan.wide
@@ -656,9 +657,9 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
             at += n
         return out
     keep, po, pl = _parts(workspace, (B * work.slots + shares) * Hq, D, dev) if work.slots or shares > B else (None, 0, 0)
-    kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride(0), kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
-                                      block_tables.data_ptr(), block_tables.stride(0), W, seq_lens.data_ptr(), po, pl,
-                                      out.data_ptr(), out.stride(0), B, Hq, Hkv, D, bs, nb, scale, work.items.data_ptr(),
+    kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride()[0], kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
+                                      block_tables.data_ptr(), block_tables.stride()[0], W, seq_lens.data_ptr(), po, pl,
+                                      out.data_ptr(), out_stride, B, Hq, Hkv, D, bs, nb, scale, work.items.data_ptr(),
                                       work.items.shape[0], plan.prefix.data_ptr(), work.counts.data_ptr(), work.slots,
                                       work.row_tiles, shares, least, stream_ptr())
     return out
