@@ -23,7 +23,7 @@
 namespace xgk {
 
 constexpr float RAISE = 8.f;          // in base 2
-constexpr float LOWEST = -1e30f;      // the maximum of no key: exp2(LOWEST - any) is 0
+constexpr float LOWEST = -3.4e38f;    // the maximum of no key, below every score's: exp2(LOWEST - any) is 0
 
 struct RowsArgs {
   const uint16_t* q;

@@ -414,6 +414,57 @@ def test_scores_far_apart(dev, fmt):
 
 @DEVICES
 @FORMATS
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("exact", [False, True])
+def test_scores_further_down_than_any_mask(dev, fmt, D, exact):
+    """All keys alike, and scores of about -2^112. Where the row's largest magnitude is the largest code times a power of two, and softmax's
+    scale ln 2 (1 in base 2, to 32 bits), each score has few bits and is exact: the mean of the values; a weight of 1 times the value's
+    scale and the output are rounded to bf16, each off by 2^-8 of it at most. Else 32 bits leave a score 2^88 of room, so the weights may be any (a product that is
+    rounded at once with the maximum's difference has the part that the maximum lost), and so may those of parts, whose log-sums of
+    2^112 and 2^112 + 8 are one number: the output lies among the values."""
+    gen = torch.Generator().manual_seed(19)
+    lens = [300, 33, 1]
+
+    def fill(k, v):
+        k.zero_()
+        k[:, :, 0] = kv_quant.LARGEST[fmt] * 2.0 ** 44 if exact else 2.0 ** 50
+
+    cache, table, truth = make(lens, 1, D, 16, fmt, dev, gen, fill)
+    q = torch.zeros(3, 4, D, dtype=torch.bfloat16)
+    q[..., 0] = -(2.0 ** 62)
+    args, scale = (q.to(dev), cache, table), math.log(2.0) if exact else 1.0
+    plan = ops.shared_prefix_plan([1, 1, 1], [64, 32, 0], 4, 1, dev)
+    outs = [(n, ops.quant_decode_attention(*args, i32(lens, dev), scale, num_splits=n)) for n in (1, 3)]
+    outs += [(n, ops.quant_prefill_attention(*args, i32([0, 1, 2, 3], dev), i32(lens, dev), 1, scale, num_splits=n, row_tiles=rt))
+             for n, rt in ((1, 1), (3, 1), (1, 2), (1, 8), (3, 8))]
+    outs.append((2, ops.shared_prefix_attention(*args, i32(lens, dev), plan, scale)))
+    for s in range(3):
+        v = truth[s][1][:, 0]
+        for parts, out in outs:
+            if exact and parts == 1:
+                check(out[s], v.mean(0).expand(4, D), ((v.abs().mean(0) + v.mean(0).abs()) * 1.01 * 2.0 ** -8 + 1e-30).expand(4, D))
+            else:
+                room = v.abs().amax(0) * 1.01 * 2.0 ** -7
+                o = out[s].double().cpu()
+                assert bool(((o >= v.amin(0) - room) & (o <= v.amax(0) + room)).all())
+
+
+@DEVICES
+@FORMATS
+def test_portions_longer_than_their_sequences(dev, fmt):
+    """Lengths below a portion's tokens, and below zero: the first token sees the first key, and none sees more than there are."""
+    gen = torch.Generator().manual_seed(20)
+    cache, table, truth = make([40, 40, 40], 2, 64, 16, fmt, dev, gen)
+    q = rows(3 * 35, 4, 64, gen).to(dev)
+    for splits, rt in ((1, 1), (1, 2), (3, 2), (1, 8), (3, 8)):
+        out = ops.quant_prefill_attention(q, cache, table, i32([0, 35, 70, 105], dev), i32([-5, 0, 20], dev), 35, 0.1,
+                                          num_splits=splits, row_tiles=rt)
+        assert bool((out[:70] == 0).all())
+        check(out[70:], *attention(q[70:].double().cpu(), *truth[2], [min(i + 1, 20) for i in range(35)], 0.1))
+
+
+@DEVICES
+@FORMATS
 def test_a_key_that_is_not_finite_reaches_only_those_who_see_it(dev, fmt):
     gen = torch.Generator().manual_seed(14)
 

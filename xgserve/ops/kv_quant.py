@@ -511,7 +511,7 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
             a, b = int(query_start_loc[s]), int(query_start_loc[s + 1])
             n, L = min(b - a, max_q_len), int(seq_lens[s])
             if n > 0:
-                k, v = _any_rows_ref(cache, block_tables[s], 0, min(L, W * bs))
+                k, v = _any_rows_ref(cache, block_tables[s], 0, max(0, min(L, W * bs)))
                 out[a:a + n] = _attend_causal(q[a:a + n], k, v, max(L - (b - a), 0), scale).to(q.dtype)
         return out
     keep, po, pl = _parts(workspace, T * Hq * splits, D, dev) if splits > 1 else (None, 0, 0)
