@@ -5,12 +5,12 @@
 // prompt portion G rows a token, a group of sequences with a common prefix G rows a member. A workgroup takes a block of
 // 16 RT rows and a range of keys; its four waves take 32-key tiles of the range in turn, each for all the rows:
 //   S^T[16 keys][16 rows] = K Q^T   v_mfma_f32_16x16x32_bf16; K fragments come from the cache as they lie (8-bit codes
-//     widened in registers), the key's scale joins softmax's scale afterwards: no rounding but the products' own
+//     widened in registers; bf16: whole rows, brought into order through LDS), the key's scale joins softmax's scale afterwards: no rounding but the products' own
 //   softmax in base 2 by running maximum. The maximum is only raised (and the accumulators rescaled) when a score passes
 //     it by more than 2^8: fp32 sums and bf16 weights are relative, so weights up to 2^8 cost no precision
 //   O^T[D][16 rows] += V^T P^T      the same instruction over 32 keys. The S^T accumulators are the P^T fragment where
 //     the 8 keys of lane group g are 4 g + {0..3} of both 16-key halves; the cache holds V in that order (bf16: V is
-//     turned through LDS). V's scale joins the weight before its rounding to bf16 (2^-9, as everywhere here)
+//     turned through LDS). V's scale joins the weight before its rounding to bf16 (2^-8 of it at most, as everywhere here)
 // The waves' states join through LDS, parts of a row's keys through rows_join_kernel: (O / l, log2-sum-exp) in fp32.
 //
 // Waves share no tile, so the key loop has no barrier, and K / V go from HBM to registers: one tile's loads are on their
@@ -277,6 +277,15 @@ __device__ __forceinline__ void load_row(const RowsArgs& p, const RowsBlock& w, 
   }
 }
 
+// bf16 K of 16 tokens in LDS: where 8 dims (chunk ch) of a token lie, in fragment order. The tokens of a chunk are turned by it, so
+// whole rows are written and fragments read without bank conflicts. Fragments straight from the cache are 16 bytes of 16 rows, for which
+// a CU's address unit takes a clock a lane in place of one for four: it was busy for 75 % of the time (64 sequences behind 4096 keys
+// 39.2 -> 34.5 us, 64 heads on 8 of 20 behind 3000 21.9 -> 18.4).
+template <int D>
+__device__ __forceinline__ uint32_t k_chunk(int token, int ch) {
+  return ((ch * 16) + (token ^ (ch & 7))) * 16;
+}
+
 template <int FMT, int D, int RT, bool ONCE>
 __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w, int kvh, uint8_t* space,
                                             float (*m_lds)[16 * RT], float (*l_lds)[16 * RT]) {
@@ -300,8 +309,8 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   const Constant<int32_t> table = constant(p.tables + w.table * p.table_stride);
   uint4 kr[2][C::LOADS], vr[2][C::LOADS];
   float4 ks[2], vs[2];
-  // a decode step reads its keys once (non-temporal); blocks of rows over the same keys find them in the L2. (bf16 K fragments are
-  // half lines, whose other half the next load finds in the L1: 43 us non-temporal 55, 64 rows behind a prefix of 4096)
+  // a decode step reads its 8-bit keys once (non-temporal); blocks of rows over the same keys find them in the L2. (bf16: 64 sequences
+  // behind 4096 keys 34.5 us, with their own keys non-temporal 38.6)
   auto load16 = [](const void* at) { return ONCE && !C::WIDE ? ld16_nt(at) : ld16(at); };
   // where the halves of a tile lie: clamped to the last tile that holds a key, and into the cache. The page numbers of the
   // tile after the next are asked for while the next one's loads go out, so no load waits for its address. Addresses are scalar
@@ -335,8 +344,7 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
     for (int a = 0; a < 2; ++a) {
       const uint8_t* base = k_head + at[a];
 #pragma unroll
-      for (int i = 0; i < C::LOADS; ++i)
-        kr[a][i] = load16(base + (C::WIDE ? static_cast<uint32_t>(li * D * 2 + 16 * g + 64 * i) : static_cast<uint32_t>(lane * 16 + 1024 * i)));
+      for (int i = 0; i < C::LOADS; ++i) kr[a][i] = load16(base + static_cast<uint32_t>(lane * 16 + 1024 * i));
       if constexpr (!C::WIDE) ks[a] = *reinterpret_cast<const float4*>(factor[a] + 4 * g);
     }
   };
@@ -385,6 +393,13 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   const int whole = max(0, min(n, ((least >> 5) - t0 + 3) >> 2) - ahead);      // tiles that every row sees
   // S^T of the tile whose K is in registers
   auto product = [&](f32x4_t (&s)[2][RT]) {
+    uint8_t* turn = space + wid * 64 * D;
+    if constexpr (C::WIDE) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < C::LOADS; ++i) st16(turn + a * 32 * D + k_chunk<D>((lane + 64 * i) / (D / 8), (lane + 64 * i) % (D / 8)), kr[a][i]);
+    }
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
 #pragma unroll
@@ -395,7 +410,7 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
         for (int x = 0; x < (C::WIDE ? 1 : 2); ++x) {
           const int kk = C::WIDE ? i : 2 * i + x;
           bf16x8_t kx;
-          if constexpr (C::WIDE) kx = as_frag(kr[a][i]);
+          if constexpr (C::WIDE) kx = as_frag(ld16(turn + a * 32 * D + k_chunk<D>(li, 4 * i + g)));
           else kx = x == 0 ? kv_widen8<FMT>(kr[a][i].x, kr[a][i].y) : kv_widen8<FMT>(kr[a][i].z, kr[a][i].w);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[a][rt] = mfma16x16x32(kx, qf[rt][kk], s[a][rt]);
@@ -979,7 +994,7 @@ __global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsA
 // others by HBM, and run beside each other. Grid (Hkv, n_items + shares heads' blocks of 16). Parts: slots a row of the common
 // ones, then the shares'.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256, RT == 1 ? 3 : 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
+__global__ void __launch_bounds__(256, RT == 1 && !(FMT == KV_BF16 && D == 128) ? 3 : 2) rows_shared_kernel(RowsArgs p, const int32_t* items, int n_items, const int32_t* prefix,
                                                              const int32_t* counts, int slots, int B, int blocks, int shares) {
   constexpr int SPACE = RT == 8 && BlockCfg<FMT, D>::SPACE > RowsCfg<FMT, D, 2>::SPACE ? BlockCfg<FMT, D>::SPACE : RowsCfg<FMT, D, 2>::SPACE;
   constexpr int LISTS = RT == 8 ? 1 : RT;

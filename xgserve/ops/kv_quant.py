@@ -37,8 +37,9 @@ SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
 WHOLE_UNITS = 16    # units of SPLIT_KEYS that stay whole where the sequences alone fill most of the chip
 SPLIT_FROM = 1024
 # the common parts of shared prefixes: at most one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences
-# behind 4096 keys: 256 workgroups 27 us, 384 30, 512 31, 1024 40; 128 behind 8000: 48, 54, 57, 61), or half as many again where one
-# would have PREFIX_LONG 32-key tiles and more (5 groups of 27 behind 5 - 30 k: 248 workgroups 88 us, 360 71, 504 74)
+# behind 4096 keys, bf16: 256 workgroups 34.5 us, 384 39.0, 512 42.7, 768 46.7; 64 heads on 8 of 20 behind 3000: 18.3, 19.4, 24.4, 26.5),
+# or half as many again where one would have PREFIX_LONG 32-key tiles and more (5 groups of 27 behind 5 - 30 k: fp8 248 workgroups
+# 88 us, 360 71, 504 74; bf16 256 153, 384 136, 512 136)
 PREFIX_WGS = 256
 PREFIX_LONG = 192
 
@@ -548,9 +549,9 @@ class SharedPrefixPlan:
     longest: int
 
 
-# bf16 pages, whose V each wave turns through LDS: blocks of 128 rows share that, from rows that nearly fill one and a share of the
-# work on which their longer start is lost. us with blocks of 32 / 128 rows: 5 groups of 108 rows behind 5 - 30 k keys 156 / 123, 512
-# rows behind 8000 keys 76 / 62, 256 behind 4096 (32 tiles a workgroup) 35 / 38. (8-bit pages, fp8: 81 / 104, 52 / 55.)
+# bf16 pages, whose K and V each wave turns through LDS: blocks of 128 rows share that, from rows that nearly fill one and a share of
+# the work on which their longer start is lost. us with blocks of 32 / 128 rows: 5 groups of 108 rows behind 5 - 30 k keys 136 / 121, 512
+# rows behind 8000 keys 47 / 44, 256 behind 4096 (32 tiles a workgroup) 35 / 38. (8-bit pages, fp8: 81 / 104, 52 / 55.)
 WIDE_ROWS = 96
 WIDE_TILES = 48
 
