@@ -38,10 +38,11 @@ WHOLE_UNITS = 16    # units of SPLIT_KEYS that stay whole where the sequences al
 SPLIT_FROM = 1024
 # the common parts of shared prefixes: at most one workgroup a CU leaves room for the sequences' own keys beside them (64 sequences
 # behind 4096 keys, bf16: 256 workgroups 34.5 us, 384 39.0, 512 42.7, 768 46.7; 64 heads on 8 of 20 behind 3000: 18.3, 19.4, 24.4, 26.5),
-# or half as many again where one would have PREFIX_LONG 32-key tiles and more (5 groups of 27 behind 5 - 30 k: fp8 248 workgroups
-# 88 us, 360 71, 504 74; bf16 256 153, 384 136, 512 136)
+# or two a CU where one would have PREFIX_LONG 32-key tiles and more (fp8, 256 / 384 / 512: 27 behind 40 k with up to 100 keys of their own
+# 48 / 47 / 40, up to 900 51 / 49 / 46; 5 groups of 27 behind 5 - 30 k 111 / 85 / 85; 27 behind 60 k 72 / 64 / 55. Shorter ones, 64 behind
+# 16 k with up to 900, have 43 / 46 / 51)
 PREFIX_WGS = 256
-PREFIX_LONG = 192
+PREFIX_LONG = 144
 
 
 def _need(ok: bool, what: str) -> None:
@@ -603,7 +604,7 @@ def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], n
     if most >= WIDE_ROWS and each >= WIDE_TILES:
         wide = _prefix_work(sizes, lens, G, num_kv_heads, 8, tiles(8, PREFIX_WGS), put)
     if each >= PREFIX_LONG:
-        each = tiles(rt, PREFIX_WGS * 3 // 2)
+        each = tiles(rt, PREFIX_WGS * 2)
     work = _prefix_work(sizes, lens, G, num_kv_heads, rt, each, put)
     prefix = [p for n, p in zip(sizes, lens) for _ in range(n)]
     return SharedPrefixPlan(len(prefix), num_heads, num_kv_heads, work, wide, max(work.slots, wide.slots if wide else 0),
