@@ -551,8 +551,8 @@ class SharedPrefixPlan:
 
 
 # bf16 pages, whose K and V each wave turns through LDS: blocks of 128 rows share that, from rows that nearly fill one and a share of
-# the work on which their longer start is lost. us with blocks of 32 / 128 rows: 5 groups of 108 rows behind 5 - 30 k keys 136 / 121, 512
-# rows behind 8000 keys 47 / 44, 256 behind 4096 (32 tiles a workgroup) 35 / 38. (8-bit pages, fp8: 81 / 104, 52 / 55.)
+# the work on which their longer start is lost. us with blocks of 32 / 128 rows: 5 groups of 108 rows behind 5 - 30 k keys 132 / 113, 108
+# rows behind 40 k 61 / 52, 512 behind 8000 47 / 44, 256 behind 4096 (32 tiles a workgroup) 35 / 38; fp8 81 / 104 and 52 / 55 (first and third).
 WIDE_ROWS = 96
 WIDE_TILES = 48
 
