@@ -108,28 +108,16 @@ def _native(cache_tensor: torch.Tensor) -> bool:
     return loaded() or use_native(cache_tensor)
 
 
-# Arguments are looked over twice: `_plain_*` ask once whether all is as it nearly always is (a call of a decode step is
-# mostly host time), and where it is not, `_check_*` allow it or say what is wrong.
+# Arguments are looked over twice: one condition asks whether all is as it nearly always is, each shape and stride asked for once (a call
+# of single tokens is mostly host time), and where it is not, `_check_*` and `_int32` allow it or say what is wrong.
 _BF16, _I32 = torch.bfloat16, torch.int32
-
-
-def _plain_heads(t: torch.Tensor, index: int, D: int, step: int, align: int) -> bool:
-    """[tokens, heads, D] bf16 whose tokens begin at multiples of `step` elements, the first of `align` bytes."""
-    st = t.stride()
-    return (len(st) == 3 and st[2] == 1 and st[1] == D and st[0] % step == 0 and t.shape[2] == D and t.dtype is _BF16
-            and t.get_device() == index and t.data_ptr() % align == 0)
 
 
 def _plain_lists(index: int, n: int, *lists: torch.Tensor) -> bool:
     for t in lists:
-        if t.dtype is not _I32 or t.shape != (n,) or t.stride() != (1,) or t.get_device() != index:
+        if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != index:
             return False
     return True
-
-
-def _plain_table(t: torch.Tensor, index: int, rows: int) -> bool:
-    st = t.stride()
-    return len(st) == 2 and st[1] == 1 and t.shape[0] == rows and t.dtype is _I32 and t.get_device() == index and t.shape[1] > 0
 
 
 # ------------------------------------------------------------------------------------------------------ plain (CPU) forms
@@ -230,9 +218,11 @@ def _check_rows(x: torch.Tensor, name: str, cache: QuantKVCache, T: int) -> None
 def kv_quant_append(k: torch.Tensor, v: torch.Tensor, cache: QuantKVCache, slot_mapping: torch.Tensor) -> None:
     """Writes rows k, v [T, Hkv, D] bf16 (tokens may be strided: views into the projection's rows) to the cache's slots
     slot_mapping [T] int32; tokens with a slot below 0 or behind the cache are left out. A slot may occur once in a call."""
-    T, index, D = k.shape[0], cache.index, cache.head_dim
-    if not (_plain_heads(k, index, D, D // 16, D // 8) and _plain_heads(v, index, D, D // 16, D // 8) and k.shape == v.shape
-            and k.shape[1] == cache.num_kv_heads and _plain_lists(index, T, slot_mapping)):
+    (nb, Hkv, bs, D), index, shape, sk, sv = cache.dims, cache.index, k.shape, k.stride(), v.stride()
+    T, kp, vp = shape[0], k.data_ptr(), v.data_ptr()
+    if not (shape == (T, Hkv, D) and v.shape == shape and sk[2] == 1 == sv[2] and sk[1] == D == sv[1] and sk[0] % (D // 16) == 0
+            and sv[0] % (D // 16) == 0 and kp % (D // 8) == 0 and vp % (D // 8) == 0 and k.dtype is _BF16 and v.dtype is _BF16
+            and k.get_device() == index and v.get_device() == index and _plain_lists(index, T, slot_mapping)):
         _check_rows(k, "k", cache, T)
         _check_rows(v, "v", cache, T)
         _int32(slot_mapping, "slot_mapping", 1, cache.device)
@@ -241,14 +231,8 @@ def kv_quant_append(k: torch.Tensor, v: torch.Tensor, cache: QuantKVCache, slot_
         return
     if not _native(cache.k):
         return kv_quant_append_ref(k, v, cache, slot_mapping)
-    _append(cache, None, k, v, slot_mapping, None, None, 0)
-
-
-def _append(cache, q, k, v, slots, positions, cos_sin, Hq) -> None:
-    nb, Hkv, bs, D = cache.dims
-    kernels().kv_append(cache.code, ptr(q), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slots.data_ptr(), ptr(positions),
-                        ptr(cos_sin), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), nb, k.shape[0], Hq, Hkv, D,
-                        bs, stream_ptr())
+    kernels().kv_append(cache.code, 0, kp, sk[0], vp, sv[0], slot_mapping.data_ptr(), 0, 0, cache.k.data_ptr(), cache.v.data_ptr(),
+                        cache.scales.data_ptr(), nb, T, 0, Hkv, D, bs, stream_ptr())
 
 
 def _check_cos_sin(cos_sin: torch.Tensor, cache: QuantKVCache) -> None:
@@ -283,7 +267,10 @@ def rope_kv_quant(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
         q = qkv[:, :num_heads * D].unflatten(1, (num_heads, D))
         q.copy_(_rotate(q.float(), cos, sin).to(qkv.dtype))
         return kv_quant_append_ref(_rotate(k.float(), cos, sin).to(torch.bfloat16), v, cache, slot_mapping)
-    _append(cache, qkv, k, v, slot_mapping, positions, cos_sin, num_heads)
+    nb, _, bs, _ = cache.dims
+    kernels().kv_append(cache.code, qkv.data_ptr(), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), slot_mapping.data_ptr(),
+                        positions.data_ptr(), cos_sin.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), nb, T,
+                        num_heads, H, D, bs, stream_ptr())
 
 
 def rope_kv_quant_partials(pend, positions: torch.Tensor, cos_sin: torch.Tensor, cache: QuantKVCache, slot_mapping: torch.Tensor,
@@ -326,17 +313,20 @@ def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch
     -> k, v [num_tokens, Hkv, D]. block_tables [S, W], starts [S], cu_tokens [S + 1] (from 0, not falling) int32; num_tokens =
     cu_tokens[S]. Tokens behind a sequence's table have no row: theirs stay as they were in `out`."""
     nb, Hkv, bs, D = cache.dims
-    S, index = starts.shape[0], cache.index
-    if not (_plain_table(block_tables, index, S) and _plain_lists(index, S, starts) and _plain_lists(index, S + 1, cu_tokens)
-            and num_tokens >= 0):
+    index, counts, table, steps = cache.index, starts.shape, block_tables.shape, block_tables.stride()
+    S = counts[0]
+    if not (len(counts) == 1 and len(table) == 2 and table[0] == S and table[1] > 0 and steps[1] == 1 and cu_tokens.shape == (S + 1,)
+            and starts.is_contiguous() and cu_tokens.is_contiguous() and block_tables.dtype is _I32 and starts.dtype is _I32
+            and cu_tokens.dtype is _I32 and block_tables.get_device() == index and starts.get_device() == index
+            and cu_tokens.get_device() == index and num_tokens >= 0):
         _int32(block_tables, "block_tables", 2, cache.device)
         _int32(starts, "starts", 1, cache.device)
         _int32(cu_tokens, "cu_tokens", 1, cache.device)
         _need(block_tables.shape[0] == S and cu_tokens.shape[0] == S + 1, "starts must have an entry a sequence, cu_tokens one more")
         _need(num_tokens >= 0, "num_tokens must not be negative")
-    W, shape = block_tables.shape[1], (num_tokens, Hkv, D)
+    W, shape = table[1], (num_tokens, Hkv, D)
     if out is None:
-        k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+        k = torch.empty_strided(shape, (Hkv * D, D, 1), dtype=_BF16, device=cache.device)   # (half of empty's host time)
         v = torch.empty_like(k)
     else:
         k, v = out
@@ -353,7 +343,7 @@ def kv_quant_read(cache: QuantKVCache, block_tables: torch.Tensor, starts: torch
                 k[a:a + n], v[a:a + n] = _rows_ref(cache, _slots_ref(block_tables[s], cache.block_size, lo, lo + n, cache.num_blocks))
         return k, v
     kernels().kv_read(cache.code, cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(), block_tables.data_ptr(),
-                      block_tables.stride()[0], W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens, nb, Hkv, D, bs,
+                      steps[0], W, starts.data_ptr(), cu_tokens.data_ptr(), S, num_tokens, nb, Hkv, D, bs,
                       k.data_ptr(), v.data_ptr(), stream_ptr())
     return k, v
 
@@ -373,8 +363,7 @@ def _check_q(q: torch.Tensor, Hkv: int, D: int, device) -> None:
 def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """The output, and the stride of its tokens."""
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        return out, out.stride()[0]
+        return torch.empty_like(q, memory_format=torch.contiguous_format), q.shape[1] * q.shape[2]
     if out.dtype != q.dtype:
         raise TypeError(f"out must be {q.dtype}, got {out.dtype}")
     _need(out.shape == q.shape and out.device == q.device, f"out must be {list(q.shape)} beside q")
@@ -392,14 +381,17 @@ def _check_tables(block_tables, seq_lens, device, S: int) -> None:
     _need(block_tables.shape[1] >= 1 or S == 0, "block_tables must have a column")
 
 
-def _check_decode(q, Hkv: int, D: int, index: int, device, block_tables, seq_lens) -> Tuple[int, int, int]:
-    """q, tables and lengths of a step with one new token of each sequence -> sequences, query heads, columns."""
-    (B, Hq, _), W = q.shape if q.dim() == 3 else (0, 0, 0), block_tables.shape[-1]
-    if not (_plain_heads(q, index, D, 8, 16) and Hq % Hkv == 0 < Hq and _plain_table(block_tables, index, B)
-            and _plain_lists(index, B, seq_lens)):
+def _check_queries(q, Hkv: int, D: int, index: int, device, block_tables, seq_lens, S: int) -> Tuple[int, int, int, int, int]:
+    """q, and tables and lengths of S sequences -> tokens, query heads, columns, strides of q's tokens and of the table's rows."""
+    shape, sq, table, st = q.shape, q.stride(), block_tables.shape, block_tables.stride()
+    if not (len(shape) == 3 and shape[2] == D == sq[1] and sq[2] == 1 and sq[0] % 8 == 0 and shape[1] % Hkv == 0 < shape[1]
+            and len(table) == 2 and table[0] == S and table[1] > 0 and st[1] == 1 and seq_lens.shape == (S,)
+            and seq_lens.is_contiguous() and q.dtype is _BF16 and block_tables.dtype is _I32 and seq_lens.dtype is _I32
+            and q.get_device() == index and block_tables.get_device() == index and seq_lens.get_device() == index
+            and q.data_ptr() % 16 == 0):
         _check_q(q, Hkv, D, device)
-        _check_tables(block_tables, seq_lens, device, B)
-    return B, Hq, W
+        _check_tables(block_tables, seq_lens, device, S)
+    return shape[0], shape[1], table[1], sq[0], st[0]
 
 
 def _splits(num_splits: Optional[int], wgs: int, max_keys: int) -> int:
@@ -428,7 +420,7 @@ def _shares(num_splits: Optional[int], B: int, wgs: int, max_keys: int) -> Tuple
 def _parts(workspace: Optional[DecodeWorkspace], parts: int, D: int, device):
     """The parts' buffer and the addresses of outputs [parts, D] and log-sums [parts] in it."""
     if workspace is None:
-        buf = torch.empty(parts * (D + 1), dtype=torch.float32, device=device)
+        buf = torch.empty_strided((parts * (D + 1),), (1,), dtype=torch.float32, device=device)
         at = buf.data_ptr()
         return buf, at, at + 4 * parts * D
     if workspace.part_lse.device != device or workspace.part_lse.numel() < parts or workspace.part_out.numel() < parts * D:
@@ -444,7 +436,7 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
     table means the whole table. num_splits: parts that a sequence's keys are cut into on average, more the longer it is; a workspace
     needs B num_splits of them (None: by the batch and the table's width, at most B + 512)."""
     (nb, Hkv, bs, D), dev = cache.dims, cache.device
-    B, Hq, W = _check_decode(q, Hkv, D, cache.index, dev, block_tables, seq_lens)
+    B, Hq, W, q_stride, t_stride = _check_queries(q, Hkv, D, cache.index, dev, block_tables, seq_lens, q.shape[0])
     out, out_stride = _check_out(out, q)
     blocks = -(-Hq // Hkv // 16)
     shares, least = _shares(num_splits, B, Hkv * blocks, W * bs)
@@ -461,8 +453,8 @@ def quant_decode_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: t
                 out[b] = _attend(q[b:b + 1], k, v, torch.tensor([L - 1], device=q.device), scale)[0].to(q.dtype)
         return out
     keep, po, pl = _parts(workspace, shares * Hq, D, dev) if shares > B else (None, 0, 0)
-    kernels().quant_decode_attention(cache.code, q.data_ptr(), q.stride()[0], cache.k.data_ptr(), cache.v.data_ptr(),
-                                     cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride()[0], W,
+    kernels().quant_decode_attention(cache.code, q.data_ptr(), q_stride, cache.k.data_ptr(), cache.v.data_ptr(),
+                                     cache.scales.data_ptr(), block_tables.data_ptr(), t_stride, W,
                                      seq_lens.data_ptr(), po, pl, out.data_ptr(), out_stride, B, Hq, Hkv, D, bs, nb, scale,
                                      shares, least, stream_ptr())
     return out
@@ -488,18 +480,15 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
     sweeps; None = `_row_tiles`): 1, 2 or 8."""
     (nb, Hkv, bs, D), dev, index = cache.dims, cache.device, cache.index
     S = seq_lens.shape[0]
-    if not (_plain_heads(q, index, D, 8, 16) and q.shape[1] % Hkv == 0 < q.shape[1] and _plain_table(block_tables, index, S)
-            and _plain_lists(index, S, seq_lens) and _plain_lists(index, S + 1, query_start_loc) and max_q_len >= 0):
-        _check_q(q, Hkv, D, dev)
-        _check_tables(block_tables, seq_lens, dev, S)
+    T, Hq, W, q_stride, t_stride = _check_queries(q, Hkv, D, index, dev, block_tables, seq_lens, S)
+    if not _plain_lists(index, S + 1, query_start_loc):
         _int32(query_start_loc, "query_start_loc", 1, dev)
         _need(query_start_loc.shape[0] == S + 1, "query_start_loc must have one entry more than seq_lens")
-        _need(0 <= max_q_len, "max_q_len must not be negative")
-    T, Hq, _ = q.shape
+    _need(0 <= max_q_len, "max_q_len must not be negative")
     out, out_stride = _check_out(out, q)
     if T == 0 or S == 0 or max_q_len == 0:
         return out
-    W, G = block_tables.shape[1], Hq // Hkv
+    G = Hq // Hkv
     max_q_len = min(max_q_len, T)
     rt = _row_tiles(max_q_len * G, S * Hkv) if row_tiles is None else row_tiles
     if rt not in (1, 2, 8):
@@ -517,8 +506,8 @@ def quant_prefill_attention(q: torch.Tensor, cache: QuantKVCache, block_tables: 
                 out[a:a + n] = _attend_causal(q[a:a + n], k, v, max(L - (b - a), 0), scale).to(q.dtype)
         return out
     keep, po, pl = _parts(workspace, T * Hq * splits, D, dev) if splits > 1 else (None, 0, 0)
-    kernels().quant_prefill_attention(cache.code, q.data_ptr(), q.stride()[0], cache.k.data_ptr(), cache.v.data_ptr(),
-                                      cache.scales.data_ptr(), block_tables.data_ptr(), block_tables.stride()[0], W,
+    kernels().quant_prefill_attention(cache.code, q.data_ptr(), q_stride, cache.k.data_ptr(), cache.v.data_ptr(),
+                                      cache.scales.data_ptr(), block_tables.data_ptr(), t_stride, W,
                                       query_start_loc.data_ptr(), seq_lens.data_ptr(), po, pl, out.data_ptr(), out_stride, T, S,
                                       max_q_len, Hq, Hkv, D, bs, nb, scale, rt, splits, stream_ptr())
     return out
@@ -532,6 +521,7 @@ class PrefixWork:
     slots: int                   # most parts that a prefix is cut into
     items: torch.Tensor          # [n, 8] int32: first sequence, sequences, block of rows, first key, end key, slot
     counts: torch.Tensor         # [num_seqs] int32: parts of each sequence's prefix
+    n: int                       # items
 
 
 @dataclass
@@ -571,7 +561,7 @@ def _prefix_work(sizes, lens, G: int, Hkv: int, rt: int, each: int, put) -> Pref
         counts += [parts] * n
         at += n
     _need(len(items) <= 65535, "too many groups")
-    return PrefixWork(rt, max(counts, default=0), put(items, (8,)), put(counts, ()))
+    return PrefixWork(rt, max(counts, default=0), put(items, (8,)), put(counts, ()), len(items))
 
 
 def shared_prefix_plan(group_sizes: Sequence[int], prefix_lens: Sequence[int], num_heads: int, num_kv_heads: int,
@@ -631,18 +621,18 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
         (nb, Hkv, bs, D), fmt = kc.shape, KV_BF16
         if D not in (64, 128) or bs < TILE or bs % TILE or nb < 1 or Hkv < 1:
             raise ValueError(f"heads of 64 or 128 numbers in pages of a multiple of {TILE} tokens")
-    dev = kc.device
-    B, Hq, W = _check_decode(q, Hkv, D, kc.get_device(), dev, block_tables, seq_lens)
+    dev, index = kc.device, kc.get_device()
+    B, Hq, W, q_stride, t_stride = _check_queries(q, Hkv, D, index, dev, block_tables, seq_lens, q.shape[0])
     if plan.num_seqs != B or plan.num_heads != Hq or plan.num_kv_heads != Hkv:
         raise ValueError(f"the plan is for {plan.num_seqs} sequences of {plan.num_heads} / {plan.num_kv_heads} heads, not {B} of {Hq} / {Hkv}")
-    if plan.prefix.device != dev or plan.longest > W * bs:
+    if plan.prefix.get_device() != index or plan.longest > W * bs:
         raise ValueError(f"the plan is on {plan.prefix.device}, the cache on {dev}" if plan.prefix.device != dev
                          else "a prefix is longer than the tables")
     out, out_stride = _check_out(out, q)
     blocks = -(-Hq // Hkv // 16)
     shares, least = _shares(num_splits, B, Hkv * blocks, W * bs - plan.shortest)
     work = plan.work if quant or plan.wide is None else plan.wide
-    if work.items.shape[0] + shares * blocks > 65535:
+    if work.n + shares * blocks > 65535:
         raise ValueError("at most 65535 parts (for each 16 query heads of a kv head)")
     if B == 0:
         return out
@@ -659,9 +649,9 @@ def shared_prefix_attention(q: torch.Tensor, kv: Union[QuantKVCache, Tuple[torch
             at += n
         return out
     keep, po, pl = _parts(workspace, (B * work.slots + shares) * Hq, D, dev) if work.slots or shares > B else (None, 0, 0)
-    kernels().shared_prefix_attention(fmt, q.data_ptr(), q.stride()[0], kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
-                                      block_tables.data_ptr(), block_tables.stride()[0], W, seq_lens.data_ptr(), po, pl,
+    kernels().shared_prefix_attention(fmt, q.data_ptr(), q_stride, kc.data_ptr(), vc.data_ptr(), ptr(kv.scales if quant else None),
+                                      block_tables.data_ptr(), t_stride, W, seq_lens.data_ptr(), po, pl,
                                       out.data_ptr(), out_stride, B, Hq, Hkv, D, bs, nb, scale, work.items.data_ptr(),
-                                      work.items.shape[0], plan.prefix.data_ptr(), work.counts.data_ptr(), work.slots,
+                                      work.n, plan.prefix.data_ptr(), work.counts.data_ptr(), work.slots,
                                       work.row_tiles, shares, least, stream_ptr())
     return out
