@@ -25,6 +25,12 @@ namespace xgk {
 constexpr float RAISE = 8.f;          // in base 2
 constexpr float LOWEST = -3.4e38f;    // the maximum of no key, below every score's: exp2(LOWEST - any) is 0
 
+// A row's weights are 2^(score - maximum - LIFT): their sum, and theirs times the values, stay below 2^127 for values of any size while
+// a wave has up to 2^16 keys 2^RAISE above the maximum (2^24 at it). Where the first keys' values (8-bit: their factors) are below 2^-64,
+// LIFT_SMALL: a weight times such a factor would be no normal bf16 number, or its product no normal float. A choice of a row's first
+// keys, so it costs nothing in the loop; later values may be as large as 2^50 then.
+constexpr float LIFT = 24.f, LIFT_SMALL = -48.f, SMALL = 0x1p-64f;
+
 struct RowsArgs {
   const uint16_t* q;
   int64_t q_stride;
@@ -96,6 +102,29 @@ __device__ __forceinline__ float join_groups(float v, F f) {
   return v;
 }
 
+// Whether numbers of the wave's lanes are not all zero and all below SMALL: of bf16, which order as whole numbers do ...
+struct Magnitudes {
+  typedef uint16_t pair_t __attribute__((ext_vector_type(2)));
+  pair_t top = {0, 0};
+  __device__ __forceinline__ void take(const uint4& x, bool in) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(pair_t, in ? w[i] & 0x7FFF7FFFu : 0u));
+  }
+  __device__ __forceinline__ bool usual() const { return __any(max(top[0], top[1]) >= __float_as_uint(SMALL) >> 16); }
+  __device__ __forceinline__ bool small() const { return !usual() && __any((top[0] | top[1]) != 0); }
+};
+
+// ... and of keys' factors (mostly the first look tells)
+template <int NA>
+__device__ __forceinline__ bool small_factors(const float4 (&vs)[NA]) {
+  if (__any(vs[0].x >= SMALL)) return false;
+  float v = 0.f;
+#pragma unroll
+  for (int a = 0; a < NA; ++a) v = fmaxf(fmaxf(fmaxf(v, vs[a].x), fmaxf(vs[a].y, vs[a].z)), vs[a].w);
+  return !__any(v >= SMALL) && __any(v > 0.f);
+}
+
 template <int FMT, int D, int RT>
 struct RowsCfg {
   static constexpr bool WIDE = FMT == KV_BF16;
@@ -111,11 +140,11 @@ struct RowsCfg {
 // Products q k of 32 keys -> scores less their rows' running maxima, which rise (and sums and outputs shrink) where a score is more
 // than RAISE above its row's. ks, vs: the keys' and values' factors (SCALED: the keys' times softmax's scale). EDGE: some row does not
 // see some key of the 32 from key0 on: its score becomes -inf. A value that is not finite then reaches the rows that see it by their
-// scores, and no other by its factor (bf16: add_odd).
-template <bool EDGE, bool WIDE, bool SCALED, int NA, int RT, int MT>
+// scores, and no other by its factor (bf16: add_odd). small(): whether these keys' values (factors) are below SMALL.
+template <bool EDGE, bool WIDE, bool SCALED, int NA, int RT, int MT, typename F>
 __device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[NA], float4 (&vs)[NA], float scale, int key0, int kbeg,
                                        int kend, const int (&limit)[RT], float (&m)[RT], float (&l)[RT], float (&high)[RT],
-                                       f32x4_t (&acc)[RT][MT]) {
+                                       f32x4_t (&acc)[RT][MT], F small) {
   float top[RT];
   bool raise = false;
 #pragma unroll
@@ -159,12 +188,21 @@ __device__ __forceinline__ void scores(f32x4_t (&s)[NA][RT], const float4 (&ks)[
     raise = raise || top[rt] > high[rt];
   }
   if (__any(raise)) {
+    bool none = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) none = none || high[rt] == -INFINITY;
+    const float lift = __any(none) && small() ? LIFT_SMALL : LIFT;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const bool first = high[rt] == -INFINITY;
       float up = join_groups(top[rt], [](float x, float y) { return fmaxf(x, y); });
-      if (first) high[rt] = up == -INFINITY ? up : RAISE;
-      up = first && up != -INFINITY ? up : fmaxf(up, 0.f);
+      if (first) {   // (maxima that would lose the lift in rounding have none: m is what the weights are relative to)
+        const float on = fabsf(up) < 0x1p20f ? lift : 0.f;
+        high[rt] = up == -INFINITY ? up : RAISE - on;
+        up = up == -INFINITY ? 0.f : up + on;
+      } else {
+        up = fmaxf(up - (high[rt] - RAISE), 0.f);
+      }
       const float alpha = first ? 1.f : exp2_fast(-up);
       m[rt] += up;
       l[rt] *= alpha;
@@ -426,7 +464,23 @@ __device__ __forceinline__ void attend_rows(const RowsArgs& p, const RowsBlock w
   // scores of tile t, whose V is in registers; bf16: its odd rows
   auto judge = [&](int t, f32x4_t (&s)[2][RT], const float4 (&factors)[2], auto edge) {
     uint32_t odd = 0;
-    scores<decltype(edge)::value, C::WIDE, false, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, end, limit, m, l, high, acc);
+    auto small = [&]() {
+      if constexpr (C::WIDE) {
+        Magnitudes x;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int i = 0; i < C::LOADS; ++i) {
+            const int key = 32 * t + 16 * a + (lane + 64 * i) / (D / 8);
+            x.take(vr[a][i], key >= w.kbeg && key < end);
+            if (a == 0 && i == 0 && x.usual()) return false;
+          }
+        return x.small();
+      } else {
+        return small_factors(vs);
+      }
+    };
+    scores<decltype(edge)::value, C::WIDE, false, 2, RT, C::MT>(s, factors, vs, p.scale, 32 * t, w.kbeg, end, limit, m, l, high, acc, small);
     if constexpr (decltype(edge)::value) {   // V of keys outside the range: anything (E4M3's NaN too), so zeros
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
@@ -736,7 +790,20 @@ __device__ __forceinline__ void attend_block(const RowsArgs& p, const RowsBlock 
           vs[a] = *reinterpret_cast<const float4*>(sd + C::KEYS + 16 * a);
         }
       }
-      scores<decltype(edge)::value, C::WIDE, true, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, kend, limit, m, l, high, acc);
+      auto small = [&]() {
+        if constexpr (C::WIDE) {
+          Magnitudes x;
+#pragma unroll
+          for (int i = 0; i < C::SIDE / 1024; ++i) {   // (zeros outside the range)
+            x.take(ld16(vd + (lane + 64 * i) * 16), true);
+            if (i == 0 && x.usual()) return false;
+          }
+          return x.small();
+        } else {
+          return small_factors(vs);
+        }
+      };
+      scores<decltype(edge)::value, C::WIDE, true, 4, C::RT, C::MT>(s, ks, vs, p.scale, key0, w.kbeg, kend, limit, m, l, high, acc, small);
       bf16x8_t pf[2][C::RT];
       weights<C::WIDE, 4, C::RT>(s, vs, l, pf);
       if constexpr (C::WIDE && decltype(edge)::value) {
@@ -962,7 +1029,7 @@ __global__ void __launch_bounds__(256, 3) rows_decode_kernel(RowsArgs p, int B, 
 
 // Prompt portions, causal. Grid (Hkv, blocks of rows of the longest, sequences splits). Late blocks see the most keys: first.
 template <int FMT, int D, int RT>
-__global__ void __launch_bounds__(256, RT <= 1 ? 3 : 2) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
+__global__ void __launch_bounds__(256, RT <= 1 || D == 64 ? 3 : 2) rows_prompt_kernel(RowsArgs p, const int32_t* qsl, int tokens, int splits) {
   const int s = blockIdx.z / splits;
   RowsBlock w;
   w.tok0 = min(max(qsl[s], 0), tokens);
@@ -1025,7 +1092,8 @@ __global__ void __launch_bounds__(256, RT == 1 && !(FMT == KV_BF16 && D == 128) 
 // Joins a row's parts: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M). They are the first counts[token] (null: all) of the
 // row's `slots`, and, of `shares`, its sequence's; rows of one part are in `out` already. qsl: tokens outside [qsl[0], qsl[S]) have
 // none. A workgroup has ROWS rows of a token, four dims a thread, and 4 x 1024 / (D ROWS) parts of a row on their way at once: one row
-// where there are few (72 rows of 57 parts took 8.3 us with D / 4 threads a row), four where workgroups would only queue.
+// where there are few (72 rows of 57 parts took 8.3 us with D / 4 threads a row), four where workgroups would only queue. Factors are
+// 2^-8 of these at most: up to 256 parts' sums of the largest numbers stay numbers.
 struct JoinArgs {
   const int32_t* counts;
   int slots;
@@ -1076,7 +1144,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(RowsArgs p, JoinArgs j) 
     o = make_float4(o.x * old, o.y * old, o.z * old, o.w * old);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const float f = exp2_fast(e[a] - M);
+      const float f = exp2_fast(e[a] - M - 8.f);
       sum += f;
       o = make_float4(o.x + f * x[a].x, o.y + f * x[a].y, o.z + f * x[a].z, o.w + f * x[a].w);
     }

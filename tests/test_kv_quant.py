@@ -450,6 +450,49 @@ def test_scores_further_down_than_any_mask(dev, fmt, D, exact):
 
 
 @DEVICES
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("first,power", [(-122, -122), (-60, -60), (126, 126), (-110, 40), (0, 126), (126, 0)])
+def test_values_of_any_size(dev, fmt, D, first, power):
+    """Values of up to 2^(power + 1) (those of a sequence's first 200 tokens: 2^(first + 1)), next to the largest number of bf16 and to the smallest normal one: what is summed is the weights times
+    these, and no part of it may leave its type's range where the output does not. Both sides times 2^-power (the output is linear in
+    the values); below 2^-126 an output's rounding is half of bf16's smallest number, 2^-134, and an fp32 scale's 2^-150 for a code of up to
+    448."""
+    gen = torch.Generator().manual_seed(24)
+    lens, Hq, unit = [700, 33, 1, 300, 90], 8, 2.0 ** -max(first, power)
+
+    def fill(k, v):
+        size = torch.cat([torch.where(torch.arange(n) < 200, 2.0 ** first, 2.0 ** power) for n in lens])[:, None, None]
+        v.copy_(v.double().div(v.abs().amax(-1, keepdim=True)).mul(1.5 * size).abs())
+
+    cache, table, truth = make(lens, 2, D, 16, fmt, dev, gen, fill)
+    q = rows(len(lens), Hq, D, gen).to(dev)
+    assert all(bool((v.abs().amax(-1) >= 1.49 * 2.0 ** min(first, power)).all()) for _, v in truth)
+
+    def hold(out, seen, s):
+        k, v = truth[s]
+        ref, bound = attention(q[s:s + 1].double().cpu(), k, v * unit, [seen], 0.1)
+        got = out.double().cpu() * unit
+        check(got, ref, bound + (2.0 ** -134 + 448 * 2.0 ** -150) * unit * 1.01)
+
+    ln = i32(lens, dev)
+    plan = ops.shared_prefix_plan([1] * len(lens), [640, 32, 0, 0, 64], Hq, 2, dev)
+    outs = [ops.shared_prefix_attention(q, cache, table, ln, plan, 0.1, num_splits=n) for n in (1, 5)]
+    if fmt == "bf16":
+        wide = ops.shared_prefix_plan([1] * len(lens), [640, 32, 0, 0, 64], Hq, 2, dev)
+        wide.wide = kv_quant._prefix_work([1] * len(lens), [640, 32, 0, 0, 64], Hq // 2, 2, 8, 4,
+                                          lambda r, w: torch.tensor(r, dtype=torch.int32).reshape(-1, *w).to(dev))
+        outs.append(ops.shared_prefix_attention(q, cache, table, ln, wide, 0.1))
+    else:
+        outs += [ops.quant_decode_attention(q, cache, table, ln, 0.1, num_splits=n) for n in (1, 3)]
+        outs += [ops.quant_prefill_attention(q, cache, table, i32(list(range(len(lens) + 1)), dev), ln, 1, 0.1, num_splits=n, row_tiles=rt)
+                 for n, rt in ((1, 1), (1, 2), (1, 8), (3, 8))]
+    for out in outs:
+        for s, L in enumerate(lens):
+            hold(out[s:s + 1], L, s)
+
+
+@DEVICES
 @FORMATS
 def test_portions_longer_than_their_sequences(dev, fmt):
     """Lengths below a portion's tokens, and below zero: the first token sees the first key, and none sees more than there are."""
