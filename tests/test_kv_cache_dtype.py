@@ -159,3 +159,14 @@ def test_engine_on_the_gpu(fmt):
         for i, tok in enumerate(o):
             row = ref[len(p) - 1 + i]
             assert float(row.max() - row[tok]) <= 0.5 * float(row.std())
+
+
+@pytest.mark.gpu
+def test_no_workspace_that_nothing_uses():
+    """An engine on an 8-bit cache holds its pages, and no buffer for the parts of the bf16 cache's decode attention."""
+    held = {}
+    for fmt in (None, "fp8"):
+        r = _engine(fmt, device="cuda:0", max_num_seqs=64).runner
+        held[fmt] = r.workspace
+        assert (r.kv_quant is None) == (fmt is None)
+    assert held[None] is not None and held["fp8"] is None

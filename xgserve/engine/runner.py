@@ -144,8 +144,10 @@ class ModelRunner:
         self.is_cuda = self.device.type == "cuda"
         Hq_local = cfg.num_heads // model.tp
         self.max_splits = tune.get_int("decode_max_splits", 16)
+        # (the 8-bit cache's attention shares a batch's keys out by itself and has its parts' buffer from the step's memory:
+        # neither the workspace nor decode_max_splits is for it)
         self.workspace = DecodeWorkspace(max(max_num_seqs, 1), Hq_local, cfg.head_dim, self.max_splits,
-                                         self.device) if (self.is_cuda and not hasattr(model, "alloc_cache")) else None
+                                         self.device) if (self.is_cuda and self.kv is not None) else None
         # pinned staging for eager steps
         cap = 9 * max_num_batched_tokens + 4 * max_num_seqs * (self.max_blocks_per_seq + 6) + 64
         # two pinned host staging buffers + device twins: a step may return

@@ -20,7 +20,7 @@ Keys (default in brackets; every default is the production setting):
   mw_max_tokens [320]      largest step on gemm_mw
   resid_inlaunch_kb [32]   in-launch residual reduce bound of the fused decode GEMMs
   decode_depth [2]         decode attention K/V register pipeline depth (4: depth 2 with the classic QKV prologue)
-  decode_max_splits [16]   split-K cap of decode attention
+  decode_max_splits [16]   split-K cap of decode attention (bf16 cache)
   gemm_ar [1]              TP decode: all-reduce inside the row-parallel O / down GEMM launches
   gemm_ar_shared [0]       test-only: GG_AR also for <= 4 ranks sharing one GPU (one-GPU boxes)
   small_m_tiles [128]      column-tile statistics a M <= 16 consumer combines (64: pair combine above)
