@@ -1,5 +1,7 @@
 """The engine on an 8-bit KV cache: the attention layer on it, whole generations, prefix pages, sizes and refusals."""
 import math
+import os
+import socket
 from dataclasses import replace
 
 import pytest
@@ -170,3 +172,76 @@ def test_no_workspace_that_nothing_uses():
         held[fmt] = r.workspace
         assert (r.kv_quant is None) == (fmt is None)
     assert held[None] is not None and held["fp8"] is None
+
+
+PROMPTS = [[1] + list(range(20, 60)), [1, 5, 6, 7, 8], [1] + list(range(20, 52)) + [7, 8]]
+
+
+def _near_the_top(model, prompts, outs):
+    """As test_engine_on_the_gpu: each token within half a deviation of the fp32 model's logits on the same tokens."""
+    from xgserve.models.reference import reference_logits
+    for p, o in zip(prompts, outs):
+        ref = reference_logits(model, p + o[:-1]).float()
+        for i, tok in enumerate(o):
+            row = ref[len(p) - 1 + i]
+            assert tok < len(row) and float(row.max() - row[tok]) <= 0.5 * float(row.std())
+
+
+@FORMATS
+@pytest.mark.parametrize("name", ["llama-tiny", "mixtral-tiny", "gpt2-tiny"])
+def test_families(fmt, name):
+    """Whole generations of each family that is served from the 8-bit cache, prompts whole and by portions."""
+    sp = SamplingParams(max_tokens=6, temperature=0.0, ignore_eos=True)
+    eng = _engine(fmt, model=name)
+    outs = eng.generate(PROMPTS, sp)
+    assert [len(o) for o in outs] == [6, 6, 6]
+    assert all(isinstance(c, ops.QuantKVCache) and c.fmt == fmt and bool((c.scales > 0).any()) for c in eng.runner.kv_caches)
+    _near_the_top(eng.model, PROMPTS, outs)
+    _near_the_top(eng.model, PROMPTS, _engine(fmt, model=name, max_num_batched_tokens=16).generate(PROMPTS, sp))
+
+
+def _rank(rank, world, port, ck, fmt, q):
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank), MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.set_num_threads(1)
+    try:
+        from xgserve.parallel.state import destroy_distributed, init_distributed
+        init_distributed(tp_size=world, backend="gloo", device=torch.device("cpu"), timeout_s=120)
+        eng = _engine(fmt, model="llama-tiny-gqa8", checkpoint=ck, tp=world, max_model_len=256)
+        outs = None
+        if rank == 0:
+            outs = eng.generate(PROMPTS, SamplingParams(max_tokens=6, temperature=0.0, ignore_eos=True))
+            eng.stop_followers()
+        else:
+            eng.follower_loop()
+        c = eng.runner.kv_caches[0]
+        q.put((rank, None, outs, (c.fmt, c.num_kv_heads, bool((c.scales > 0).any()))))
+        destroy_distributed()
+    except Exception as e:  # noqa: BLE001 - reported to the parent
+        q.put((rank, repr(e), None, None))
+
+
+@FORMATS
+def test_ranks_of_a_group(fmt, tmp_path):
+    """Two ranks, each with an 8-bit cache of its own kv heads."""
+    from xgserve.models import save_checkpoint
+    full = build_model(get_config("llama-tiny-gqa8"), device="cpu", dtype=torch.bfloat16, seed=11)
+    ck = str(tmp_path / "ckpt")
+    save_checkpoint(full, ck)
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = torch.multiprocessing.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, 2, port, ck, fmt, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    try:
+        res = {r[0]: r[1:] for r in (q.get(timeout=240) for _ in procs)}
+    finally:
+        for p in procs:
+            p.join(timeout=60)
+            if p.is_alive():
+                p.kill()
+    assert [res[r][0] for r in (0, 1)] == [None, None]
+    assert [res[r][2] for r in (0, 1)] == [(fmt, full.cfg.num_kv_heads // 2, True)] * 2
+    _near_the_top(full, PROMPTS, res[0][1])
