@@ -1135,7 +1135,10 @@ __global__ void __launch_bounds__(256) rows_join_kernel(RowsArgs p, JoinArgs j) 
     }
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      if (i0 + a * OF_ROW >= n) e[a] = -INFINITY;
+      if (i0 + a * OF_ROW >= n) {   // (read once more: 0 times an infinity of it would be NaN)
+        e[a] = -INFINITY;
+        x[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
       top = fmaxf(top, e[a]);
     }
     const float old = exp2_fast(M - top);

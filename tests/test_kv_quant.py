@@ -645,6 +645,29 @@ def test_a_value_that_is_not_finite_reaches_only_those_who_see_it(dev, fmt, D, H
         check(got[good], ref[good], bound[good])
 
 
+@DEVICES
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5])
+def test_an_infinity_in_any_part(dev, D, splits):
+    """bf16: a part of a row's keys whose output is infinite, the first, one in the midst or the last of 2 to 6."""
+    gen = torch.Generator().manual_seed(26)
+    lens, at = [700] * 6, [0, 70, 199, 300, 500, 699]
+
+    def fill(k, v):
+        for s, x in enumerate(at):
+            v[700 * s + x, s % 2, 5] = math.inf * (1 - 2 * (s % 3 == 0))
+
+    cache, table, truth = make(lens, 2, D, 16, "bf16", dev, gen, fill)
+    q = rows(6, 8, D, gen).to(dev)
+    plan = ops.shared_prefix_plan([1] * 6, [128] * 6, 8, 2, dev)
+    out = ops.shared_prefix_attention(q, cache, table, i32(lens, dev), plan, 0.1, num_splits=splits)
+    for s in range(6):
+        ref, bound = attention(q[s:s + 1].double().cpu(), *truth[s], [700], 0.1)
+        got, good = out[s:s + 1].double().cpu(), ref.isfinite()
+        assert int((~good).sum()) == 4 and torch.equal(got[~good], ref[~good])
+        check(got[good], ref[good], bound[good])
+
+
 def test_work_of_a_plan():
     """Every (block of rows, 32 keys) of every group is in one item, in blocks of either size."""
     sizes, prefixes, G, Hkv = [40, 1, 9, 3], [30000, 0, 9001, 31], 4, 8
