@@ -359,6 +359,49 @@ def test_decode_of_batches_of_any_lengths(dev, fmt, B, splits):
     assert torch.equal(out, same)
 
 
+@pytest.mark.gpu
+@FORMATS
+@pytest.mark.parametrize("lens,W,shares", [
+    ([(i * 53) % 300 for i in range(120)] + [4000] + [(i * 71) % 280 for i in range(79)], 4096, (400, 16)),   # one is cut
+    ([(i * 211) % 2048 for i in range(200)], 4096, (400, 16)),                                                # none is
+    ([2049] * 200, 4096, (400, 16)),                                                                          # all are: 17 units each
+    ([20000], 20000, (158, 1)), ([16385, 5], 16400, (260, 1))])   # parts at their limit (2 + 2 x ceil(16400 / 128) shares)
+def test_decode_where_the_rule_cuts(fmt, lens, W, shares):
+    """Automatic shares of wide tables: batches that fill the chip leave sequences of up to 2048 keys whole; 128 parts at most."""
+    gen = torch.Generator().manual_seed(len(lens))
+    B = len(lens)
+    assert kv_quant._shares(None, B, 1, W) == shares
+    cache, table, truth = make(lens, 1, 64, 16, fmt, "cuda", gen)
+    table = torch.cat([table, table.new_full((B, -(-W // 16) - table.shape[1]), cache.num_blocks - 1)], 1)
+    q = rows(B, 4, 64, gen).to("cuda")
+    out = ops.quant_decode_attention(q, cache, table, i32(lens, "cuda"), 0.125)
+    for s in range(B) if B < 100 else [0, 1, 63, 64, 119, 120, 121, 127, 128, 192, 198, 199]:
+        check(out[s:s + 1], *attention(q[s:s + 1].double().cpu(), *truth[s], [lens[s]], 0.125))
+
+
+@pytest.mark.gpu
+@FORMATS
+def test_prompts_where_the_rule_cuts(fmt):
+    """Automatic parts of a short portion behind many keys, and automatic blocks of 128 rows."""
+    gen = torch.Generator().manual_seed(27)
+    for Hq, Hkv, new, ctx, cut in ((8, 1, [37, 5], [1500, 0], True), (24, 12, [1900, 1850, 300], [0, 17, 90], False)):
+        lens = [a + b for a, b in zip(new, ctx)]
+        cache, table, truth = make(lens, Hkv, 64, 16, fmt, "cuda", gen)
+        rt = kv_quant._row_tiles(max(new) * Hq // Hkv, len(new) * Hkv)
+        blocks = -(-max(new) * (Hq // Hkv) // (16 * rt))
+        splits = kv_quant._splits(None, len(new) * Hkv * blocks, table.shape[1] * 16)
+        assert (splits > 1 and rt < 8) if cut else (splits == 1 and rt == 8)
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        q = rows(cu[-1], Hq, 64, gen).to("cuda")
+        out = ops.quant_prefill_attention(q, cache, table, i32(cu, "cuda"), i32(lens, "cuda"), max(new), 0.125)
+        for s, n in enumerate(new):
+            for i in sorted({0, 1, n // 3, n // 2, n - 2, n - 1}):
+                at = slice(cu[s] + i, cu[s] + i + 1)
+                check(out[at], *attention(q[at].double().cpu(), *truth[s], [ctx[s] + i + 1], 0.125))
+
+
 @DEVICES
 def test_decode_into_a_strided_output_with_a_workspace(dev):
     gen = torch.Generator().manual_seed(2)
@@ -643,6 +686,49 @@ def test_a_value_that_is_not_finite_reaches_only_those_who_see_it(dev, fmt, D, H
         assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got[ref.isinf()], ref[ref.isinf()])
         good = ref.isfinite()
         check(got[good], ref[good], bound[good])
+
+
+@DEVICES
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("Hq,D,sizes,rt", [(8, 128, [3, 2], 1), (8, 64, [4, 2], 1), (12, 128, [9, 2], 2), (40, 64, [5, 2], 2),
+                                           (8, 128, [33, 3], 8), (8, 64, [33, 3], 8)])
+def test_many_tiles_of_a_shared_prefix(dev, fmt, Hq, D, sizes, rt, monkeypatch):
+    """Workgroups with far more 32-key tiles than waves, of common and own keys: tiles that all rows see, then those behind the end of
+    the group's shortest sequence, in whose midst is an infinity that some see; the second group has whole tiles only."""
+    monkeypatch.setattr(kv_quant, "PREFIX_WGS", 4)
+    wide = rt == 8
+    monkeypatch.setattr(kv_quant, "WIDE_ROWS", 0 if wide else 1 << 30)
+    monkeypatch.setattr(kv_quant, "WIDE_TILES", 0)
+    gen = torch.Generator().manual_seed(25)
+    prefixes, at = ([1500, 900], 777) if wide else ([3000, 1700], 1777)
+    tails = [[600, 1] + [45] * (sizes[0] - 2), [500] + [3] * (sizes[1] - 1)]
+
+    def fill(k, v):
+        v[at - 1, 0, 3] = math.inf
+        v[at + 40, 1, D - 1] = -math.inf
+        v[at + 300, 1, 7] = math.nan
+        v[prefixes[0] + 580, 0, 5] = math.inf
+
+    cache, table, lens, seqs = groups_of(sizes, prefixes, tails, 2, D, 16, fmt, dev, gen, fill)
+    short = list(lens)
+    short[1:3] = [at, at + 41]
+    q = rows(len(lens), Hq, D, gen).to(dev)
+    plan = ops.shared_prefix_plan(sizes, prefixes, Hq, 2, dev)
+    assert plan.work.row_tiles == (1 if sizes[0] * Hq // 2 <= 16 else 2) and (plan.wide is not None) == wide
+    if wide and fmt == "bf16":
+        assert plan.wide.row_tiles == 8
+    for work in (plan.work, plan.wide) if wide else (plan.work,):
+        assert max(it[4] - it[3] for it in work.items.tolist()) > 16 * 32
+    out = ops.shared_prefix_attention(q, cache, table, i32(short, dev), plan, 0.1, num_splits=1)
+    cut = ops.shared_prefix_attention(q, cache, table, i32(short, dev), plan, 0.1, num_splits=3)
+    for s in [0, 1, 2, sizes[0] - 1] + list(range(sizes[0], len(lens))):
+        ref, bound = attention(q[s:s + 1].double().cpu(), *seqs[s], [short[s]], 0.1)
+        good = ref.isfinite()
+        assert good.all() == (s >= sizes[0])
+        for o in (out, cut):
+            got = o[s:s + 1].double().cpu()
+            assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got[ref.isinf()], ref[ref.isinf()])
+            check(got[good], ref[good], bound[good])
 
 
 @DEVICES
