@@ -10,7 +10,9 @@
 //     it by more than 2^8: fp32 sums and bf16 weights are relative, so weights up to 2^8 cost no precision
 //   O^T[D][16 rows] += V^T P^T      the same instruction over 32 keys. The S^T accumulators are the P^T fragment where
 //     the 8 keys of lane group g are 4 g + {0..3} of both 16-key halves; the cache holds V in that order (bf16: V is
-//     turned through LDS). V's scale joins the weight before its rounding to bf16 (2^-8 of it at most, as everywhere here)
+//     turned through LDS). V's scale joins the weight before its rounding to bf16, half a step of 2^-8 at most: the instruction's
+//     other operand has to be bf16 too. An output's error, its own rounding's 1.6e-3 in root mean square of itself, becomes 2.0 to
+//     2.4e-3 by it (32-bit weights, which would need a second product for their rest, 1.6 to 1.8e-3)
 // The waves' states join through LDS, parts of a row's keys through rows_join_kernel: (O / l, log2-sum-exp) in fp32.
 //
 // Waves share no tile, so the key loop has no barrier, and K / V go from HBM to registers: one tile's loads are on their
@@ -880,8 +882,10 @@ __device__ __forceinline__ void share(int& kbeg, int& kend, int split, int split
 // A batch's sequences are of any lengths, which the host does not know, so the keys are shared out here: of `shares` workgroups a kv
 // head (and block of 16 query heads) each takes up to `run` units of 128 keys (a 32-key tile a wave) of one sequence, with run the
 // batch's units over shares - B, and `least` where none has more: a short search, for share i is sequence i then (256 sequences of
-// 300 - 900 keys 71 -> 68 us). So a sequence has ceil(units / run) parts, at least one, and all have shares at most. (With as many
-// parts for each sequence the longest one bounds the step: 1 sequence of 60 k keys beside 63 of 500, fp8, took 423 us, and takes 42.)
+// 300 - 900 keys 71 -> 68 us). So a sequence has ceil(units / run) parts, at least one and MAX_PARTS at most (the join's factors leave
+// room for 256 with those of the common keys), and all have shares at most. (With as many parts for each sequence the longest one
+// bounds the step: 1 sequence of 60 k keys beside 63 of 500, fp8, takes 428 us whole and 41 so.) The limit leaves CUs idle where few
+// long sequences have one kv head: 1 of 131072 keys, 8 / 1 heads of 128, fp8, 17.7 us for a floor of 7.3, 2 20.4 for 14.5.
 constexpr int MAX_PARTS = 128;
 
 template <int CTRL, int ROWS>
