@@ -277,7 +277,8 @@ template <int FMT, int D>
 static void launch_append(const KvAppend& p, int from, hipStream_t st) {
   const dim3 grid((p.T + 15) / 16, p.Hkv + (from != KV_ROWS ? p.Hq : 0));
   // two heads a wave from 16 k rows on: half the waves, each with twice the loads on their way, 14.5 -> 11.5 us for 8192 tokens of 8
-  // heads and 46 -> 34 (6 TB/s) for 32768; 4.0 for 3.5 with 64 tokens, where they are too few
+  // heads and 46 -> 34 (6 TB/s) for 32768, the same rows each time (in turn with others 11.8 and 42); 4.0 for 3.5 with 64 tokens, where
+  // they are too few
   if (from == KV_PARTS) hipLaunchKernelGGL((kv_append_kernel<FMT, D, KV_PARTS, 1>), grid, dim3(256), 0, st, p);
   else if (from == KV_ROPE) hipLaunchKernelGGL((kv_append_kernel<FMT, D, KV_ROPE, 1>), grid, dim3(256), 0, st, p);
   else if (p.Hkv % 2 == 0 && static_cast<int64_t>(p.T) * p.Hkv >= 16384)

@@ -35,8 +35,8 @@ KV_FORMATS = {"fp8": KV_FP8, "int8": KV_INT8}
 LARGEST = {"fp8": 448.0, "int8": 127.0}
 TILE = 16           # tokens whose codes lie together in the order of the matrix instructions (csrc/kernels/kv_quant.h)
 MAX_SPLITS = 64
-# us of decode, one part / the parts that this makes: 1 sequence of 640 keys 6.0 / 6.5, 1280 8.5 / 6.9, 5120 35.7 / 8.9; 16 of 640
-# 8.5 / 9.4, 5120 48.8 / 30.5; 48 of 1280 25.2 / 25.4 (8 kv heads of 128). Below SPLIT_FROM keys a second launch costs more
+# us of decode, one part / the parts that this makes: 1 sequence of 640 keys 5.9 / 7.7, 1280 8.2 / 7.9, 5120 36 / 10.3; 16 of 640
+# 8.9 / 11.7, 5120 44 / 35; 48 of 1280 24.6 / 32.6 (8 kv heads of 128, fp8). Below SPLIT_FROM keys a second launch costs more
 SPLIT_WGS = 512     # workgroups that fill the chip: two a CU
 SPLIT_KEYS = 128    # a workgroup's four waves have a 32-key tile each
 WHOLE_UNITS = 16    # units of SPLIT_KEYS that stay whole where the sequences alone fill most of the chip
